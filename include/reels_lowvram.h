@@ -331,6 +331,92 @@ int reels_gated_residual_backward(const void *dout, const void *y, const void *g
                                   void *workspace, size_t ws_bytes, void *stream);
 
 /* ---------------------------------------------------------------------
+ * The block's attention stretch, between the q/k/v projections and the
+ * output projection: the norm of q and k with the video's rotary positions,
+ * and softmax attention, each with its pullback. */
+
+/* Rotary positions of a video's tokens: time, height, width.
+ * `table` holds, axis after axis, [size[a]][dim[a] / 2] pairs (cos, sin) of
+ * the angles at that axis's positions 0 .. size[a] - 1; the axes' features
+ * sum to head_dim, and feature pair i of a head belongs to the axis whose
+ * pairs hold it (time first).  A model with fewer axes gives the others
+ * dim 0 and size 1.
+ * Without `positions`, token i of a sample is at (t, h, w) in raster order
+ * (width fastest) and tokens behind the grid are padding.  With it, row m is
+ * at positions[m][0..2]; a negative one marks padding.  Padding is normed and
+ * not turned; so is a token with a position behind its table, which also
+ * sets a bit of the device status. */
+#define REELS_ROPE_INTERLEAVED 0 /* pair i of a head: features 2 i and 2 i + 1 */
+#define REELS_ROPE_HALF 1        /* pair i of a head: features i and i + head_dim / 2 */
+typedef struct reels_rope {
+    const float *table;       /* device, 8-byte aligned */
+    const int32_t *positions; /* device [M][3], or NULL */
+    int32_t size[3];
+    int32_t dim[3];
+    int32_t pairing;
+} reels_rope;
+
+/* out = R(x / sqrt(mean(x^2) + epsilon) * weight), one pass per row of
+ * x [M][heads * head_dim]: the norm spans all heads of a token, weight
+ * [heads * head_dim] is nullable, rope is nullable (the norm alone, as for
+ * the cross-attention's q and k).  Computed in fp32 and rounded once; out may
+ * be x.  heads * head_dim <= 16384.  `tokens_per_sample`: where the raster
+ * order starts again. */
+int reels_rms_norm_rope(const void *x, int64_t M, int64_t heads, int64_t head_dim, const void *weight,
+                        const reels_rope *rope, int64_t tokens_per_sample, float epsilon, int act_dtype, void *out,
+                        void *stream);
+
+/* Its pullback: dx for dout, both [M][heads * head_dim]; dx may be dout or x.
+ * The weight is frozen and receives no gradient. */
+int reels_rms_norm_rope_backward(const void *x, const void *dout, int64_t M, int64_t heads, int64_t head_dim,
+                                 const void *weight, const reels_rope *rope, int64_t tokens_per_sample, float epsilon,
+                                 int act_dtype, void *dx, void *stream);
+
+/* q [batch][q_tokens][heads][head_dim] and k, v [batch][k_tokens][kv_heads]
+ * [head_dim] by strides (batch, token, head; in elements; the features of a
+ * head are contiguous), so that parts of a fused projection are read in
+ * place.  heads is a multiple of kv_heads: query head h reads key head
+ * h / (heads / kv_heads).  head_dim <= 256.
+ * 16-bit tensors with head_dim a multiple of 8 up to 128, 16-byte aligned
+ * pointers and positive strides in multiples of 8 run on the tcgen05 path;
+ * every other case runs on CUDA-core kernels. */
+typedef struct reels_attn_shape {
+    int64_t batch, heads, kv_heads, q_tokens, k_tokens, head_dim;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+} reels_attn_shape;
+
+/* Bytes of scratch of a forward or backward call (REELS_PASS_FORWARD,
+ * REELS_PASS_BACKWARD).  0 for a shape that the calls refuse. */
+size_t reels_attention_workspace_bytes(const reels_attn_shape *shape, int act_dtype, int pass);
+
+/* The plan for aligned pointers, for diagnostics and tests; no device work.
+ * info[0] path, info[1] key splits of the forward, info[2] keys per split,
+ * info[3] splits of the walk over the queries for dk and dv. */
+int reels_attention_plan(const reels_attn_shape *shape, int act_dtype, int64_t *info);
+
+/* out = softmax(scale q k') v over all keys of the sample, and
+ * lse = log sum exp(scale q k') (natural logarithm, fp32).
+ * out [batch][q_tokens][heads][head_dim] and lse [batch][heads][q_tokens] are
+ * contiguous.  kv_lengths (device int32 [batch], nullable): keys at and
+ * behind a sample's length take no part, whatever they hold; values outside
+ * 0 .. k_tokens are clamped.  A sample without keys has out 0 and
+ * lse -infinity.  scale > 0. */
+int reels_attention_forward(const reels_attn_shape *shape, const void *q, const void *k, const void *v,
+                            const int32_t *kv_lengths, float scale, int act_dtype, void *out, float *lse,
+                            void *workspace, size_t ws_bytes, void *stream);
+
+/* Its pullback, with the probabilities recomputed from q, k and lse:
+ * dq [batch][q_tokens][heads][head_dim], dk and dv [batch][k_tokens]
+ * [kv_heads][head_dim], contiguous, summed over the query heads that share a
+ * key head.  `out` and `lse` are the forward's, dout is contiguous.  Keys
+ * behind a sample's length receive 0.  Sums run in a fixed order: the same
+ * inputs give the same bits. */
+int reels_attention_backward(const reels_attn_shape *shape, const void *q, const void *k, const void *v,
+                             const void *out, const float *lse, const void *dout, const int32_t *kv_lengths,
+                             float scale, int act_dtype, void *dq, void *dk, void *dv, void *workspace,
+                             size_t ws_bytes, void *stream);
+
+/* ---------------------------------------------------------------------
  * The optimizer step after the gradient all-reduce (src/training/
  * wan_runner.jl:213-227 and AdamW update!, src/training/optimizer.jl:48-73),
  * over all adapter tensors in two launches and without a host round trip:

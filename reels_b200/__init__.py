@@ -2,9 +2,20 @@
 
 The compute lives in libreels_lowvram.so (include/reels_lowvram.h); this
 package is the Python-side mirror of the reference's layer API
-(:mod:`reels_b200.lowvram`) and its data-parallel gradient all-reduce
+(:mod:`reels_b200.lowvram`), the attention between its projections
+(:mod:`reels_b200.attention`) and its data-parallel gradient all-reduce
 (:mod:`reels_b200.distributed`).
 """
+from .attention import (  # noqa: F401
+    AttentionFunction,
+    RMSNormRopeFunction,
+    RopeTable,
+    attention,
+    attention_backward,
+    rms_norm_rope,
+    rms_norm_rope_backward,
+    rope_table,
+)
 from .lowvram import (  # noqa: F401
     DenseLayer,
     FrozenLinearFunction,

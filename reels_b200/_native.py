@@ -19,6 +19,7 @@ W_OUT_CONTIGUOUS, W_IN_CONTIGUOUS = 0, 1
 PASS_FORWARD, PASS_BACKWARD, PASS_DROPOUT = 0, 1, 2
 PATH_NONE, PATH_TENSORCORE, PATH_CUDACORE = 0, 1, 2
 ACT_NONE, ACT_GELU_TANH = 0, 1
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 OK, EINVAL, EDEVICE = 0, -1, -2
 
 class OptTensor(ctypes.Structure):
@@ -26,6 +27,18 @@ class OptTensor(ctypes.Structure):
     _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("m", ctypes.c_void_p),
                 ("v", ctypes.c_void_p), ("master", ctypes.c_void_p), ("n", ctypes.c_int64),
                 ("param_dtype", ctypes.c_int), ("decay", ctypes.c_int)]
+
+
+class Rope(ctypes.Structure):
+    """reels_rope: rotary positions of a video's tokens."""
+    _fields_ = [("table", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("size", ctypes.c_int32 * 3),
+                ("dim", ctypes.c_int32 * 3), ("pairing", ctypes.c_int32)]
+
+
+class AttnShape(ctypes.Structure):
+    """reels_attn_shape: sizes and element strides of q, k and v."""
+    _fields_ = [(n, ctypes.c_int64) for n in ("batch", "heads", "kv_heads", "q_tokens", "k_tokens", "head_dim")] + [
+        (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
 
 
 # Every symbol the header declares, with (restype, argtypes).
@@ -74,6 +87,15 @@ SIGNATURES = {
     "reels_gated_residual": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _vp]),
     "reels_gated_residual_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "reels_gated_residual_backward": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _int, _vp, _sz, _vp]),
+    "reels_rms_norm_rope": (_int, [_vp, _i64, _i64, _i64, _vp, ctypes.POINTER(Rope), _i64, _f, _int, _vp, _vp]),
+    "reels_rms_norm_rope_backward": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, ctypes.POINTER(Rope), _i64, _f, _int, _vp,
+                                            _vp]),
+    "reels_attention_workspace_bytes": (_sz, [ctypes.POINTER(AttnShape), _int, _int]),
+    "reels_attention_plan": (_int, [ctypes.POINTER(AttnShape), _int, ctypes.POINTER(ctypes.c_int64)]),
+    "reels_attention_forward": (_int, [ctypes.POINTER(AttnShape), _vp, _vp, _vp, _vp, _f, _int, _vp, _vp, _vp, _sz,
+                                       _vp]),
+    "reels_attention_backward": (_int, [ctypes.POINTER(AttnShape), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _int, _vp,
+                                        _vp, _vp, _vp, _sz, _vp]),
     "reels_opt_workspace_bytes": (_sz, [_int]),
     "reels_opt_prepare": (_int, [ctypes.POINTER(OptTensor), _int, _vp, _sz, _vp]),
     "reels_grad_norm_sq": (_int, [_vp, _f, _vp, _vp]),

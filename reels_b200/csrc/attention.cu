@@ -1,0 +1,535 @@
+// Host side of the block's attention stretch: argument checks, plans and
+// launches of the q/k norm with rotary positions (norm_rope.cuh) and of
+// softmax attention and its gradient (attn_fwd.cuh, attn_bwd.cuh,
+// attn_simt.cuh), behind the C ABI of include/reels_lowvram.h.
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+#include <type_traits>
+
+#include "../../include/reels_lowvram.h"
+#include "attn_bwd.cuh"
+#include "attn_fwd.cuh"
+#include "host.h"
+#include "norm_rope.cuh"
+
+using namespace reels;
+
+namespace {
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+bool known_dtype(int dt) { return dt == REELS_F32 || dt == REELS_F16 || dt == REELS_BF16; }
+int bytes_of(int dt) { return dt == REELS_F32 ? 4 : 2; }
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename F>
+void with_dtype(int dt, F &&f) {
+    if (dt == REELS_BF16) f(std::integral_constant<int, DT_BF16>{});
+    else if (dt == REELS_F16) f(std::integral_constant<int, DT_F16>{});
+    else f(std::integral_constant<int, DT_F32>{});
+}
+
+#define RA_LAUNCH(expr)                                                                              \
+    do {                                                                                             \
+        cudaError_t e_ = (expr);                                                                     \
+        if (e_ == cudaSuccess) e_ = cudaGetLastError();                                              \
+        if (e_ != cudaSuccess) return host_fail_dev(std::string("kernel launch: ") + cudaGetErrorString(e_)); \
+        host_count_launch();                                                                         \
+    } while (0)
+
+// ------------------------------------------------------- norm and rotation
+int check_norm_rope(const void *x, int64_t M, int64_t heads, int64_t D, const reels_rope *rope, int64_t tps, float eps,
+                    int dt) {
+    if (M < 0 || heads <= 0 || D <= 0 || heads > NR_MAX_C || D > NR_MAX_C || heads * D > NR_MAX_C)
+        return host_fail("rms_norm_rope needs 0 <= M and 0 < heads * head_dim <= " + std::to_string(NR_MAX_C));
+    if (!x && M > 0) return host_fail("null x");
+    if (tps <= 0 || tps > INT32_MAX) return host_fail("tokens_per_sample must be positive");
+    if (!(eps >= 0.0f) || !std::isfinite(eps)) return host_fail("epsilon must be finite and non-negative");
+    if (!known_dtype(dt)) return host_fail("unknown act_dtype");
+    if (!rope) return REELS_OK;
+    if (!rope->table) return host_fail("null rotary table");
+    if ((reinterpret_cast<uintptr_t>(rope->table) & 7) != 0) return host_fail("the rotary table must be 8-byte aligned");
+    if (D & 1) return host_fail("rotary positions need an even head_dim");
+    int64_t feats = 0, entries = 0, grid = 1;
+    for (int i = 0; i < NR_AXES; ++i) {
+        if (rope->size[i] <= 0 || rope->dim[i] < 0 || (rope->dim[i] & 1))
+            return host_fail("a rotary axis needs a positive size and an even number of features");
+        feats += rope->dim[i];
+        entries += (int64_t)rope->size[i] * (rope->dim[i] / 2);
+        grid *= rope->size[i];
+        if (entries > INT32_MAX || grid > INT32_MAX) return host_fail("the rotary table is too large");
+    }
+    if (feats != D) return host_fail("the rotary axes' features must sum to head_dim");
+    if (rope->pairing != REELS_ROPE_INTERLEAVED && rope->pairing != REELS_ROPE_HALF)
+        return host_fail("unknown rotary pairing");
+    return REELS_OK;
+}
+
+template <int DT, bool BWD, bool ROPE, bool HALF>
+cudaError_t launch_norm_rope(int upt, dim3 grid, dim3 block, cudaStream_t st, const NormRopeArgs &a) {
+    switch (upt) {
+        case 1: return host_launch_pdl(norm_rope_kernel<DT, BWD, ROPE, HALF, 1>, grid, block, 0, st, a);
+        case 2: return host_launch_pdl(norm_rope_kernel<DT, BWD, ROPE, HALF, 2>, grid, block, 0, st, a);
+        default: return host_launch_pdl(norm_rope_kernel<DT, BWD, ROPE, HALF, 4>, grid, block, 0, st, a);
+    }
+}
+
+int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t heads, int64_t D, const void *weight,
+              const reels_rope *rope, int64_t tps, float eps, int dt, void *out, void *stream) {
+    int rc = check_norm_rope(x, M, heads, D, rope, tps, eps, dt);
+    if (rc) return rc;
+    if (M == 0) return host_ok(REELS_PATH_NONE);
+    if (!out) return host_fail(bwd ? "null dx" : "null out");
+    if (bwd && !dout) return host_fail("null dout");
+    HostCall call;
+    rc = call.bind(x);
+    if (rc) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    NormRopeArgs a = {};
+    a.x = x, a.dout = dout, a.weight = weight, a.out = out;
+    a.M = M, a.C = (int)(heads * D), a.D = (int)D, a.tps = (int)tps, a.eps = eps, a.err = call.status;
+    if (rope) {
+        a.table = reinterpret_cast<const float2 *>(rope->table);
+        a.pos = rope->positions;
+        for (int i = 0; i < NR_AXES; ++i) a.size[i] = rope->size[i], a.pairs[i] = rope->dim[i] / 2;
+        a.half = rope->pairing == REELS_ROPE_HALF;
+    }
+    const int64_t units = a.C / 16;
+    const bool heads_fit = !rope || (D % 16 == 0 && 32 % (D / 16) == 0);
+    const bool vec = a.C % 16 == 0 && heads_fit && aligned16(x) && aligned16(out) && aligned16(weight) &&
+                     (!bwd || aligned16(dout)) && units <= 4 * 256;
+    if (!vec) {
+        const dim3 grid((unsigned)std::min<int64_t>(M, 8ll * call.sms));
+        with_dtype(dt, [&](auto t) {
+            constexpr int DT = decltype(t)::value;
+            if (bwd) host_launch_pdl(norm_rope_any_kernel<DT, true>, grid, dim3(256), 0, st, a);
+            else host_launch_pdl(norm_rope_any_kernel<DT, false>, grid, dim3(256), 0, st, a);
+        });
+        RA_LAUNCH(cudaSuccess);
+        return host_ok(REELS_PATH_CUDACORE);
+    }
+    if (!rope) a.D = 16;
+    // units a thread: as few as keep the block at 256 threads
+    const int upt = units <= 256 ? 1 : units <= 512 ? 2 : 4;
+    const int threads = (int)ceil_div(ceil_div(units, upt), 32) * 32;
+    const dim3 grid((unsigned)std::min<int64_t>(M, (int64_t)call.sms * (2048 / threads)));
+    cudaError_t e = cudaSuccess;
+    with_dtype(dt, [&](auto t) {
+        constexpr int DT = decltype(t)::value;
+        const dim3 block((unsigned)threads);
+        if (bwd)
+            e = !rope    ? launch_norm_rope<DT, true, false, false>(upt, grid, block, st, a)
+                : a.half ? launch_norm_rope<DT, true, true, true>(upt, grid, block, st, a)
+                         : launch_norm_rope<DT, true, true, false>(upt, grid, block, st, a);
+        else
+            e = !rope    ? launch_norm_rope<DT, false, false, false>(upt, grid, block, st, a)
+                : a.half ? launch_norm_rope<DT, false, true, true>(upt, grid, block, st, a)
+                         : launch_norm_rope<DT, false, true, false>(upt, grid, block, st, a);
+    });
+    RA_LAUNCH(e);
+    return host_ok(REELS_PATH_CUDACORE);
+}
+
+// ---------------------------------------------------------------- attention
+constexpr int kPlanSms = 148;
+
+struct AttnPlan {
+    bool tc = false;
+    int splits = 1, split_keys = 1;  // forward
+    int red_splits = 1;              // backward, dK and dV
+    int Sqp = 0;
+};
+
+bool tma_strides(const int64_t (&stride)[3], const int64_t (&n)[3]) {
+    for (int i = 0; i < 3; ++i)
+        if (n[i] > 1 && (stride[i] <= 0 || stride[i] % 8 != 0 || stride[i] >= (int64_t(1) << 38))) return false;
+    return true;
+}
+
+int check_shape(const reels_attn_shape *s, int dt) {
+    if (!s) return host_fail("null attention shape");
+    if (s->batch < 0 || s->q_tokens < 0 || s->k_tokens < 0 || s->heads <= 0 || s->kv_heads <= 0)
+        return host_fail("attention needs non-negative batch and tokens and positive heads");
+    if (s->heads % s->kv_heads != 0) return host_fail("heads must be a multiple of kv_heads");
+    if (s->head_dim <= 0 || s->head_dim > AT_MAX_D)
+        return host_fail("head_dim must be between 1 and " + std::to_string(AT_MAX_D));
+    const int64_t lim = INT32_MAX - 256;
+    if (s->batch > lim || s->heads > lim || s->q_tokens > lim || s->k_tokens > lim ||
+        s->batch * s->heads > lim || ceil_div(std::max(s->q_tokens, s->k_tokens), AS_T) > lim / std::max<int64_t>(1, s->batch * s->heads))
+        return host_fail("attention shape too large");
+    for (int i = 0; i < 3; ++i)
+        if (s->q_stride[i] < 0 || s->k_stride[i] < 0 || s->v_stride[i] < 0) return host_fail("negative stride");
+    if (!known_dtype(dt)) return host_fail("unknown act_dtype");
+    return REELS_OK;
+}
+
+// The tensor-core kernels take 16-bit tensors, heads of up to 128 features in
+// multiples of 8 (one 16-byte piece) and strides TMA can follow.
+AttnPlan plan_attention(const reels_attn_shape &s, int dt, const void *q, const void *k, const void *v) {
+    AttnPlan p;
+    const int64_t nq[3] = {s.batch, s.q_tokens, s.heads}, nk[3] = {s.batch, s.k_tokens, s.kv_heads};
+    p.tc = dt != REELS_F32 && s.head_dim % 8 == 0 && s.head_dim <= 128 && tma_strides(s.q_stride, nq) &&
+           tma_strides(s.k_stride, nk) && tma_strides(s.v_stride, nk) && aligned16(q) && aligned16(k) && aligned16(v);
+    p.Sqp = (int)(ceil_div(s.q_tokens, AT_TILE) * AT_TILE);
+    // Forward: few rows leave SMs idle, so the keys are split over them and
+    // joined; a split keeps at least four tiles of keys.
+    const int tile = p.tc ? AT_TILE : AS_T;
+    const int64_t rows = ceil_div(s.q_tokens, p.tc ? 2 * AT_TILE : AS_T) * s.batch * s.heads;
+    const int64_t tiles = std::max<int64_t>(1, ceil_div(s.k_tokens, tile));
+    int64_t want = rows > 0 ? std::min<int64_t>((p.tc ? 1 : 4) * kPlanSms / std::max<int64_t>(rows, 1), tiles / 4) : 1;
+    want = std::max<int64_t>(1, std::min<int64_t>(want, 1024));
+    const int64_t per = ceil_div(tiles, want);
+    p.splits = (int)ceil_div(tiles, per);
+    p.split_keys = (int)std::min<int64_t>(per * tile, INT32_MAX - 256);
+    // dK, dV: the walk over queries is split where whole walks would leave
+    // SMs idle in the last round.  Steps of a round, and the partial sums'
+    // way through memory, in units of a step (about 1.2 us).
+    if (p.tc && s.q_tokens > 0 && s.k_tokens > 0) {
+        const int64_t units = ceil_div(s.k_tokens, AT_TILE) * s.batch * s.kv_heads;
+        const int64_t steps = s.heads / s.kv_heads * (p.Sqp / AT_TILE);
+        const double mb = 2.0 * 2.0 * 4.0 * (double)(s.batch * s.k_tokens * s.kv_heads * s.head_dim) / 5e6;
+        double best = 1e300;
+        for (int64_t n = 1; n <= std::min<int64_t>(steps, 32); ++n) {
+            const double cost = (double)ceil_div(units * n, kPlanSms) * (double)(ceil_div(steps, n) + 3) +
+                                (n > 1 ? 4.0 + mb * (double)n / 1.2 : 0.0);
+            if (cost < best * 0.97) best = cost, p.red_splits = (int)n;
+        }
+        p.red_splits = (int)ceil_div(steps, ceil_div(steps, p.red_splits));
+    }
+    return p;
+}
+
+struct AttnWs {
+    size_t part_o = 0, part_lse = 0, stat_l = 0, stat_d = 0, range = 0, part_k = 0, part_v = 0, total = 0;
+};
+AttnWs attn_ws(const reels_attn_shape &s, const AttnPlan &p, bool bwd) {
+    AttnWs w;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t r = at;
+        at += up256(bytes);
+        return r;
+    };
+    if (!bwd) {
+        if (p.splits > 1) {
+            const size_t rows = (size_t)p.splits * s.batch * s.heads * s.q_tokens;
+            w.part_o = take(rows * s.head_dim * 4);
+            w.part_lse = take(rows * 4);
+        }
+    } else {
+        const size_t rows = (size_t)s.batch * s.heads * p.Sqp;
+        w.stat_l = take(rows * 4);
+        w.stat_d = take(rows * 4);
+        w.range = take(8);
+        if (p.red_splits > 1) {
+            const size_t n = (size_t)p.red_splits * s.batch * s.k_tokens * s.kv_heads * s.head_dim * 4;
+            w.part_k = take(n);
+            w.part_v = take(n);
+        }
+    }
+    w.total = at;
+    return w;
+}
+
+int check_workspace(const void *ws, size_t have, size_t need) {
+    if (need == 0) return REELS_OK;
+    if (!ws) return host_fail("null workspace; size it with reels_attention_workspace_bytes");
+    if ((reinterpret_cast<uintptr_t>(ws) & 255u) != 0) return host_fail("workspace must be 256-byte aligned");
+    if (have < need) return host_fail("workspace too small; size it with reels_attention_workspace_bytes");
+    return REELS_OK;
+}
+
+AttnArgs attn_args(const reels_attn_shape &s, const AttnPlan &p, const void *q, const void *k, const void *v,
+                   const int32_t *lengths, float scale) {
+    AttnArgs a = {};
+    a.q = q, a.k = k, a.v = v, a.lengths = lengths, a.scale = scale;
+    for (int i = 0; i < 3; ++i) a.qs[i] = s.q_stride[i], a.ks[i] = s.k_stride[i], a.vs[i] = s.v_stride[i];
+    a.B = (int)s.batch, a.H = (int)s.heads, a.HK = (int)s.kv_heads;
+    a.Sq = (int)s.q_tokens, a.Sk = (int)s.k_tokens, a.D = (int)s.head_dim;
+    a.splits = p.splits, a.split_keys = p.split_keys, a.red_splits = p.red_splits, a.Sqp = p.Sqp;
+    return a;
+}
+
+// [batch][tokens][heads][D] by strides, boxes of 64 features x 128 tokens
+int attn_map(CUtensorMap *tm, const void *base, int dt, int64_t B, int64_t S, int64_t H, int64_t D,
+             const int64_t (&stride)[3]) {
+    const uint64_t n[4] = {(uint64_t)D, (uint64_t)S, (uint64_t)H, (uint64_t)B};
+    auto st = [&](int64_t n_, int64_t s_) { return (uint64_t)(n_ > 1 ? s_ : ceil_div(D, 8) * 8) * 2; };
+    const uint64_t b[3] = {st(S, stride[1]), st(H, stride[2]), st(B, stride[0])};
+    const uint32_t box[4] = {64, AT_TILE, 1, 1};
+    return host_tmap_4d(tm, base, dt == REELS_BF16, n, b, box);
+}
+
+template <typename K>
+cudaError_t big_smem(K kern, int bytes) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+template <int DT, int DP>
+cudaError_t simt_attrs() {
+    cudaError_t e = big_smem(attn_simt_fwd_kernel<DT, DP>, as_smem_bytes(DP, 3));
+    if (e == cudaSuccess) e = big_smem(attn_simt_dkdv_kernel<DT, DP>, as_smem_bytes(DP, 4));
+    if (e == cudaSuccess) e = big_smem(attn_simt_dq_kernel<DT, DP>, as_smem_bytes(DP, 4));
+    return e;
+}
+template <int DT, int DP>
+cudaError_t tc_attrs() {
+    cudaError_t e = big_smem(attn_fwd_kernel<DT, DP>, AttnFwdGeom<DP>::SMEM_BYTES);
+    if (e == cudaSuccess) e = big_smem(attn_dkdv_kernel<DT, DP>, AttnKvGeom<DP>::SMEM_BYTES);
+    if (e == cudaSuccess) e = big_smem(attn_dq_kernel<DT, DP>, AttnQGeom<DP>::SMEM_BYTES);
+    return e;
+}
+// Shared-memory sizes of the kernels, once per device (which is current).
+int attn_ready(int device) {
+    static std::mutex mu;
+    static bool ready[64];
+    std::lock_guard<std::mutex> lock(mu);
+    if (ready[device]) return REELS_OK;
+    cudaError_t e = cudaSuccess;
+    auto also = [&](cudaError_t x) {
+        if (e == cudaSuccess) e = x;
+    };
+    also(simt_attrs<DT_F32, 64>()), also(simt_attrs<DT_F32, 128>()), also(simt_attrs<DT_F32, 256>());
+    also(simt_attrs<DT_F16, 64>()), also(simt_attrs<DT_F16, 128>()), also(simt_attrs<DT_F16, 256>());
+    also(simt_attrs<DT_BF16, 64>()), also(simt_attrs<DT_BF16, 128>()), also(simt_attrs<DT_BF16, 256>());
+    also(tc_attrs<DT_F16, 64>()), also(tc_attrs<DT_F16, 128>());
+    also(tc_attrs<DT_BF16, 64>()), also(tc_attrs<DT_BF16, 128>());
+    if (e != cudaSuccess) return host_fail_dev(std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+    ready[device] = true;
+    return REELS_OK;
+}
+
+template <typename F>
+void with_simt_dim(int64_t D, F &&f) {
+    if (D <= 64) f(std::integral_constant<int, 64>{});
+    else if (D <= 128) f(std::integral_constant<int, 128>{});
+    else f(std::integral_constant<int, 256>{});
+}
+template <typename F>
+void with_tc_type(int dt, int64_t D, F &&f) {
+    auto dim = [&](auto t) {
+        if (D <= 64) f(t, std::integral_constant<int, 64>{});
+        else f(t, std::integral_constant<int, 128>{});
+    };
+    if (dt == REELS_BF16) dim(std::integral_constant<int, DT_BF16>{});
+    else dim(std::integral_constant<int, DT_F16>{});
+}
+
+}  // namespace
+
+extern "C" {
+
+int reels_rms_norm_rope(const void *x, int64_t M, int64_t heads, int64_t head_dim, const void *weight,
+                        const reels_rope *rope, int64_t tokens_per_sample, float epsilon, int act_dtype, void *out,
+                        void *stream) {
+    return norm_rope(x, nullptr, false, M, heads, head_dim, weight, rope, tokens_per_sample, epsilon, act_dtype, out,
+                     stream);
+}
+
+int reels_rms_norm_rope_backward(const void *x, const void *dout, int64_t M, int64_t heads, int64_t head_dim,
+                                 const void *weight, const reels_rope *rope, int64_t tokens_per_sample, float epsilon,
+                                 int act_dtype, void *dx, void *stream) {
+    return norm_rope(x, dout, true, M, heads, head_dim, weight, rope, tokens_per_sample, epsilon, act_dtype, dx,
+                     stream);
+}
+
+size_t reels_attention_workspace_bytes(const reels_attn_shape *shape, int act_dtype, int pass) {
+    if (check_shape(shape, act_dtype) != REELS_OK) return 0;
+    // The larger of the two paths: which one runs also depends on the pointers.
+    AttnPlan p = plan_attention(*shape, act_dtype, nullptr, nullptr, nullptr);
+    size_t n = attn_ws(*shape, p, pass == REELS_PASS_BACKWARD).total;
+    p = plan_attention(*shape, act_dtype, reinterpret_cast<const void *>(1), nullptr, nullptr);
+    return std::max(n, attn_ws(*shape, p, pass == REELS_PASS_BACKWARD).total);
+}
+
+int reels_attention_plan(const reels_attn_shape *shape, int act_dtype, int64_t *info) {
+    int rc = check_shape(shape, act_dtype);
+    if (rc) return rc;
+    if (!info) return host_fail("null info");
+    const AttnPlan p = plan_attention(*shape, act_dtype, nullptr, nullptr, nullptr);
+    info[0] = p.tc ? REELS_PATH_TENSORCORE : REELS_PATH_CUDACORE;
+    info[1] = p.splits;
+    info[2] = p.split_keys;
+    info[3] = p.red_splits;
+    return host_ok(REELS_PATH_NONE);
+}
+
+int reels_attention_forward(const reels_attn_shape *shape, const void *q, const void *k, const void *v,
+                            const int32_t *kv_lengths, float scale, int act_dtype, void *out, float *lse,
+                            void *workspace, size_t ws_bytes, void *stream) {
+    int rc = check_shape(shape, act_dtype);
+    if (rc) return rc;
+    const reels_attn_shape &s = *shape;
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return host_fail("scale must be finite and positive");
+    if (s.batch == 0 || s.q_tokens == 0) return host_ok(REELS_PATH_NONE);
+    if (!q || !out || !lse) return host_fail("null q, out or lse");
+    if (s.k_tokens > 0 && (!k || !v)) return host_fail("null k or v");
+    const AttnPlan p = plan_attention(s, act_dtype, q, k, v);
+    const bool tc = p.tc && aligned16(out) && s.k_tokens > 0;
+    AttnPlan plan = p;
+    if (!tc && p.tc) plan = plan_attention(s, act_dtype, reinterpret_cast<const void *>(1), k, v);
+    const AttnWs w = attn_ws(s, plan, false);
+    rc = check_workspace(workspace, ws_bytes, w.total);
+    if (rc) return rc;
+    HostCall call;
+    rc = call.bind(q);
+    if (rc) return rc;
+    rc = attn_ready(call.device);
+    if (rc) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    AttnArgs a = attn_args(s, plan, q, k, v, kv_lengths, scale);
+    a.out = out, a.lse = lse, a.err = call.status;
+    if (plan.splits > 1) {
+        a.part_o = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + w.part_o);
+        a.part_lse = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + w.part_lse);
+    }
+    cudaError_t e = cudaSuccess;
+    if (tc) {
+        CUtensorMap mq, mk, mv;
+        if ((rc = attn_map(&mq, q, act_dtype, s.batch, s.q_tokens, s.heads, s.head_dim, s.q_stride)) ||
+            (rc = attn_map(&mk, k, act_dtype, s.batch, s.k_tokens, s.kv_heads, s.head_dim, s.k_stride)) ||
+            (rc = attn_map(&mv, v, act_dtype, s.batch, s.k_tokens, s.kv_heads, s.head_dim, s.v_stride)))
+            return rc;
+        const long long units = ceil_div(s.q_tokens, 2 * AT_TILE) * s.batch * s.heads * plan.splits;
+        with_tc_type(act_dtype, s.head_dim, [&](auto t, auto d) {
+            constexpr int DT = decltype(t)::value, DP = decltype(d)::value;
+            e = host_launch_pdl(attn_fwd_kernel<DT, DP>, dim3((unsigned)std::min<long long>(units, call.sms)),
+                                dim3(AF_THREADS), AttnFwdGeom<DP>::SMEM_BYTES, st, mq, mk, mv, a, units);
+        });
+    } else {
+        const dim3 grid((unsigned)(ceil_div(s.q_tokens, AS_T) * s.batch * s.heads), (unsigned)plan.splits);
+        with_dtype(act_dtype, [&](auto t) {
+            with_simt_dim(s.head_dim, [&](auto d) {
+                constexpr int DT = decltype(t)::value, DP = decltype(d)::value;
+                e = host_launch_pdl(attn_simt_fwd_kernel<DT, DP>, grid, dim3(AS_THREADS), as_smem_bytes(DP, 3), st, a);
+            });
+        });
+    }
+    RA_LAUNCH(e);
+    if (plan.splits > 1) {
+        const int64_t rows = s.batch * s.heads * s.q_tokens;
+        with_dtype(act_dtype, [&](auto t) {
+            e = host_launch_pdl(attn_join_kernel<decltype(t)::value>,
+                                dim3((unsigned)std::min<int64_t>(ceil_div(rows, 8), 8ll * call.sms)), dim3(256), 0, st,
+                                a);
+        });
+        RA_LAUNCH(e);
+    }
+    return host_ok(tc ? REELS_PATH_TENSORCORE : REELS_PATH_CUDACORE);
+}
+
+int reels_attention_backward(const reels_attn_shape *shape, const void *q, const void *k, const void *v,
+                             const void *out, const float *lse, const void *dout, const int32_t *kv_lengths,
+                             float scale, int act_dtype, void *dq, void *dk, void *dv, void *workspace,
+                             size_t ws_bytes, void *stream) {
+    int rc = check_shape(shape, act_dtype);
+    if (rc) return rc;
+    const reels_attn_shape &s = *shape;
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return host_fail("scale must be finite and positive");
+    if (s.batch == 0 || (s.q_tokens == 0 && s.k_tokens == 0)) return host_ok(REELS_PATH_NONE);
+    if (s.q_tokens > 0 && (!q || !out || !lse || !dout || !dq)) return host_fail("null q, out, lse, dout or dq");
+    if (s.k_tokens > 0 && (!k || !v || !dk || !dv)) return host_fail("null k, v, dk or dv");
+    HostCall call;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (s.q_tokens == 0 || s.k_tokens == 0) {  // nothing attends: zero gradients
+        rc = call.bind(s.q_tokens ? dq : dk);
+        if (rc) return rc;
+        const size_t row = (size_t)s.head_dim * bytes_of(act_dtype);
+        cudaError_t e = cudaSuccess;
+        if (s.q_tokens) e = cudaMemsetAsync(dq, 0, (size_t)s.batch * s.q_tokens * s.heads * row, st);
+        if (s.k_tokens) {
+            e = cudaMemsetAsync(dk, 0, (size_t)s.batch * s.k_tokens * s.kv_heads * row, st);
+            if (e == cudaSuccess) e = cudaMemsetAsync(dv, 0, (size_t)s.batch * s.k_tokens * s.kv_heads * row, st);
+        }
+        if (e != cudaSuccess) return host_fail_dev(std::string("cudaMemsetAsync: ") + cudaGetErrorString(e));
+        return host_ok(REELS_PATH_NONE);
+    }
+    AttnPlan plan = plan_attention(s, act_dtype, q, k, v);
+    if (plan.tc && !(aligned16(out) && aligned16(dout) && aligned16(dq) && aligned16(dk) && aligned16(dv)))
+        plan = plan_attention(s, act_dtype, reinterpret_cast<const void *>(1), k, v);
+    const AttnWs w = attn_ws(s, plan, true);
+    rc = check_workspace(workspace, ws_bytes, w.total);
+    if (rc) return rc;
+    rc = call.bind(q);
+    if (rc) return rc;
+    rc = attn_ready(call.device);
+    if (rc) return rc;
+    char *ws = reinterpret_cast<char *>(workspace);
+    AttnArgs a = attn_args(s, plan, q, k, v, kv_lengths, scale);
+    a.out = const_cast<void *>(out), a.lse = const_cast<float *>(lse), a.dout = dout;
+    a.dq = dq, a.dk = dk, a.dv = dv, a.err = call.status;
+    float *stat_l = reinterpret_cast<float *>(ws + w.stat_l), *stat_d = reinterpret_cast<float *>(ws + w.stat_d);
+    a.stat_l = stat_l, a.stat_d = stat_d;
+    a.part_k = reinterpret_cast<float *>(ws + w.part_k), a.part_v = reinterpret_cast<float *>(ws + w.part_v);
+    unsigned *range = nullptr;
+    cudaError_t e = cudaSuccess;
+    if (plan.tc && act_dtype == REELS_F16) {
+        range = reinterpret_cast<unsigned *>(ws + w.range);
+        a.range = range;
+        e = cudaMemsetAsync(range, 0, 8, st);
+        if (e != cudaSuccess) return host_fail_dev(std::string("cudaMemsetAsync: ") + cudaGetErrorString(e));
+    }
+    const int64_t rows = s.batch * s.heads * plan.Sqp, keys = s.batch * s.kv_heads * s.k_tokens;
+    with_dtype(act_dtype, [&](auto t) {
+        e = host_launch_pdl(attn_stat_kernel<decltype(t)::value>,
+                            dim3((unsigned)std::min<int64_t>(ceil_div(rows, 8), 8ll * call.sms)), dim3(256), 0, st, a,
+                            stat_l, stat_d, range);
+    });
+    RA_LAUNCH(e);
+    if (!plan.tc) {
+        with_dtype(act_dtype, [&](auto t) {
+            with_simt_dim(s.head_dim, [&](auto d) {
+                constexpr int DT = decltype(t)::value, DP = decltype(d)::value;
+                e = host_launch_pdl(attn_simt_dkdv_kernel<DT, DP>,
+                                    dim3((unsigned)(ceil_div(s.k_tokens, AS_T) * s.batch * s.kv_heads)),
+                                    dim3(AS_THREADS), as_smem_bytes(DP, 4), st, a);
+                if (e == cudaSuccess)
+                    e = host_launch_pdl(attn_simt_dq_kernel<DT, DP>,
+                                        dim3((unsigned)(ceil_div(s.q_tokens, AS_T) * s.batch * s.heads)),
+                                        dim3(AS_THREADS), as_smem_bytes(DP, 4), st, a);
+            });
+        });
+        RA_LAUNCH(e);
+        host_count_launch();
+        return host_ok(REELS_PATH_CUDACORE);
+    }
+    if (range) {
+        with_dtype(act_dtype, [&](auto t) {
+            e = host_launch_pdl(attn_range_kernel<decltype(t)::value>,
+                                dim3((unsigned)std::min<int64_t>(ceil_div(keys, 8), 8ll * call.sms)), dim3(256), 0, st,
+                                a, range + 1);
+        });
+        RA_LAUNCH(e);
+    }
+    const int64_t og[3] = {s.q_tokens * s.heads * s.head_dim, s.heads * s.head_dim, s.head_dim};
+    CUtensorMap mq, mk, mv, mg;
+    if ((rc = attn_map(&mq, q, act_dtype, s.batch, s.q_tokens, s.heads, s.head_dim, s.q_stride)) ||
+        (rc = attn_map(&mk, k, act_dtype, s.batch, s.k_tokens, s.kv_heads, s.head_dim, s.k_stride)) ||
+        (rc = attn_map(&mv, v, act_dtype, s.batch, s.k_tokens, s.kv_heads, s.head_dim, s.v_stride)) ||
+        (rc = attn_map(&mg, dout, act_dtype, s.batch, s.q_tokens, s.heads, s.head_dim, og)))
+        return rc;
+    const long long kv_units = ceil_div(s.k_tokens, AT_TILE) * s.batch * s.kv_heads * plan.red_splits;
+    const long long q_units = (long long)(plan.Sqp / AT_TILE) * s.batch * s.heads;
+    with_tc_type(act_dtype, s.head_dim, [&](auto t, auto d) {
+        constexpr int DT = decltype(t)::value, DP = decltype(d)::value;
+        e = host_launch_pdl(attn_dkdv_kernel<DT, DP>, dim3((unsigned)std::min<long long>(kv_units, call.sms)),
+                            dim3(AB_THREADS), AttnKvGeom<DP>::SMEM_BYTES, st, mq, mk, mv, mg, a, kv_units);
+        if (e == cudaSuccess && plan.red_splits > 1) {
+            const long long n = (long long)keys * s.head_dim;
+            const dim3 grid((unsigned)std::min<long long>(ceil_div(n, 1024), 8ll * call.sms));
+            e = host_launch_pdl(attn_sum_kernel<DT>, grid, dim3(256), 0, st, (const float *)a.part_k, n,
+                                plan.red_splits, a.dk);
+            if (e == cudaSuccess)
+                e = host_launch_pdl(attn_sum_kernel<DT>, grid, dim3(256), 0, st, (const float *)a.part_v, n,
+                                    plan.red_splits, a.dv);
+        }
+        if (e == cudaSuccess)
+            e = host_launch_pdl(attn_dq_kernel<DT, DP>, dim3((unsigned)std::min<long long>(q_units, call.sms)),
+                                dim3(AB_THREADS), AttnQGeom<DP>::SMEM_BYTES, st, mq, mk, mv, mg, a, q_units);
+    });
+    RA_LAUNCH(e);
+    for (int i = 0; i < (plan.red_splits > 1 ? 3 : 1); ++i) host_count_launch();
+    return host_ok(REELS_PATH_TENSORCORE);
+}
+
+}  // extern "C"

@@ -1,0 +1,709 @@
+// Gradient of softmax attention on the 5th-gen tensor cores (sm_100a): the
+// probabilities are recomputed from q, k and the forward's L.
+//
+//   P = exp2(c S - L2)                 c = scale log2(e), L2 = L log2(e)
+//   dS = P (dP - delta),  dP = dO V',  delta = rowsum(dO * O)
+//   dV = P' dO,   dK = scale dS' Q,   dQ = scale dS K
+//
+// Two kernels, each a sum in registers' order with no atomics, so repeated
+// calls give the same bits: one walks the queries of a key tile (dK, dV; four
+// products a step), one the keys of a query tile (dQ; three).  Seven products
+// where one pass with scattered sums of dQ would need five.
+//
+// In both, the second product's operand (P', dS', dS) is written by the CUDA
+// cores into tensor memory over the scores it came from, which the same
+// issuing thread overwrites only after that product.  Two issuers: S and dV,
+// dP and dK (dQ kernel: S; dP and dQ), whose chains meet only in the
+// elementwise warps.
+#pragma once
+#include "attn_common.cuh"
+
+namespace reels {
+
+constexpr int AB_THREADS = 32 * 12;  // 8 elementwise warps, loads, two MMA issuers, one idle
+
+// fp16: exponent e with |dS| 2^e <= 2^15, from |dP|, |delta| <= |dO row| |v row|.
+template <int DT>
+__device__ __forceinline__ int attn_grad_exp(const AttnArgs &a) {
+    if (DT != DT_F16) return 0;
+    const float top = __uint_as_float(__ldcg(a.range)) * __uint_as_float(__ldcg(a.range + 1));
+    if (!(top > 1e-30f) || !(top < 1e30f)) return 0;
+    return 13 - ilogbf(top);
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+        "r"(bytes), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// 32 accumulator columns of this thread's row, times f, to dst (features c0 ..): 16-bit or fp32.
+template <int DT>
+__device__ __forceinline__ void ab_store32(const uint32_t (&o)[32], float f, typename Elem<DT>::T *dst, float *part,
+                                           int c0, int D) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 8) {
+        if (c0 + e >= D) continue;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[e + k]) * f;
+        if (part) {
+            float4 *p = reinterpret_cast<float4 *>(part + c0 + e);
+            p[0] = make_float4(v[0], v[1], v[2], v[3]);
+            p[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            *reinterpret_cast<uint4 *>(dst + c0 + e) =
+                make_uint4(Elem<DT>::pack2(v[0], v[1]), Elem<DT>::pack2(v[2], v[3]), Elem<DT>::pack2(v[4], v[5]),
+                           Elem<DT>::pack2(v[6], v[7]));
+        }
+    }
+}
+
+// Waits for both issuers' last commits, then gives the tensor memory back.
+__device__ __forceinline__ void ab_finish(uint32_t tmem, uint64_t *mma_done, unsigned *err) {
+    tc_fence_after();
+    for (int t = 0; t < 2; ++t) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&mma_done[t], 0)) {
+            if (clock64() - t0 > REELS_WAIT_LIMIT_CYCLES) {
+                if ((threadIdx.x & 31) == 0) atomicOr(err, DEVERR_TIMEOUT_ACC);
+                break;
+            }
+        }
+    }
+    __syncwarp();
+    tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------ dK and dV
+// Unit: a tile of 128 keys of one key head and a range of the walk over the
+// query tiles of the heads that share it.  Everything is computed transposed
+// (lanes are keys):
+//   S' = K Q',  dP' = V dO'   (128 x 128),   dV += P' dO,  dK += dS' Q
+// TMEM: S'/P', dP'/dS', dV, dK, 128 columns each.  The elementwise warps come
+// in two groups, one per 64 queries; each overwrites its own half of S' with
+// its half of P' (columns 0.. and 64..).
+template <int DP>
+struct AttnKvGeom {
+    static constexpr int TILE = AT_TILE * DP * 2;
+    static constexpr int NST = DP == 128 ? 2 : 4;
+    static constexpr int STAGE = 2 * TILE;        // Q and dO
+    static constexpr int RING_OFF = 2 * TILE;     // behind K and V
+    static constexpr int STAT_OFF = RING_OFF + NST * STAGE;  // per stage: L2[128], delta[128]
+    static constexpr int BAR_OFF = STAT_OFF + NST * 1024;
+    // kv_full, kv_empty, s_full, p_full, dp_full, ds_full, acc_full, acc_empty, mma_done[2]; q_full, q_empty, g_full, g_empty
+    static constexpr int NBAR = 10 + 4 * NST;
+    static constexpr int MISC_OFF = BAR_OFF + NBAR * 8;
+    static constexpr int SMEM_BYTES = MISC_OFF + 16 + 1024;
+    static_assert(SMEM_BYTES <= 232448, "shared memory plan exceeds 227 KB");
+};
+
+struct AttnKvUnit {
+    int b, hk, k0, rows, split;  // rows: keys of the tile before the sample's length
+    int it0, n;                  // steps: head it / nqt of the group, query tile it % nqt
+};
+
+__device__ __forceinline__ AttnKvUnit attn_kv_unit(const AttnArgs &a, long long u) {
+    const int kt = (a.Sk + AT_TILE - 1) / AT_TILE;
+    AttnKvUnit w;
+    w.k0 = (int)(u % kt) * AT_TILE;
+    u /= kt;
+    w.hk = (int)(u % a.HK);
+    u /= a.HK;
+    w.b = (int)(u % a.B);
+    w.split = (int)(u / a.B);
+    const int total = a.H / a.HK * (a.Sqp / AT_TILE), per = (total + a.red_splits - 1) / a.red_splits;
+    w.rows = min(AT_TILE, attn_keys(a, w.b) - w.k0);
+    w.it0 = min(total, w.split * per);
+    w.n = w.rows > 0 ? min(total, w.it0 + per) - w.it0 : 0;
+    return w;
+}
+
+template <int DT, int DP>
+__global__ void __launch_bounds__(AB_THREADS, 1)
+    attn_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG,
+                     const AttnArgs a, const long long units) {
+    using G = AttnKvGeom<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_u32(smem);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
+    uint64_t *kv_full = bars, *kv_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 3, *dp_full = bars + 4,
+             *ds_full = bars + 5, *acc_full = bars + 6, *acc_empty = bars + 7, *mma_done = bars + 8,
+             *q_full = bars + 10, *q_empty = q_full + G::NST, *g_full = q_empty + G::NST, *g_empty = g_full + G::NST;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + G::MISC_OFF);
+    volatile int *abort = reinterpret_cast<volatile int *>(smem + G::MISC_OFF + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        mbar_init(kv_full, 1);
+        mbar_init(kv_empty, 2);
+        mbar_init(s_full, 1);
+        mbar_init(p_full, 8);
+        mbar_init(dp_full, 1);
+        mbar_init(ds_full, 8);
+        mbar_init(acc_full, 2);
+        mbar_init(acc_empty, 8);
+        mbar_init(&mma_done[0], 1);
+        mbar_init(&mma_done[1], 1);
+        for (int s = 0; s < G::NST; ++s) {
+            mbar_init(&q_full[s], 1);
+            mbar_init(&q_empty[s], 2);
+            mbar_init(&g_full[s], 1);
+            mbar_init(&g_empty[s], 2);
+        }
+        *abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8) {
+        if (lane == 0) {
+            tma_prefetch_desc(&tmQ);
+            tma_prefetch_desc(&tmK);
+            tma_prefetch_desc(&tmV);
+            tma_prefetch_desc(&tmG);
+        }
+        __syncwarp();
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    griddep_wait();
+    const int nqt = a.Sqp / AT_TILE, group = a.H / a.HK;
+
+    if (warp == 8) {
+        // ------------------------------------------------------------ loads
+        at_fewer_registers();
+        if (lane == 0) {
+            uint32_t g = 0, nu = 0;
+            bool good = true;
+            for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+                const AttnKvUnit w = attn_kv_unit(a, u);
+                if (w.n == 0) continue;
+                good = wait_bar(kv_empty, (nu++ & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_W_EMPTY);
+                if (!good) break;
+                mbar_arrive_expect_tx(kv_full, 2 * G::TILE);
+                at_load_tile<DP>(sbase, &tmK, w.k0, w.hk, w.b, kv_full);
+                at_load_tile<DP>(sbase + G::TILE, &tmV, w.k0, w.hk, w.b, kv_full);
+                for (int i = 0; i < w.n; ++i, ++g) {
+                    const int it = w.it0 + i, h = w.hk * group + it / nqt, q0 = it % nqt * AT_TILE;
+                    const int s = g % G::NST;
+                    const uint32_t ph = ((g / G::NST) & 1) ^ 1;
+                    const uint32_t dst = sbase + G::RING_OFF + s * G::STAGE, st = sbase + G::STAT_OFF + s * 1024;
+                    const long long at = ((long long)w.b * a.H + h) * a.Sqp + q0;
+                    good = wait_bar(&q_empty[s], ph, abort, a.err, DEVERR_TIMEOUT_AB_EMPTY);
+                    if (!good) break;
+                    mbar_arrive_expect_tx(&q_full[s], G::TILE + 1024);
+                    at_load_tile<DP>(dst, &tmQ, q0, h, w.b, &q_full[s]);
+                    bulk_load(st, a.stat_l + at, 512, &q_full[s]);
+                    bulk_load(st + 512, a.stat_d + at, 512, &q_full[s]);
+                    good = wait_bar(&g_empty[s], ph, abort, a.err, DEVERR_TIMEOUT_AB_EMPTY);
+                    if (!good) break;
+                    mbar_arrive_expect_tx(&g_full[s], G::TILE);
+                    at_load_tile<DP>(dst + G::TILE, &tmG, q0, h, w.b, &g_full[s]);
+                }
+            }
+        }
+    } else if (warp == 11) {
+        at_fewer_registers();  // idle: completes the third group of four warps
+    } else if (warp > 8) {
+        // ------------------------------------------------- MMAs: 9 S', dV; 10 dP', dK
+        at_fewer_registers();
+        const int second = warp - 9;
+        if (lane == 0) {
+            constexpr int ab = DT == DT_BF16 ? 1 : 0;
+            constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
+            const uint32_t S = tmem + second * 128, O = tmem + 256 + second * 128, A = sbase + second * G::TILE;
+            // score operand of a stage (Q, dO), and the other one (dO, Q)
+            uint64_t *in_full = second ? g_full : q_full, *in_empty = second ? g_empty : q_empty;
+            uint64_t *ot_full = second ? q_full : g_full, *ot_empty = second ? q_empty : g_empty;
+            uint64_t *scored = second ? dp_full : s_full, *ready = second ? ds_full : p_full;
+            const uint32_t in_off = second ? G::TILE : 0, ot_off = second ? 0 : G::TILE;
+            uint32_t g = 0, np = 0, nu = 0;
+            bool good = true;
+            auto scores = [&](uint32_t i) {
+                const int s = i % G::NST;
+                good = good && wait_bar(&in_full[s], (i / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
+                if (!good) return;
+                tc_fence_after();
+                const uint32_t B = sbase + G::RING_OFF + s * G::STAGE + in_off;
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) mma_f16_ss(S, at_desc_k(A, kk), at_desc_k(B, kk), id_s, kk > 0);
+                mma_commit(scored);
+                mma_commit(&in_empty[s]);
+            };
+            for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+                const AttnKvUnit w = attn_kv_unit(a, u);
+                if (w.n == 0) continue;
+                good = wait_bar(kv_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
+                scores(g);
+                for (int i = 0; i < w.n && good; ++i, ++g) {
+                    const int s = g % G::NST;
+                    if (i == w.n - 1) mma_commit(kv_empty);  // the last scores were issued
+                    good = wait_bar(&ot_full[s], (g / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL) &&
+                           wait_bar(ready, np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (i == 0) good = good && wait_bar(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (!good) break;
+                    tc_fence_after();
+                    const uint32_t B = sbase + G::RING_OFF + s * G::STAGE + ot_off;
+#pragma unroll
+                    for (int kk = 0; kk < AT_TILE / 16; ++kk)
+                        at_mma_ts(O, S + (kk >> 2) * 64 + (kk & 3) * 8, at_desc_mn(B, kk), id_o, i > 0 || kk > 0);
+                    mma_commit(&ot_empty[s]);
+                    if (i + 1 < w.n) scores(g + 1);
+                }
+                if (!good) break;
+                mma_commit(acc_full);
+                ++nu;
+            }
+            mma_commit(&mma_done[second]);
+        }
+    } else {
+        // --------------------------------------------- P', dS' and the output
+        at_more_registers();
+        const int half = warp >> 2;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t S = tmem + lanes + 64 * half, DS = S + 128, O = tmem + lanes + 256 + 128 * half;
+        const float c = a.scale * CUDART_L2E_F;
+        const int e = attn_grad_exp<DT>(a);
+        const float grow = exp2f((float)e - AtRange<DT>::BWD_SHIFT);
+        const float f = half ? a.scale * exp2f(-(float)e) : exp2f(-AtRange<DT>::BWD_SHIFT);
+        uint32_t g = 0, ns = 0, nu = 0;
+        bool good = true;
+        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+            const AttnKvUnit w = attn_kv_unit(a, u);
+            const int row = (warp & 3) * 32 + lane;
+            const bool live = row < w.rows;
+            for (int i = 0; i < w.n; ++i, ++g, ++ns) {
+                const int s = g % G::NST;
+                const float4 *L = reinterpret_cast<const float4 *>(smem + G::STAT_OFF + s * 1024 + half * 256);
+                const float4 *Dl = L + 32;
+                good = at_wait(&q_full[s], (g / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL) &&
+                       at_wait(s_full, ns & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                if (!good) break;
+                tc_fence_after();
+                uint32_t x[64];
+                at_tmem_ld32(S, x);
+                at_tmem_ld32(S + 32, x + 32);
+                tmem_wait_ld();
+                uint32_t p[32];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const float4 l = L[k];
+                    float v[4];
+                    v[0] = at_exp2(fmaf(__uint_as_float(x[4 * k]), c, AtRange<DT>::BWD_SHIFT - l.x));
+                    v[1] = at_exp2(fmaf(__uint_as_float(x[4 * k + 1]), c, AtRange<DT>::BWD_SHIFT - l.y));
+                    v[2] = at_exp2(fmaf(__uint_as_float(x[4 * k + 2]), c, AtRange<DT>::BWD_SHIFT - l.z));
+                    v[3] = at_exp2(fmaf(__uint_as_float(x[4 * k + 3]), c, AtRange<DT>::BWD_SHIFT - l.w));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (!live) v[j] = 0.0f;
+                        x[4 * k + j] = __float_as_uint(v[j]);
+                    }
+                    p[2 * k] = Elem<DT>::pack2(v[0], v[1]);
+                    p[2 * k + 1] = Elem<DT>::pack2(v[2], v[3]);
+                }
+                at_tmem_st32(S, p);
+                at_tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full);
+                good = at_wait(dp_full, ns & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                if (!good) break;
+                tc_fence_after();
+                uint32_t y[64];
+                at_tmem_ld32(DS, y);
+                at_tmem_ld32(DS + 32, y + 32);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const float4 d = Dl[k];
+                    float v[4];
+                    v[0] = __uint_as_float(x[4 * k]) * (__uint_as_float(y[4 * k]) - d.x);
+                    v[1] = __uint_as_float(x[4 * k + 1]) * (__uint_as_float(y[4 * k + 1]) - d.y);
+                    v[2] = __uint_as_float(x[4 * k + 2]) * (__uint_as_float(y[4 * k + 2]) - d.z);
+                    v[3] = __uint_as_float(x[4 * k + 3]) * (__uint_as_float(y[4 * k + 3]) - d.w);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (DT == DT_F16) v[j] *= grow;
+                        if (!live) v[j] = 0.0f;
+                    }
+                    p[2 * k] = Elem<DT>::pack2(v[0], v[1]);
+                    p[2 * k + 1] = Elem<DT>::pack2(v[2], v[3]);
+                }
+                at_tmem_st32(DS, p);
+                at_tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ds_full);
+            }
+            if (!good) break;
+            if (w.n > 0) {
+                good = at_wait(acc_full, nu++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                if (!good) break;
+                tc_fence_after();
+            }
+            const int t = w.k0 + row;
+            const long long at = (((long long)w.b * a.Sk + t) * a.HK + w.hk) * a.D;
+            float *part = a.red_splits > 1
+                              ? (half ? a.part_k : a.part_v) + (long long)w.split * a.B * a.Sk * a.HK * a.D + at
+                              : nullptr;
+            auto *dst = reinterpret_cast<typename Elem<DT>::T *>(half ? a.dk : a.dv) + at;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                uint32_t o[32];
+                if (w.n > 0) {
+                    at_tmem_ld32(O + 32 * i, o);
+                    tmem_wait_ld();
+                }
+                if (i == DP / 32 - 1 && w.n > 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acc_empty);
+                }
+                if (w.n == 0 || !live) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = 0u;
+                }
+                if (t < a.Sk) ab_store32<DT>(o, f, dst, part, 32 * i, a.D);
+                __syncwarp();
+            }
+        }
+    }
+
+    if (*abort) {
+        for (int i = 0; i < 64; ++i) __nanosleep(2000);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) ab_finish(tmem, mma_done, a.err);
+}
+
+// Adds the partial dK and dV of the split walk in order.
+template <int DT>
+__global__ void __launch_bounds__(256) attn_sum_kernel(const float *part, long long n, int splits, void *out) {
+    griddep_wait();
+    for (long long i = 4ll * (blockIdx.x * 256ll + threadIdx.x); i < n; i += 1024ll * gridDim.x) {
+        float4 s = __ldcg(reinterpret_cast<const float4 *>(part + i));
+        for (int k = 1; k < splits; ++k) {
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part + k * n + i));
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        *reinterpret_cast<uint2 *>(reinterpret_cast<typename Elem<DT>::T *>(out) + i) =
+            make_uint2(Elem<DT>::pack2(s.x, s.y), Elem<DT>::pack2(s.z, s.w));
+    }
+}
+
+// ------------------------------------------------------------------- dQ
+// Unit: a tile of 128 queries of one head, walking the keys 128 at a time:
+//   S = Q K',  dP = dO V'   (128 x 128),   dQ += dS K
+// TMEM: S twice (the scores of the next tile are ready when this one's dS is
+// written), dP/dS, dQ.
+template <int DP>
+struct AttnQGeom {
+    static constexpr int TILE = AT_TILE * DP * 2;
+    static constexpr int NK = DP == 128 ? 3 : 5, NV = DP == 128 ? 2 : 4;  // tiles in flight
+    static constexpr int K_OFF = 2 * TILE;  // behind Q and dO
+    static constexpr int V_OFF = K_OFF + NK * TILE;
+    static constexpr int BAR_OFF = V_OFF + NV * TILE;
+    // q_full, q_empty, s_full[2], s_empty[2], dp_full, ds_full, acc_full, acc_empty, raw, mma_done[2]; rings
+    static constexpr int NBAR = 13 + 2 * (NK + NV);
+    static constexpr int MISC_OFF = BAR_OFF + NBAR * 8;
+    static constexpr int SMEM_BYTES = MISC_OFF + 16 + 1024;
+    static_assert(SMEM_BYTES <= 232448, "shared memory plan exceeds 227 KB");
+};
+
+struct AttnQUnit {
+    int b, h, hk, q0, len, nk;
+};
+__device__ __forceinline__ AttnQUnit attn_q_unit(const AttnArgs &a, long long u) {
+    const int qt = a.Sqp / AT_TILE;
+    AttnQUnit w;
+    w.q0 = (int)(u % qt) * AT_TILE;
+    u /= qt;
+    w.h = (int)(u % a.H);
+    w.b = (int)(u / a.H);
+    w.hk = w.h / (a.H / a.HK);
+    w.len = attn_keys(a, w.b);
+    w.nk = (w.len + AT_TILE - 1) / AT_TILE;
+    return w;
+}
+
+template <int DT, int DP>
+__global__ void __launch_bounds__(AB_THREADS, 1)
+    attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const AttnArgs a,
+                   const long long units) {
+    using G = AttnQGeom<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_u32(smem);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
+    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *s_empty = bars + 4, *dp_full = bars + 6,
+             *ds_full = bars + 7, *acc_full = bars + 8, *acc_empty = bars + 9, *raw = bars + 10, *mma_done = bars + 11,
+             *k_full = bars + 13, *k_empty = k_full + G::NK, *v_full = k_empty + G::NK, *v_empty = v_full + G::NV;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + G::MISC_OFF);
+    volatile int *abort = reinterpret_cast<volatile int *>(smem + G::MISC_OFF + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 2);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&s_full[s], 1);
+            mbar_init(&s_empty[s], 8);
+            mbar_init(&mma_done[s], 1);
+        }
+        mbar_init(dp_full, 1);
+        mbar_init(ds_full, 8);
+        mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 8);
+        mbar_init(raw, 1);
+        for (int s = 0; s < G::NK; ++s) {
+            mbar_init(&k_full[s], 1);
+            mbar_init(&k_empty[s], 2);
+        }
+        for (int s = 0; s < G::NV; ++s) {
+            mbar_init(&v_full[s], 1);
+            mbar_init(&v_empty[s], 1);
+        }
+        *abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8) {
+        if (lane == 0) {
+            tma_prefetch_desc(&tmQ);
+            tma_prefetch_desc(&tmK);
+            tma_prefetch_desc(&tmV);
+            tma_prefetch_desc(&tmG);
+        }
+        __syncwarp();
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    griddep_wait();
+
+    if (warp == 8) {
+        // ------------------------------------------------------------ loads
+        at_fewer_registers();
+        uint32_t g = 0, nu = 0, nraw = 0;
+        bool good = true;
+        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+            const AttnQUnit w = attn_q_unit(a, u);
+            if (w.nk == 0) continue;
+            good = at_wait(q_empty, (nu++ & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_AB_EMPTY);
+            if (!good) break;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(q_full, 2 * G::TILE);
+                at_load_tile<DP>(sbase, &tmQ, w.q0, w.h, w.b, q_full);
+                at_load_tile<DP>(sbase + G::TILE, &tmG, w.q0, w.h, w.b, q_full);
+            }
+            for (int j = 0; j < w.nk; ++j, ++g) {
+                const int s = g % G::NK, t = g % G::NV;
+                good = at_wait(&k_empty[s], ((g / G::NK) & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_W_EMPTY);
+                if (!good) break;
+                // keys behind the length: zeroed in K (in V they only make values that are replaced)
+                const int rows = w.len - j * AT_TILE;
+                const bool fix = rows < AT_TILE && w.len < a.Sk;
+                uint64_t *bar = fix ? raw : &k_full[s];
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(bar, G::TILE);
+                    at_load_tile<DP>(sbase + G::K_OFF + s * G::TILE, &tmK, j * AT_TILE, w.hk, w.b, bar);
+                }
+                if (fix) {
+                    good = at_wait(raw, nraw++ & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
+                    at_zero_rows<DP>(smem + G::K_OFF + s * G::TILE, rows);
+                    if (lane == 0) mbar_arrive(&k_full[s]);
+                }
+                good = good && at_wait(&v_empty[t], ((g / G::NV) & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_W_EMPTY);
+                if (!good) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&v_full[t], G::TILE);
+                    at_load_tile<DP>(sbase + G::V_OFF + t * G::TILE, &tmV, j * AT_TILE, w.hk, w.b, &v_full[t]);
+                }
+            }
+        }
+    } else if (warp == 9) {
+        // ---------------------------------------------------------- MMAs: S
+        at_fewer_registers();
+        if (lane == 0) {
+            constexpr uint32_t id_s = idesc_f16(DT == DT_BF16 ? 1 : 0, 0, 0, 128, AT_TILE);
+            uint32_t g = 0, nu = 0;
+            bool good = true;
+            for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+                const AttnQUnit w = attn_q_unit(a, u);
+                if (w.nk == 0) continue;
+                good = wait_bar(q_full, nu++ & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
+                for (int j = 0; j < w.nk && good; ++j, ++g) {
+                    const int s = g % G::NK, t = g & 1;
+                    good = wait_bar(&k_full[s], (g / G::NK) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL) &&
+                           wait_bar(&s_empty[t], ((g >> 1) & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (!good) break;
+                    tc_fence_after();
+                    const uint32_t K = sbase + G::K_OFF + s * G::TILE;
+#pragma unroll
+                    for (int kk = 0; kk < DP / 16; ++kk)
+                        mma_f16_ss(tmem + 128 * t, at_desc_k(sbase, kk), at_desc_k(K, kk), id_s, kk > 0);
+                    mma_commit(&s_full[t]);
+                    mma_commit(&k_empty[s]);
+                }
+                if (good) mma_commit(q_empty);
+            }
+            mma_commit(&mma_done[0]);
+        }
+    } else if (warp == 11) {
+        at_fewer_registers();  // idle: completes the third group of four warps
+    } else if (warp == 10) {
+        // ---------------------------------------------------- MMAs: dP and dQ
+        at_fewer_registers();
+        if (lane == 0) {
+            constexpr int ab = DT == DT_BF16 ? 1 : 0;
+            constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
+            const uint32_t DS = tmem + 256, O = tmem + 384;
+            uint32_t g = 0, nu = 0, np = 0;
+            bool good = true;
+            auto scores = [&](uint32_t i) {
+                const int t = i % G::NV;
+                good = good && wait_bar(&v_full[t], (i / G::NV) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
+                if (!good) return;
+                tc_fence_after();
+                const uint32_t V = sbase + G::V_OFF + t * G::TILE;
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_f16_ss(DS, at_desc_k(sbase + G::TILE, kk), at_desc_k(V, kk), id_s, kk > 0);
+                mma_commit(dp_full);
+                mma_commit(&v_empty[t]);
+            };
+            for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+                const AttnQUnit w = attn_q_unit(a, u);
+                if (w.nk == 0) continue;
+                good = wait_bar(q_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
+                scores(g);
+                for (int j = 0; j < w.nk && good; ++j, ++g) {
+                    const int s = g % G::NK;
+                    if (j == w.nk - 1) mma_commit(q_empty);  // the last product with dO was issued
+                    good = wait_bar(&k_full[s], (g / G::NK) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL) &&
+                           wait_bar(ds_full, np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (j == 0) good = good && wait_bar(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (!good) break;
+                    tc_fence_after();
+                    const uint32_t K = sbase + G::K_OFF + s * G::TILE;
+#pragma unroll
+                    for (int kk = 0; kk < AT_TILE / 16; ++kk)
+                        at_mma_ts(O, DS + (kk >> 2) * 64 + (kk & 3) * 8, at_desc_mn(K, kk), id_o, j > 0 || kk > 0);
+                    mma_commit(&k_empty[s]);
+                    if (j + 1 < w.nk) scores(g + 1);
+                }
+                if (!good) break;
+                mma_commit(acc_full);
+                ++nu;
+            }
+            mma_commit(&mma_done[1]);
+        }
+    } else {
+        // ----------------------------------------------------- dS and the output
+        at_more_registers();
+        const int half = warp >> 2;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t DS = tmem + lanes + 256 + 64 * half, O = tmem + lanes + 384;
+        const float c = a.scale * CUDART_L2E_F;
+        const int e = attn_grad_exp<DT>(a);
+        const float grow = exp2f((float)e), f = a.scale * exp2f(-(float)e);
+        uint32_t g = 0, nu = 0;
+        bool good = true;
+        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+            const AttnQUnit w = attn_q_unit(a, u);
+            const int row = w.q0 + (warp & 3) * 32 + lane;
+            const long long st = ((long long)w.b * a.H + w.h) * a.Sqp + row;
+            const float L = __ldcg(a.stat_l + st), delta = __ldcg(a.stat_d + st);
+            for (int j = 0; j < w.nk; ++j, ++g) {
+                const int t = g & 1;
+                good = at_wait(&s_full[t], (g >> 1) & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                if (!good) break;
+                tc_fence_after();
+                uint32_t x[64];
+                at_tmem_ld32(tmem + lanes + 128 * t + 64 * half, x);
+                at_tmem_ld32(tmem + lanes + 128 * t + 64 * half + 32, x + 32);
+                tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_empty[t]);
+#pragma unroll
+                for (int k = 0; k < 64; ++k) x[k] = __float_as_uint(at_exp2(fmaf(__uint_as_float(x[k]), c, -L)));
+                good = at_wait(dp_full, g & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                if (!good) break;
+                tc_fence_after();
+                uint32_t y[64];
+                at_tmem_ld32(DS, y);
+                at_tmem_ld32(DS + 32, y + 32);
+                tmem_wait_ld();
+                const int rows = w.len - j * AT_TILE - 64 * half;
+#pragma unroll
+                for (int k = 0; k < 64; ++k) {
+                    float v = __uint_as_float(x[k]) * (__uint_as_float(y[k]) - delta);
+                    if (DT == DT_F16) v *= grow;
+                    y[k] = __float_as_uint(v);
+                }
+                if (rows < 64) {
+#pragma unroll
+                    for (int k = 0; k < 64; ++k)
+                        if (k >= rows) y[k] = 0u;
+                }
+                uint32_t p[32];
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                    p[k] = Elem<DT>::pack2(__uint_as_float(y[2 * k]), __uint_as_float(y[2 * k + 1]));
+                at_tmem_st32(DS, p);
+                at_tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ds_full);
+            }
+            if (!good) break;
+            if (w.nk > 0) {
+                good = at_wait(acc_full, nu++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                if (!good) break;
+                tc_fence_after();
+            }
+            // the two groups of warps write half of the features each
+            auto *dst = reinterpret_cast<typename Elem<DT>::T *>(a.dq) +
+                        (((long long)w.b * a.Sq + row) * a.H + w.h) * a.D;
+#pragma unroll
+            for (int i = 0; i < DP / 64; ++i) {
+                const int c0 = half * (DP / 2) + 32 * i;
+                uint32_t o[32];
+                if (w.nk > 0) {
+                    at_tmem_ld32(O + c0, o);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = 0u;
+                }
+                if (i == DP / 64 - 1 && w.nk > 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acc_empty);
+                }
+                if (row < a.Sq) ab_store32<DT>(o, f, dst, nullptr, c0, a.D);
+                __syncwarp();
+            }
+        }
+    }
+
+    if (*abort) {
+        for (int i = 0; i < 64; ++i) __nanosleep(2000);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) ab_finish(tmem, mma_done, a.err);
+}
+
+}  // namespace reels

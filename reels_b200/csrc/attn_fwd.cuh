@@ -1,0 +1,365 @@
+// Softmax attention forward on the 5th-gen tensor cores (sm_100a).
+//
+// A work unit is 256 queries of one head (two tiles of 128) against a range
+// of its keys, walked 128 at a time with a running maximum and sum:
+//   S_t = Q_t K'   (128 x 128, fp32 in tensor memory)
+//   P_t = exp2(S_t c - m)      c = scale log2(e)
+//   O_t += P_t V   (P_t as 16-bit operand in tensor memory, over S_t)
+// The two tiles share every K and V tile and alternate: while one tile's
+// softmax runs on the CUDA cores, the other's two products run on the tensor
+// core.  A product of 128 x 128 x D takes as long as the exponentials of
+// its tile, so the two sides are balanced by construction.
+//
+// The running maximum lags: O is rescaled only when a row's maximum outgrows
+// the one in use by 2^8, which leaves every term below 2^8 (exact in the fp32
+// sums' range) and makes rescaling rare.  S_t(j) is issued behind PV_t(j-1) by
+// the same thread, so its completion also means that O_t may be rescaled.
+//
+// Warps: 0-3 and 4-7 softmax and output of tile 0 and 1 (a thread a row),
+// 8 loads, 9 and 10 the tiles' MMA issuers (one thread cannot issue
+// 128-column MMAs at the rate the tensor core takes them; two can).
+// TMEM: S0, S1, O0, O1, 128 columns each.  Persistent, one CTA per SM.
+#pragma once
+#include "attn_common.cuh"
+
+namespace reels {
+
+constexpr int AF_THREADS = 32 * 12;
+
+template <int DP>
+struct AttnFwdGeom {
+    static constexpr int TILE = AT_TILE * DP * 2;
+    static constexpr int NST = DP == 128 ? 5 : 8;  // K and V tiles in flight
+    static constexpr int KV_OFF = 2 * TILE;
+    static constexpr int BAR_OFF = KV_OFF + NST * TILE;
+    // q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2], mma_done[2], raw, kv_full, kv_empty
+    static constexpr int NBAR = 15 + 2 * NST;
+    static constexpr int MISC_OFF = BAR_OFF + NBAR * 8;
+    static constexpr int SMEM_BYTES = MISC_OFF + 16 + 1024;
+    static_assert(SMEM_BYTES <= 232448, "shared memory plan exceeds 227 KB");
+};
+
+struct AttnUnit {
+    int b, h, hk, q0, tiles, split;
+    int k0, kn;  // first key, keys (0: nothing to do but write the empty result)
+    int nk;      // key tiles
+};
+
+// Unit u: query tile pairs fastest, so that neighbouring CTAs read the same keys.
+__device__ __forceinline__ AttnUnit attn_unit(const AttnArgs &a, long long u) {
+    const int pairs = (a.Sq + 2 * AT_TILE - 1) / (2 * AT_TILE);
+    AttnUnit w;
+    w.q0 = (int)(u % pairs) * 2 * AT_TILE;
+    u /= pairs;
+    w.h = (int)(u % a.H);
+    u /= a.H;
+    w.b = (int)(u % a.B);
+    w.split = (int)(u / a.B);
+    w.hk = w.h / (a.H / a.HK);
+    w.tiles = a.Sq - w.q0 > AT_TILE ? 2 : 1;
+    const int len = attn_keys(a, w.b);
+    w.k0 = min(len, w.split * a.split_keys);
+    w.kn = min(len, w.k0 + a.split_keys) - w.k0;
+    w.nk = (w.kn + AT_TILE - 1) / AT_TILE;
+    return w;
+}
+
+template <int DT, int DP>
+__global__ void __launch_bounds__(AF_THREADS, 1)
+    attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                    const __grid_constant__ CUtensorMap tmV, const AttnArgs a, const long long units) {
+    using G = AttnFwdGeom<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_u32(smem);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
+    uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 8,
+             *o_empty = bars + 10, *mma_done = bars + 12, *raw = bars + 14, *kv_full = bars + 15,
+             *kv_empty = bars + 15 + G::NST;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + G::MISC_OFF);
+    volatile int *abort = reinterpret_cast<volatile int *>(smem + G::MISC_OFF + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&q_full[t], 1);
+            mbar_init(&q_empty[t], 1);
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_full[t], 4);
+            mbar_init(&o_full[t], 1);
+            mbar_init(&o_empty[t], 4);
+            mbar_init(&mma_done[t], 1);
+        }
+        mbar_init(raw, 1);
+        for (int s = 0; s < G::NST; ++s) {
+            mbar_init(&kv_full[s], 1);
+            mbar_init(&kv_empty[s], 2);
+        }
+        *abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8) {
+        if (lane == 0) {
+            tma_prefetch_desc(&tmQ);
+            tma_prefetch_desc(&tmK);
+            tma_prefetch_desc(&tmV);
+        }
+        __syncwarp();
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    griddep_wait();
+
+    if (warp == 8) {
+        // ------------------------------------------------------------ loads
+        at_fewer_registers();
+        uint32_t g = 0, qn[2] = {0, 0}, nraw = 0;
+        bool good = true;
+        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+            const AttnUnit w = attn_unit(a, u);
+            if (w.nk == 0) continue;
+            auto load_q = [&](int t) {
+                good = good && at_wait(&q_empty[t], (qn[t] & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_AB_EMPTY);
+                if (!good) return;
+                ++qn[t];
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&q_full[t], G::TILE);
+                    at_load_tile<DP>(sbase + t * G::TILE, &tmQ, w.q0 + t * AT_TILE, w.h, w.b, &q_full[t]);
+                }
+            };
+            auto load_kv = [&](int j, bool is_v) {
+                const int s = g % G::NST;
+                good = good && at_wait(&kv_empty[s], ((g / G::NST) & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_W_EMPTY);
+                if (!good) return;
+                ++g;
+                // keys behind the range: zeroed in V (in K they only make scores that are replaced)
+                const int rows = w.kn - j * AT_TILE;
+                const bool fix = is_v && rows < AT_TILE && w.k0 + w.kn < a.Sk;
+                const uint32_t dst = sbase + G::KV_OFF + s * G::TILE;
+                uint64_t *bar = fix ? raw : &kv_full[s];
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(bar, G::TILE);
+                    at_load_tile<DP>(dst, is_v ? &tmV : &tmK, w.k0 + j * AT_TILE, w.hk, w.b, bar);
+                }
+                if (fix) {
+                    good = at_wait(raw, nraw++ & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
+                    at_zero_rows<DP>(smem + G::KV_OFF + s * G::TILE, rows);
+                    if (lane == 0) mbar_arrive(&kv_full[s]);
+                }
+            };
+            load_q(0);
+            load_kv(0, false);
+            if (w.tiles == 2) load_q(1);
+            load_kv(0, true);
+            for (int j = 1; j < w.nk && good; ++j) {
+                load_kv(j, false);
+                load_kv(j, true);
+            }
+        }
+    } else if (warp == 11) {
+        at_fewer_registers();  // idle: completes the third group of four warps
+    } else if (warp > 8) {
+        // -------------------------------------------------------------- MMAs
+        at_fewer_registers();
+        const int t = warp - 9;
+        if (lane == 0) {
+            constexpr int ab = DT == DT_BF16 ? 1 : 0;
+            constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
+            const uint32_t S = tmem + t * 128, O = tmem + 256 + t * 128, Q = sbase + t * G::TILE;
+            uint32_t g = 0, np = 0, nu = 0;
+            bool good = true;
+            auto wait_kv = [&](uint32_t i) {
+                good = good && wait_bar(&kv_full[i % G::NST], (i / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
+                tc_fence_after();
+            };
+            auto scores = [&](uint32_t i) {
+                const uint32_t K = sbase + G::KV_OFF + (i % G::NST) * G::TILE;
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) mma_f16_ss(S, at_desc_k(Q, kk), at_desc_k(K, kk), id_s, kk > 0);
+                mma_commit(&s_full[t]);
+                mma_commit(&kv_empty[i % G::NST]);
+            };
+            for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+                const AttnUnit w = attn_unit(a, u);
+                if (w.nk == 0) continue;
+                if (t >= w.tiles) {  // no second tile: only pass the ring on
+                    for (int j = 0; j < 2 * w.nk && good; ++j, ++g) {
+                        wait_kv(g);
+                        mbar_arrive(&kv_empty[g % G::NST]);
+                    }
+                    continue;
+                }
+                good = wait_bar(&q_full[t], nu & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
+                wait_kv(g);
+                if (!good) break;
+                scores(g);
+                for (int j = 0; j < w.nk; ++j, g += 2) {
+                    if (j == w.nk - 1) mma_commit(&q_empty[t]);  // the last scores were issued
+                    wait_kv(g + 1);
+                    good = good && wait_bar(&p_full[t], np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (j == 0) good = good && wait_bar(&o_empty[t], (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (!good) break;
+                    tc_fence_after();
+                    const uint32_t V = sbase + G::KV_OFF + ((g + 1) % G::NST) * G::TILE;
+#pragma unroll
+                    for (int kk = 0; kk < AT_TILE / 16; ++kk)
+                        at_mma_ts(O, S + kk * 8, at_desc_mn(V, kk), id_o, j > 0 || kk > 0);
+                    mma_commit(&kv_empty[(g + 1) % G::NST]);
+                    if (j + 1 < w.nk) {
+                        wait_kv(g + 2);
+                        if (!good) break;
+                        scores(g + 2);
+                    }
+                }
+                if (!good) break;
+                mma_commit(&o_full[t]);
+                ++nu;
+            }
+            mma_commit(&mma_done[t]);
+        }
+    } else {
+        // ------------------------------------------------- softmax and output
+        at_more_registers();
+        const int t = warp >> 2;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t S = tmem + t * 128 + lanes, O = tmem + 256 + t * 128 + lanes;
+        const float c = a.scale * CUDART_L2E_F;
+        uint32_t ns = 0, nu = 0;
+        bool good = true;
+        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+            const AttnUnit w = attn_unit(a, u);
+            if (t >= w.tiles) continue;
+            const int row = w.q0 + t * AT_TILE + (warp & 3) * 32 + lane;
+            float m = 0.0f, l = 0.0f;  // m: the maximum in use, in log2 units, less the fp16 shift
+            for (int j = 0; j < w.nk; ++j) {
+                good = at_wait(&s_full[t], ns++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                if (!good) break;
+                tc_fence_after();
+                uint32_t s[AT_TILE];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) at_tmem_ld32(S + 32 * i, s + 32 * i);
+                tmem_wait_ld();
+                const int rows = w.kn - j * AT_TILE;
+                if (rows < AT_TILE) {
+#pragma unroll
+                    for (int i = 0; i < AT_TILE; ++i)
+                        if (i >= rows) s[i] = 0xff800000u;  // -inf
+                }
+                float mx[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s[i]);
+#pragma unroll
+                for (int i = 4; i < AT_TILE; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                top = (top == -CUDART_INF_F ? 0.0f : top) - AtRange<DT>::FWD_SHIFT;
+                if (j == 0) m = top;
+                else if (__any_sync(0xffffffffu, top - m > 8.0f)) {
+                    const float to = top - m > 8.0f ? top : m, keep = at_exp2(m - to);
+                    m = to;
+                    l *= keep;
+#pragma unroll
+                    for (int i = 0; i < DP / 32; ++i) {
+                        uint32_t o[32];
+                        at_tmem_ld32(O + 32 * i, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                        at_tmem_st32(O + 32 * i, o);
+                    }
+                }
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float x = at_exp2(fmaf(__uint_as_float(s[32 * i + 2 * e]), c, -m));
+                        const float y = at_exp2(fmaf(__uint_as_float(s[32 * i + 2 * e + 1]), c, -m));
+                        p[e] = Elem<DT>::pack2(x, y);
+                        sum[e & 1] += x;
+                        sum[2 + (e & 1)] += y;
+                    }
+                    at_tmem_st16(S + 16 * i, p);
+                }
+                at_tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t]);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            }
+            if (!good) break;
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            const float lse = w.nk > 0 ? (m + log2f(l)) * CUDART_LN2_F : -CUDART_INF_F;
+            const long long at = ((long long)w.split * a.B + w.b) * a.H + w.h;
+            const bool in = row < a.Sq;
+            if (in) (a.splits > 1 ? a.part_lse : a.lse)[at * a.Sq + row] = lse;
+            if (w.nk > 0) {
+                good = at_wait(&o_full[t], nu++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                if (!good) break;
+                tc_fence_after();
+            }
+            typename Elem<DT>::T *out = reinterpret_cast<typename Elem<DT>::T *>(a.out) +
+                                        (((long long)w.b * a.Sq + row) * a.H + w.h) * a.D;
+            float *part = a.part_o + (at * a.Sq + row) * a.D;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                uint32_t o[32];
+                if (w.nk > 0) {
+                    at_tmem_ld32(O + 32 * i, o);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;
+                }
+                if (i == DP / 32 - 1 && w.nk > 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&o_empty[t]);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    if (!in || 32 * i + e >= a.D) continue;
+                    float v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[e + k]) * inv;
+                    if (a.splits > 1) {
+                        float4 *dst = reinterpret_cast<float4 *>(part + 32 * i + e);
+                        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                    } else {
+                        *reinterpret_cast<uint4 *>(out + 32 * i + e) =
+                            make_uint4(Elem<DT>::pack2(v[0], v[1]), Elem<DT>::pack2(v[2], v[3]),
+                                       Elem<DT>::pack2(v[4], v[5]), Elem<DT>::pack2(v[6], v[7]));
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+
+    if (*abort) {  // give the copies in flight time to land before the CTA's shared memory goes
+        for (int i = 0; i < 64; ++i) __nanosleep(2000);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        for (int t = 0; t < 2; ++t) {
+            const long long t0 = clock64();
+            while (!mbar_try_wait(&mma_done[t], 0)) {
+                if (clock64() - t0 > REELS_WAIT_LIMIT_CYCLES) {
+                    if (lane == 0) atomicOr(a.err, DEVERR_TIMEOUT_ACC);
+                    break;
+                }
+            }
+        }
+        __syncwarp();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace reels

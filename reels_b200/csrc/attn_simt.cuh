@@ -1,0 +1,386 @@
+// Softmax attention and its gradient on the CUDA cores: fp32 tensors, head
+// sizes that are no multiple of 8 or above 128, and strides the tensor-core
+// kernels (attn_fwd.cuh, attn_bwd.cuh) cannot read.  Also the small kernels
+// both share: the join of key splits and the gradient's row statistics.
+//
+//   S = scale q k',  P = softmax over the keys before the sample's length,
+//   O = P v,  L = log sum exp S
+//   delta = rowsum(dO * O),  P = exp(S - L),  dS = P * (dO v' - delta)
+//   dV = P' dO,  dQ = scale dS k,  dK = scale dS' q
+// A row without keys has O = 0, L = -inf and no part in any gradient.
+//
+// 32 x 32 tiles of S in registers (2 x 4 a thread, 128 threads), operands in
+// shared memory as fp32; every sum is fp32 and in a fixed order.
+#pragma once
+#include <math_constants.h>
+
+#include "common.cuh"
+
+namespace reels {
+
+constexpr int AT_MAX_D = 256;  // head size
+constexpr int AS_T = 32;       // tile of the CUDA-core kernels
+constexpr int AS_THREADS = 128;
+
+struct AttnArgs {
+    const void *q, *k, *v;                   // [batch][token][head][D] by strides, D contiguous
+    long long qs[3], ks[3], vs[3];           // batch, token and head strides in elements
+    const int *lengths;                      // [B] keys of a sample, nullable
+    int B, H, HK, Sq, Sk, D;
+    float scale;
+    void *out;                               // [B][Sq][H][D]
+    float *lse;                              // [B][H][Sq]
+    int splits, split_keys;                  // forward: key ranges of a row and their length
+    float *part_o, *part_lse;                // [splits][B][H][Sq][D], [splits][B][H][Sq]
+    // backward
+    const void *dout;                        // [B][Sq][H][D]
+    const float *stat_l, *stat_d;            // [B][H][Sqp]: L in log2 units (+inf: no part), delta
+    int Sqp;                                 // Sq rounded up to whole tiles
+    void *dq, *dk, *dv;                      // contiguous, in the layout of q, k and v
+    const unsigned *range;                   // fp16: largest |dO row|, |v row| (float bits)
+    int red_splits;                          // dK, dV: ranges of the (head, query tile) walk
+    float *part_k, *part_v;                  // [red_splits][B][Sk][HK][D]
+    unsigned *err;
+};
+
+// Keys of sample b that take part.
+__device__ __forceinline__ int attn_keys(const AttnArgs &a, int b) {
+    if (!a.lengths) return a.Sk;
+    const int n = __ldcg(a.lengths + b);
+    return n < 0 ? 0 : (n < a.Sk ? n : a.Sk);
+}
+
+// 32 rows of D elements into dst[32][DP + 4], rows from `n` on and features from D on as zeros.
+template <int DT, int DP>
+__device__ __forceinline__ void as_load(float *dst, const void *src, long long at, long long pitch, int n, int D) {
+    for (int i = threadIdx.x; i < AS_T * DP; i += AS_THREADS) {
+        const int r = i / DP, d = i - r * DP;
+        dst[r * (DP + 4) + d] = (r < n && d < D) ? load_act(src, at + r * pitch + d, DT) : 0.0f;
+    }
+}
+// acc[i][j] = A[2 ty + i] . B[tx + 8 j]
+template <int DP>
+__device__ __forceinline__ void as_dot(const float *A, const float *B, int ty, int tx, float (&acc)[2][4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+#pragma unroll 4
+    for (int d = 0; d < DP; d += 4) {
+        float4 x[2], y[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[i] = *reinterpret_cast<const float4 *>(A + (2 * ty + i) * (DP + 4) + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4 *>(B + (tx + 8 * j) * (DP + 4) + d);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                acc[i][j] += x[i].x * y[j].x + x[i].y * y[j].y + x[i].z * y[j].z + x[i].w * y[j].w;
+    }
+}
+// acc[i][c][.] += sum_n W(2 ty + i, n) B[n][4 tx + 32 c ..]; W(r, n) = w[r * rs + n * ns]
+template <int DP>
+__device__ __forceinline__ void as_mix(const float *w, int rs, int ns, const float *B, int ty, int tx,
+                                       float (&acc)[2][DP / 32][4]) {
+#pragma unroll 2
+    for (int n = 0; n < AS_T; ++n) {
+        const float w0 = w[(2 * ty) * rs + n * ns], w1 = w[(2 * ty + 1) * rs + n * ns];
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c) {
+            const float4 b = *reinterpret_cast<const float4 *>(B + n * (DP + 4) + 4 * tx + 32 * c);
+            acc[0][c][0] += w0 * b.x, acc[0][c][1] += w0 * b.y, acc[0][c][2] += w0 * b.z, acc[0][c][3] += w0 * b.w;
+            acc[1][c][0] += w1 * b.x, acc[1][c][1] += w1 * b.y, acc[1][c][2] += w1 * b.z, acc[1][c][3] += w1 * b.w;
+        }
+    }
+}
+__host__ __device__ constexpr int as_smem_bytes(int DP, int tiles) {
+    return (tiles * AS_T * (DP + 4) + 2 * AS_T * (AS_T + 1)) * 4;
+}
+
+// grid: query tiles * B * H, splits
+template <int DT, int DP>
+__global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(const AttnArgs a) {
+    extern __shared__ float sm[];
+    float *Q = sm, *K = Q + AS_T * (DP + 4), *V = K + AS_T * (DP + 4), *P = V + AS_T * (DP + 4);
+    griddep_wait();
+    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const int tiles = (a.Sq + AS_T - 1) / AS_T, bh = (int)(blockIdx.x / tiles);
+    const int q0 = (int)(blockIdx.x % tiles) * AS_T, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.HK);
+    const int len = attn_keys(a, b);
+    const int k_begin = min(len, (int)blockIdx.y * a.split_keys), k_end = min(len, k_begin + a.split_keys);
+    as_load<DT, DP>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
+    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.0f, 0.0f}, o[2][DP / 32][4] = {};
+    for (int k0 = k_begin; k0 < k_end; k0 += AS_T) {
+        __syncthreads();
+        as_load<DT, DP>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], k_end - k0, a.D);
+        as_load<DT, DP>(V, a.v, b * a.vs[0] + k0 * a.vs[1] + hk * a.vs[2], a.vs[1], k_end - k0, a.D);
+        __syncthreads();
+        float s[2][4];
+        as_dot<DP>(Q, K, ty, tx, s);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float mx = -CUDART_INF_F;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[i][j] = k0 + tx + 8 * j < k_end ? s[i][j] * a.scale : -CUDART_INF_F;
+                mx = fmaxf(mx, s[i][j]);
+            }
+#pragma unroll
+            for (int w = 1; w < 8; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+            mx = fmaxf(m[i], mx);
+            const float ref = mx == -CUDART_INF_F ? 0.0f : mx;
+            const float keep = expf(m[i] - ref);
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = expf(s[i][j] - ref);
+                P[(2 * ty + i) * (AS_T + 1) + tx + 8 * j] = p;
+                sum += p;
+            }
+#pragma unroll
+            for (int w = 1; w < 8; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+            l[i] = l[i] * keep + sum;
+            m[i] = mx;
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][c][e] *= keep;
+        }
+        __syncwarp();  // the rows of P that a warp reads are its own
+        as_mix<DP>(P, AS_T + 1, 1, V, ty, tx, o);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int q = q0 + 2 * ty + i;
+        if (q >= a.Sq) continue;
+        const float inv = l[i] > 0.0f || l[i] != l[i] ? 1.0f / l[i] : 0.0f;
+        const float lse = (m[i] == -CUDART_INF_F ? 0.0f : m[i]) + logf(l[i]);
+        const long long at = ((long long)blockIdx.y * a.B + b) * a.H + h;
+        if (tx == 0) (a.splits > 1 ? a.part_lse : a.lse)[at * a.Sq + q] = lse;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = 4 * tx + 32 * c + e;
+                if (d >= a.D) continue;
+                const float v = o[i][c][e] * inv;
+                if (a.splits > 1) a.part_o[(at * a.Sq + q) * a.D + d] = v;
+                else store_act(a.out, (((long long)b * a.Sq + q) * a.H + h) * a.D + d, DT, v);
+            }
+    }
+}
+
+// Joins the key splits of a row: weights exp(L_i - L), splits in order.  One warp a row.
+template <int DT>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
+    griddep_wait();
+    const int lane = threadIdx.x & 31;
+    const long long rows = (long long)a.B * a.H * a.Sq;
+    for (long long row = blockIdx.x * 8ll + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8ll) {
+        float m = -CUDART_INF_F;
+        bool nan = false;
+        for (int s = lane; s < a.splits; s += 32) {
+            const float x = __ldcg(a.part_lse + s * rows + row);
+            m = fmaxf(m, x);
+            nan |= x != x;
+        }
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+        if (__any_sync(0xffffffffu, nan)) m = CUDART_NAN_F;
+        const float ref = m == -CUDART_INF_F ? 0.0f : m;
+        float total = 0.0f;
+        for (int s = 0; s < a.splits; ++s) total += expf(__ldcg(a.part_lse + s * rows + row) - ref);
+        const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+        if (lane == 0) a.lse[row] = ref + logf(total);
+        const int q = (int)(row % a.Sq), h = (int)(row / a.Sq % a.H), b = (int)(row / a.Sq / a.H);
+        for (int d = lane; d < a.D; d += 32) {
+            float acc = 0.0f;
+#pragma unroll 4
+            for (int s = 0; s < a.splits; ++s)
+                acc += expf(__ldcg(a.part_lse + s * rows + row) - ref) * __ldcg(a.part_o + (s * rows + row) * a.D + d);
+            store_act(a.out, (((long long)b * a.Sq + q) * a.H + h) * a.D + d, DT, acc * inv);
+        }
+    }
+}
+
+// Row statistics of the gradient: (L in log2 units, delta) of every query row,
+// padded to Sqp rows a head.  Rows without keys and padding get L = +inf, so
+// their probabilities come out as exp2(-inf) = 0.  One warp a row.
+template <int DT>
+__global__ void __launch_bounds__(256) attn_stat_kernel(const AttnArgs a, float *stat_l, float *stat_d, unsigned *range) {
+    griddep_wait();
+    const int lane = threadIdx.x & 31;
+    const long long rows = (long long)a.B * a.H * a.Sqp;
+    float top = 0.0f;  // fp16: largest |dO row|^2
+    for (long long row = blockIdx.x * 8ll + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8ll) {
+        const int q = (int)(row % a.Sqp), h = (int)(row / a.Sqp % a.H), b = (int)(row / a.Sqp / a.H);
+        float2 st = make_float2(CUDART_INF_F, 0.0f);
+        if (q < a.Sq) {
+            const long long at = (((long long)b * a.Sq + q) * a.H + h) * a.D;
+            float delta = 0.0f, n2 = 0.0f;
+            if (DT != DT_F32 && (a.D & 7) == 0) {
+                for (int d = 8 * lane; d < a.D; d += 256) {
+                    const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(
+                        reinterpret_cast<const typename Elem<DT>::T *>(a.dout) + at + d));
+                    const uint4 y = __ldcg(reinterpret_cast<const uint4 *>(
+                        reinterpret_cast<const typename Elem<DT>::T *>(a.out) + at + d));
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float g = load_act(&x, j, DT);
+                        delta += g * load_act(&y, j, DT);
+                        n2 += g * g;
+                    }
+                }
+            } else {
+                for (int d = lane; d < a.D; d += 32) {
+                    const float g = load_act(a.dout, at + d, DT);
+                    delta += g * load_act(a.out, at + d, DT);
+                    n2 += g * g;
+                }
+            }
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) {
+                delta += __shfl_xor_sync(0xffffffffu, delta, w);
+                n2 += __shfl_xor_sync(0xffffffffu, n2, w);
+            }
+            const float lse = __ldcg(a.lse + ((long long)b * a.H + h) * a.Sq + q);
+            if (lse != -CUDART_INF_F) st = make_float2(lse * CUDART_L2E_F, delta);
+            top = fmaxf(top, n2);
+        }
+        if (lane == 0) {
+            stat_l[row] = st.x;
+            stat_d[row] = st.y;
+        }
+    }
+    if (range && lane == 0) atomicMax(range, __float_as_uint(sqrtf(top)));
+}
+
+// fp16: the largest |v row|, so that the gradients' operands can be held in
+// range.  A maximum does not depend on the order of its atomics.
+template <int DT>
+__global__ void __launch_bounds__(256) attn_range_kernel(const AttnArgs a, unsigned *range) {
+    griddep_wait();
+    const int lane = threadIdx.x & 31;
+    const long long rows = (long long)a.B * a.HK * a.Sk;
+    float top = 0.0f;
+    for (long long row = blockIdx.x * 8ll + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8ll) {
+        const int h = (int)(row % a.HK), t = (int)(row / a.HK % a.Sk), b = (int)(row / a.HK / a.Sk);
+        if (t >= attn_keys(a, b)) continue;
+        const long long at = b * a.vs[0] + t * a.vs[1] + h * a.vs[2];
+        float n2 = 0.0f;
+        for (int d = lane; d < a.D; d += 32) {
+            const float x = load_act(a.v, at + d, DT);
+            n2 += x * x;
+        }
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, w);
+        top = fmaxf(top, n2);
+    }
+    if (lane == 0) atomicMax(range, __float_as_uint(sqrtf(top)));
+}
+
+// P and dS of one 32 x 32 tile into shared memory, [query][key].
+template <int DP>
+__device__ __forceinline__ void as_grad_tile(const AttnArgs &a, const float *Q, const float *K, const float *V,
+                                             const float *G, float *P, float *S, long long stat_at, int k0, int len,
+                                             int ty, int tx) {
+    float s[2][4], dp[2][4];
+    as_dot<DP>(Q, K, ty, tx, s);
+    as_dot<DP>(G, V, ty, tx, dp);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float2 st = make_float2(__ldcg(a.stat_l + stat_at + 2 * ty + i), __ldcg(a.stat_d + stat_at + 2 * ty + i));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool in = k0 + tx + 8 * j < len && st.x != CUDART_INF_F;
+            const float p = in ? exp2f(s[i][j] * a.scale * CUDART_L2E_F - st.x) : 0.0f;
+            const int at = (2 * ty + i) * (AS_T + 1) + tx + 8 * j;
+            P[at] = p;
+            S[at] = in ? p * (dp[i][j] - st.y) : 0.0f;
+        }
+    }
+}
+
+// dK and dV of a tile of keys: all query tiles of all heads that share it.  grid: key tiles * B * HK
+template <int DT, int DP>
+__global__ void __launch_bounds__(AS_THREADS) attn_simt_dkdv_kernel(const AttnArgs a) {
+    extern __shared__ float sm[];
+    constexpr int T = AS_T * (DP + 4);
+    float *K = sm, *V = K + T, *Q = V + T, *G = Q + T, *P = G + T, *S = P + AS_T * (AS_T + 1);
+    griddep_wait();
+    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const int tiles = (a.Sk + AS_T - 1) / AS_T, bh = (int)(blockIdx.x / tiles);
+    const int k0 = (int)(blockIdx.x % tiles) * AS_T, b = bh / a.HK, hk = bh % a.HK, group = a.H / a.HK;
+    const int len = attn_keys(a, b);
+    as_load<DT, DP>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], len - k0, a.D);
+    as_load<DT, DP>(V, a.v, b * a.vs[0] + k0 * a.vs[1] + hk * a.vs[2], a.vs[1], len - k0, a.D);
+    float dk[2][DP / 32][4] = {}, dv[2][DP / 32][4] = {};
+    for (int h = hk * group; h < (hk + 1) * group && k0 < len; ++h)
+        for (int q0 = 0; q0 < a.Sq; q0 += AS_T) {
+            __syncthreads();
+            as_load<DT, DP>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
+            as_load<DT, DP>(G, a.dout, (((long long)b * a.Sq + q0) * a.H + h) * a.D, (long long)a.H * a.D, a.Sq - q0,
+                            a.D);
+            __syncthreads();
+            as_grad_tile<DP>(a, Q, K, V, G, P, S, ((long long)b * a.H + h) * a.Sqp + q0, k0, len, ty, tx);
+            __syncthreads();
+            as_mix<DP>(P, 1, AS_T + 1, G, ty, tx, dv);
+            as_mix<DP>(S, 1, AS_T + 1, Q, ty, tx, dk);
+        }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t = k0 + 2 * ty + i;
+        if (t >= a.Sk) continue;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = 4 * tx + 32 * c + e;
+                if (d >= a.D) continue;
+                const long long at = (((long long)b * a.Sk + t) * a.HK + hk) * a.D + d;
+                store_act(a.dk, at, DT, t < len ? dk[i][c][e] * a.scale : 0.0f);
+                store_act(a.dv, at, DT, t < len ? dv[i][c][e] : 0.0f);
+            }
+    }
+}
+
+// dQ of a tile of queries.  grid: query tiles * B * H
+template <int DT, int DP>
+__global__ void __launch_bounds__(AS_THREADS) attn_simt_dq_kernel(const AttnArgs a) {
+    extern __shared__ float sm[];
+    constexpr int T = AS_T * (DP + 4);
+    float *K = sm, *V = K + T, *Q = V + T, *G = Q + T, *P = G + T, *S = P + AS_T * (AS_T + 1);
+    griddep_wait();
+    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const int tiles = (a.Sq + AS_T - 1) / AS_T, bh = (int)(blockIdx.x / tiles);
+    const int q0 = (int)(blockIdx.x % tiles) * AS_T, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.HK);
+    const int len = attn_keys(a, b);
+    as_load<DT, DP>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
+    as_load<DT, DP>(G, a.dout, (((long long)b * a.Sq + q0) * a.H + h) * a.D, (long long)a.H * a.D, a.Sq - q0, a.D);
+    float dq[2][DP / 32][4] = {};
+    for (int k0 = 0; k0 < len; k0 += AS_T) {
+        __syncthreads();
+        as_load<DT, DP>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], len - k0, a.D);
+        as_load<DT, DP>(V, a.v, b * a.vs[0] + k0 * a.vs[1] + hk * a.vs[2], a.vs[1], len - k0, a.D);
+        __syncthreads();
+        as_grad_tile<DP>(a, Q, K, V, G, P, S, ((long long)b * a.H + h) * a.Sqp + q0, k0, len, ty, tx);
+        __syncwarp();  // the rows of S that a warp reads are its own
+        as_mix<DP>(S, AS_T + 1, 1, K, ty, tx, dq);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t = q0 + 2 * ty + i;
+        if (t >= a.Sq) continue;
+#pragma unroll
+        for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = 4 * tx + 32 * c + e;
+                if (d < a.D)
+                    store_act(a.dq, (((long long)b * a.Sq + t) * a.H + h) * a.D + d, DT, dq[i][c][e] * a.scale);
+            }
+    }
+}
+
+}  // namespace reels

@@ -28,6 +28,7 @@ enum DevErr : unsigned {
     DEVERR_OPT_TABLE = 512u,  // an optimizer workspace that was not prepared
     // a row whose max|w| / 127 underflows to 0 holds a zero: 0 / 0 is NaN
     DEVERR_QUANT_NAN = 1024u,
+    DEVERR_ROPE_POSITION = 2048u,  // a rotary position behind its table
 };
 
 // ---------------------------------------------------------------- elements

@@ -14,6 +14,7 @@
 
 #include "../../include/reels_lowvram.h"
 #include "aux_kernels.cuh"
+#include "host.h"
 #include "q8_gemm.cuh"
 #include "dropout.cuh"
 #include "norm.cuh"
@@ -1283,6 +1284,41 @@ int prep_lora(int dt, int ext_kind, const void *B, const float *scales, float s,
 
 }  // namespace
 
+// Host services for the library's other translation units (host.h).
+namespace reels {
+int host_fail(const std::string &msg) { return fail(msg); }
+int host_fail_dev(const std::string &msg) { return fail_dev(msg); }
+int host_ok(int path) { return ok(path); }
+void host_count_launch() { count_launch(); }
+
+int HostCall::bind(const void *ptr) {
+    DeviceScope *scope = new DeviceScope;
+    scope_ = scope;
+    DeviceState *ds = nullptr;
+    const int rc = bind_device(ptr, &ds, *scope);
+    if (rc) return rc;
+    device = ds->index;
+    sms = ds->sms;
+    status = ds->status;
+    return REELS_OK;
+}
+HostCall::~HostCall() { delete static_cast<DeviceScope *>(scope_); }
+
+int host_tmap_4d(CUtensorMap *tm, const void *base, bool bf16, const uint64_t (&n)[4], const uint64_t (&stride)[3],
+                 const uint32_t (&box)[4]) {
+    cuuint64_t dims[4] = {n[0], n[1], n[2], n[3]};
+    cuuint64_t strides[3] = {stride[0], stride[1], stride[2]};
+    cuuint32_t bx[4] = {box[0], box[1], box[2], box[3]};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = g_encode(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                          const_cast<void *>(base), dims, strides, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+    return REELS_OK;
+}
+}  // namespace reels
+
 // Calls f with the element type as a compile-time constant.
 template <typename F>
 void dispatch_dt(int dt, F &&f) {
@@ -1388,7 +1424,8 @@ int reels_lowvram_check_device_status(void *stream) {
         char buf[128];
         snprintf(buf, sizeof buf, "device status 0x%x: %s", h,
                  (h & DEVERR_OPT_TABLE) ? "an optimizer call on a workspace that reels_opt_prepare did not set up"
-                                        : "a pipeline wait timed out");
+                 : (h & DEVERR_ROPE_POSITION) ? "a rotary position lies behind its table"
+                                              : "a pipeline wait timed out");
         return fail_dev(buf);
     }
     t_last_error.clear();
