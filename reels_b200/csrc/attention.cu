@@ -66,13 +66,24 @@ int check_norm_rope(const void *x, int64_t M, int64_t heads, int64_t D, const re
     return REELS_OK;
 }
 
-template <int DT, bool BWD, bool ROPE, bool HALF>
-cudaError_t launch_norm_rope(int upt, dim3 grid, dim3 block, cudaStream_t st, const NormRopeArgs &a) {
-    switch (upt) {
-        case 1: return host_launch_pdl(norm_rope_kernel<DT, BWD, ROPE, HALF, 1>, grid, block, 0, st, a);
-        case 2: return host_launch_pdl(norm_rope_kernel<DT, BWD, ROPE, HALF, 2>, grid, block, 0, st, a);
-        default: return host_launch_pdl(norm_rope_kernel<DT, BWD, ROPE, HALF, 4>, grid, block, 0, st, a);
+constexpr int kNormRopeSmem = 220 * 1024;  // of an SM's 228 KB, 1 KB a block is the system's
+
+template <int DT, bool BWD, bool ROPE, bool HALF, int UPT>
+cudaError_t launch_norm_rope(const NormRopeArgs &a, int threads, int sms, cudaStream_t st) {
+    // Blocks that fit beside each other with a ring of at least two rows, then
+    // as many rows as the shared memory holds.
+    const int budget = kNormRopeSmem, fixed = nr_smem_bytes(a.C, bytes_of(DT), BWD, 0, a.D) + 1024;
+    const int step = a.C * bytes_of(DT) * (BWD ? 2 : 1);
+    const int blocks = std::max(1, std::min({(UPT == 1 ? 1024 : UPT == 2 ? 768 : 256) / threads, 24, budget / (fixed + 2 * step)}));
+    const int stages = std::max(2, std::min(NR_STAGES, (budget / blocks - fixed) / step));  // (two rows were checked to fit)
+    const int smem = nr_smem_bytes(a.C, bytes_of(DT), BWD, stages, a.D);
+    auto kern = norm_rope_kernel<DT, BWD, ROPE, HALF, UPT>;
+    if (smem > 48 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
     }
+    const dim3 grid((unsigned)std::min<int64_t>(a.M, (int64_t)sms * blocks));
+    return host_launch_pdl(kern, grid, dim3((unsigned)threads), smem, st, a, stages);
 }
 
 int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t heads, int64_t D, const void *weight,
@@ -88,17 +99,22 @@ int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t head
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     NormRopeArgs a = {};
     a.x = x, a.dout = dout, a.weight = weight, a.out = out;
-    a.M = M, a.C = (int)(heads * D), a.D = (int)D, a.tps = (int)tps, a.eps = eps, a.err = call.status;
+    a.M = M, a.C = (int)(heads * D), a.D = (int)D, a.tps = (int)tps, a.eps = eps, a.inv_c = 1.0f / (float)a.C;
+    a.err = call.status;
     if (rope) {
         a.table = reinterpret_cast<const float2 *>(rope->table);
         a.pos = rope->positions;
         for (int i = 0; i < NR_AXES; ++i) a.size[i] = rope->size[i], a.pairs[i] = rope->dim[i] / 2;
         a.half = rope->pairing == REELS_ROPE_HALF;
+        a.by_hw = NrDivide::by((uint32_t)a.size[1] * (uint32_t)a.size[2]);
+        a.by_w = NrDivide::by((uint32_t)a.size[2]);
     }
     const int64_t units = a.C / 16;
     const bool heads_fit = !rope || (D % 16 == 0 && 32 % (D / 16) == 0);
     const bool vec = a.C % 16 == 0 && heads_fit && aligned16(x) && aligned16(out) && aligned16(weight) &&
-                     (!bwd || aligned16(dout)) && units <= 4 * 256;
+                     (!bwd || aligned16(dout)) &&
+                     // two rows have to fit the shared memory beside the weight
+                     nr_smem_bytes(a.C, bytes_of(dt), bwd, 2, a.D) <= kNormRopeSmem;
     if (!vec) {
         const dim3 grid((unsigned)std::min<int64_t>(M, 8ll * call.sms));
         with_dtype(dt, [&](auto t) {
@@ -110,22 +126,28 @@ int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t head
         return host_ok(REELS_PATH_CUDACORE);
     }
     if (!rope) a.D = 16;
-    // units a thread: as few as keep the block at 256 threads
-    const int upt = units <= 256 ? 1 : units <= 512 ? 2 : 4;
-    const int threads = (int)ceil_div(ceil_div(units, upt), 32) * 32;
-    const dim3 grid((unsigned)std::min<int64_t>(M, (int64_t)call.sms * (2048 / threads)));
+    // Units a thread, and a thread for each pair of a head.  Forward, two (the
+    // angles, waits and sums are shared); backward one, whose registers leave
+    // room for twice the warps: 8190 x 5120 forward 31 us with two and 37 with
+    // one, backward 54 and 49.
+    const int upt = units > 2 * 256 ? (bwd && units <= NR_THREADS ? 1 : 4) : bwd || units <= 32 ? 1 : 2;
+    const int threads = (int)ceil_div(std::max<int64_t>(ceil_div(units, upt), rope ? D / 2 : 1), 32) * 32;
     cudaError_t e = cudaSuccess;
     with_dtype(dt, [&](auto t) {
         constexpr int DT = decltype(t)::value;
-        const dim3 block((unsigned)threads);
-        if (bwd)
-            e = !rope    ? launch_norm_rope<DT, true, false, false>(upt, grid, block, st, a)
-                : a.half ? launch_norm_rope<DT, true, true, true>(upt, grid, block, st, a)
-                         : launch_norm_rope<DT, true, true, false>(upt, grid, block, st, a);
-        else
-            e = !rope    ? launch_norm_rope<DT, false, false, false>(upt, grid, block, st, a)
-                : a.half ? launch_norm_rope<DT, false, true, true>(upt, grid, block, st, a)
-                         : launch_norm_rope<DT, false, true, false>(upt, grid, block, st, a);
+        auto form = [&](auto b, auto r, auto h) {
+            constexpr bool B = decltype(b)::value, R = decltype(r)::value, H = decltype(h)::value;
+            e = upt == 1   ? launch_norm_rope<DT, B, R, H, 1>(a, threads, call.sms, st)
+                : upt == 2 ? launch_norm_rope<DT, B, R, H, 2>(a, threads, call.sms, st)
+                           : launch_norm_rope<DT, B, R, H, 4>(a, threads, call.sms, st);
+        };
+        auto dir = [&](auto b) {
+            if (!rope) form(b, std::false_type{}, std::false_type{});
+            else if (a.half) form(b, std::true_type{}, std::true_type{});
+            else form(b, std::true_type{}, std::false_type{});
+        };
+        if (bwd) dir(std::true_type{});
+        else dir(std::false_type{});
     });
     RA_LAUNCH(e);
     return host_ok(REELS_PATH_CUDACORE);

@@ -31,13 +31,6 @@ __device__ __forceinline__ int attn_grad_exp(const AttnArgs &a) {
     return 13 - ilogbf(top);
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-        "r"(bytes), "r"(smem_u32(bar))
-        : "memory");
-}
-
 // 32 accumulator columns of this thread's row, times f, to dst (features c0 ..): 16-bit or fp32.
 template <int DT>
 __device__ __forceinline__ void ab_store32(const uint32_t (&o)[32], float f, typename Elem<DT>::T *dst, float *part,

@@ -20,6 +20,22 @@ namespace reels {
 constexpr int NR_MAX_C = 16384;
 constexpr int NR_AXES = 3;
 
+// Division of n < 2^31 by a constant d: n / d = n m >> (31 + s) with
+// s = ceil(log2 d) and m = ceil(2^(31 + s) / d), whose error m d - 2^(31 + s)
+// < d <= 2^s is too small to reach the next quotient.
+struct NrDivide {
+    uint32_t d, m, s;
+    static NrDivide by(uint32_t d) {
+        NrDivide v = {d, 0, 0};
+        while ((1ull << v.s) < d) ++v.s;
+        v.m = (uint32_t)(((1ull << (31 + v.s)) + d - 1) / d);
+        return v;
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        return (uint32_t)(((uint64_t)n * m) >> 31) >> s;
+    }
+};
+
 struct NormRopeArgs {
     const void *x;
     const void *dout;     // backward only
@@ -33,7 +49,8 @@ struct NormRopeArgs {
     int size[NR_AXES];    // positions of an axis
     int pairs[NR_AXES];   // feature pairs of an axis
     int half;             // pairs (i, i + D/2) instead of (2i, 2i + 1)
-    float eps;
+    float eps, inv_c;
+    NrDivide by_hw, by_w;  // positions of a token in raster order
     unsigned *err;
 };
 
@@ -42,10 +59,11 @@ struct NrToken {
     bool turn;
 };
 
-// The token's position on each axis.  Raster order: width fastest; tokens
-// behind the grid are padding.  A negative position marks padding, one
-// behind its table is reported in the status word; neither is turned.
-__device__ __forceinline__ NrToken nr_token(const NormRopeArgs &a, long long row) {
+// The position on each axis of row `row`, token `tok` of its sample.  Raster
+// order: width fastest; tokens behind the grid are padding.  A negative
+// position marks padding, one behind its table is reported in the status
+// word; neither is turned.
+__device__ __forceinline__ NrToken nr_token(const NormRopeArgs &a, long long row, uint32_t tok) {
     NrToken t;
     if (a.pos) {
         t.turn = true;
@@ -59,12 +77,10 @@ __device__ __forceinline__ NrToken nr_token(const NormRopeArgs &a, long long row
             t.turn = false;
         }
     } else {
-        const unsigned i = (unsigned)(row % a.tps);
-        const unsigned hw = (unsigned)a.size[1] * (unsigned)a.size[2];
-        t.p[0] = (int)(i / hw);
-        const unsigned rest = i - (unsigned)t.p[0] * hw;
-        t.p[1] = (int)(rest / (unsigned)a.size[2]);
-        t.p[2] = (int)(rest - (unsigned)t.p[1] * (unsigned)a.size[2]);
+        const uint32_t t0 = a.by_hw(tok), rest = tok - t0 * a.by_hw.d, t1 = a.by_w(rest);
+        t.p[0] = (int)t0;
+        t.p[1] = (int)t1;
+        t.p[2] = (int)(rest - t1 * a.by_w.d);
         t.turn = t.p[0] < a.size[0];
     }
     return t;
@@ -87,44 +103,67 @@ __device__ __forceinline__ int nr_axis(const NormRopeArgs &a, int i, int &base) 
     return 2;
 }
 
-// Eight consecutive elements as fp32.
-template <int DT>
-struct NrVec;
-template <>
-struct NrVec<DT_F32> {
-    float4 a, b;
-    __device__ __forceinline__ void load(const void *p, long long i) {
-        const float4 *q = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + i);
-        a = __ldcg(q);
-        b = __ldcg(q + 1);
-    }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    }
-    static __device__ __forceinline__ void store(void *p, long long i, const float (&v)[8]) {
-        float4 *q = reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + i);
-        q[0] = make_float4(v[0], v[1], v[2], v[3]);
-        q[1] = make_float4(v[4], v[5], v[6], v[7]);
+// Two fp32 values in one register pair, and the packed arithmetic on them.
+struct F2 {
+    unsigned long long v;
+    __device__ __forceinline__ F2() {}
+    __device__ __forceinline__ F2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+    __device__ __forceinline__ float2 get() const {
+        float2 r;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+        return r;
     }
 };
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+// Eight consecutive elements, from memory to four packed pairs and back.
 template <int DT>
-struct NrVec {
-    using T = typename Elem<DT>::T;
-    uint4 a;
-    __device__ __forceinline__ void load(const void *p, long long i) {
-        a = __ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(p) + i));
-    }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        const T *t = reinterpret_cast<const T *>(&a);
+__device__ __forceinline__ void nr_read(const typename Elem<DT>::T *p, F2 (&v)[4]) {
+    if constexpr (DT == DT_F32) {
+        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+        v[0] = F2(a.x, a.y), v[1] = F2(a.z, a.w), v[2] = F2(b.x, b.y), v[3] = F2(b.z, b.w);
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = Elem<DT>::to_f(t[j]);
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == DT_BF16)
+                v[j] = F2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+            else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+                v[j] = F2(f.x, f.y);
+            }
+        }
     }
-    static __device__ __forceinline__ void store(void *p, long long i, const float (&v)[8]) {
-        uint4 o = make_uint4(Elem<DT>::pack2(v[0], v[1]), Elem<DT>::pack2(v[2], v[3]), Elem<DT>::pack2(v[4], v[5]),
-                             Elem<DT>::pack2(v[6], v[7]));
-        *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(p) + i) = o;
+}
+template <int DT>
+__device__ __forceinline__ void nr_read_global(const typename Elem<DT>::T *p, F2 (&v)[4]) {
+    __align__(16) typename Elem<DT>::T t[8];
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(t) / 16; ++j)
+        reinterpret_cast<uint4 *>(t)[j] = __ldcg(reinterpret_cast<const uint4 *>(p) + j);
+    nr_read<DT>(t, v);
+}
+template <int DT>
+__device__ __forceinline__ void nr_write(typename Elem<DT>::T *p, const F2 (&v)[4]) {
+    const float2 a = v[0].get(), b = v[1].get(), c = v[2].get(), d = v[3].get();
+    if constexpr (DT == DT_F32) {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(a.x, a.y, b.x, b.y);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(c.x, c.y, d.x, d.y);
+    } else {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(Elem<DT>::pack2(a.x, a.y), Elem<DT>::pack2(b.x, b.y),
+                                                   Elem<DT>::pack2(c.x, c.y), Elem<DT>::pack2(d.x, d.y));
     }
-};
+}
 
 // (a, b) turned by the angle, or back.
 template <bool BACK>
@@ -138,161 +177,239 @@ __device__ __forceinline__ void nr_turn(float &a, float &b, float2 cs) {
 // Sums of two values over the block's warps, the same bits in every thread;
 // `buf` alternates between calls, so one barrier a call is enough.  The
 // barrier also publishes what the caller left in shared memory before.
+template <bool TWO>
 __device__ __forceinline__ float2 nr_block_sum(float2 v, float2 *buf) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+        if (TWO) v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     }
     if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
     __syncthreads();
     v = buf[0];
     for (int w = 1; w < (int)(blockDim.x >> 5); ++w) {
         v.x += buf[w].x;
-        v.y += buf[w].y;
+        if (TWO) v.y += buf[w].y;
     }
     return v;
 }
 
-// One block per row at a time, the row and the weight in registers.
+// One block per row at a time.  Rows (x, and dout backward) arrive in a ring of
+// `stages` slots of shared memory by bulk copies, so that what is in flight
+// does not depend on registers or on how far a block's warps have come; the
+// weight is kept beside it.  A row is read twice from its slot (sum, result);
+// the barrier of row i's sums also says that row i-1's slot is free.
 // A thread owns UPT units; unit u is 8 features at i0 = 8 (u mod D/16) of the
 // lower half of head u / (D/16) and the 8 features D/2 above, so that both
 // pairings find their partners within a thread.  D/16 divides 32 and the block
 // is a multiple of 32 wide, so all units of a thread sit at the same place of
 // their heads and share their eight (cos, sin), which the block fetches once
-// a row into shared memory (through L2: half the requests of a row otherwise).
+// a row into shared memory, two rows ahead (a barrier lies between its writing
+// and its reading, and another before it is written over).
 // ROPE = 0 runs with D = 16 (two neighbouring vectors a unit).
+// Issue slots come next to HBM here: two units a thread share the angles, the
+// waits and the sums' tail, and pairs of values run through packed fp32
+// instructions where the pairing allows.
+constexpr int NR_THREADS = 512;  // at most
+constexpr int NR_STAGES = 4;     // at most
+// Shared memory: stages of rows, the weight (forward as fp32, which spares
+// conversions; backward as it is, which leaves room for another block), angles
+// of three rows.
+__host__ __device__ constexpr int nr_smem_bytes(int C, int elem, bool bwd, int stages, int D) {
+    return stages * C * elem * (bwd ? 2 : 1) + C * (bwd ? elem : 4) + 3 * (D / 2) * 8;
+}
+
 template <int DT, bool BWD, bool ROPE, bool HALF, int UPT>
-__global__ void __launch_bounds__(256) norm_rope_kernel(const NormRopeArgs a) {
-    __shared__ float2 buf[2][8];
-    __shared__ __align__(16) float2 turn[2][256];
+__global__ void __launch_bounds__(UPT == 1 ? 512 : 256, UPT == 1 ? 2 : UPT == 2 ? 3 : 1) norm_rope_kernel(const NormRopeArgs a, const int stages) {
+    using T = typename Elem<DT>::T;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ float2 buf[2][NR_THREADS / 32];
+    __shared__ uint64_t full[NR_STAGES];
+    __shared__ int abort_flag;
+    const int row_bytes = a.C * (int)sizeof(T), slot_bytes = row_bytes * (BWD ? 2 : 1);
+    // fp32 as two planes, the first and second four of every eight features,
+    // so that a warp's 16-byte reads meet no bank twice
+    uint8_t *const weight = ring + stages * slot_bytes;
+    float2 *const turn = reinterpret_cast<float2 *>(weight + a.C * (BWD ? (int)sizeof(T) : 4));
+    volatile int *const abort = &abort_flag;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
+        abort_flag = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
     griddep_wait();
+    auto fill = [&](long long row, int s) {
+        mbar_arrive_expect_tx(&full[s], slot_bytes);
+        bulk_load(smem_u32(ring + s * slot_bytes), reinterpret_cast<const T *>(a.x) + row * a.C, row_bytes, &full[s]);
+        if (BWD)
+            bulk_load(smem_u32(ring + s * slot_bytes + row_bytes), reinterpret_cast<const T *>(a.dout) + row * a.C,
+                      row_bytes, &full[s]);
+    };
+    if (threadIdx.x == 0)
+        for (int s = 0; s < stages; ++s)
+            if (blockIdx.x + (long long)s * gridDim.x < a.M) fill(blockIdx.x + (long long)s * gridDim.x, s);
+    for (int i = threadIdx.x; i < a.C / 8; i += blockDim.x) {
+        F2 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = F2(1.0f, 1.0f);
+        if (a.weight) nr_read_global<DT>(reinterpret_cast<const T *>(a.weight) + 8 * i, w);
+        if (BWD) {
+            nr_write<DT>(reinterpret_cast<T *>(weight) + 8 * i, w);
+        } else {
+            const float2 p = w[0].get(), q = w[1].get(), u = w[2].get(), v = w[3].get();
+            reinterpret_cast<float4 *>(weight)[i] = make_float4(p.x, p.y, q.x, q.y);
+            reinterpret_cast<float4 *>(weight)[a.C / 8 + i] = make_float4(u.x, u.y, v.x, v.y);
+        }
+    }
     const int upr = a.C / 16, uph = a.D / 16;  // units of a row, of a head
     const int i0 = 8 * ((int)threadIdx.x % uph);
     // features of unit k of this thread: f, and f + D/2
-    auto feature = [&](int k) { return ((int)threadIdx.x + k * (int)blockDim.x) / uph * a.D + i0; };
-    auto owned = [&](int k) { return (int)threadIdx.x + k * (int)blockDim.x < upr; };
-    NrVec<DT> wv[UPT][2];
-    if (a.weight) {
+    int feat[UPT];
 #pragma unroll
-        for (int k = 0; k < UPT; ++k)
-            if (owned(k)) {
-                wv[k][0].load(a.weight, feature(k));
-                wv[k][1].load(a.weight, feature(k) + a.D / 2);
+    for (int k = 0; k < UPT; ++k) feat[k] = ((int)threadIdx.x + k * (int)blockDim.x) / uph * a.D + i0;
+    auto owned = [&](int k) { return (int)threadIdx.x + k * (int)blockDim.x < upr; };
+    auto read = [&](const T *from, int k, F2 (&lo)[4], F2 (&hi)[4]) {
+        nr_read<DT>(from + feat[k], lo);
+        nr_read<DT>(from + feat[k] + a.D / 2, hi);
+    };
+    auto weigh = [&](int k, F2 (&lo)[4], F2 (&hi)[4]) {
+        F2 wl[4], wh[4];
+        if (BWD) {
+            read(reinterpret_cast<const T *>(weight), k, wl, wh);
+        } else {
+            const float4 *const w = reinterpret_cast<const float4 *>(weight) + feat[k] / 8;
+            const float4 w0 = w[0], w1 = w[a.C / 8], w2 = w[a.D / 16], w3 = w[a.C / 8 + a.D / 16];
+            wl[0] = F2(w0.x, w0.y), wl[1] = F2(w0.z, w0.w), wl[2] = F2(w1.x, w1.y), wl[3] = F2(w1.z, w1.w);
+            wh[0] = F2(w2.x, w2.y), wh[1] = F2(w2.z, w2.w), wh[2] = F2(w3.x, w3.y), wh[3] = F2(w3.z, w3.w);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lo[j] = mul2(lo[j], wl[j]), hi[j] = mul2(hi[j], wh[j]);
+    };
+    // The angles: thread i < D/2 fetches pair i of a row and leaves it where
+    // the threads at position l of their heads find pairs 2p, 2p + 1 of their
+    // eight side by side: [p][l] (no bank twice in a warp's reads).
+    const bool turner = ROPE && (int)threadIdx.x < a.D / 2;
+    float2 nt = make_float2(1.0f, 0.0f);
+    int base = 0, axis = 0, put = 0;
+    if (turner) {
+        const int i = threadIdx.x;
+        axis = nr_axis(a, i, base);
+        const int l = HALF ? i / 8 : (i % (a.D / 4)) / 4, j = HALF ? i % 8 : i % 4 + i / (a.D / 4) * 4;
+        put = ((j >> 1) * uph + l) * 2 + (j & 1);
+    }
+    const uint32_t stride = ROPE ? gridDim.x % (uint32_t)a.tps : 0;
+    uint32_t tok = ROPE ? blockIdx.x % (uint32_t)a.tps : 0;  // of the next row to fetch
+    auto fetch_angles = [&](long long row) {
+        const NrToken t = nr_token(a, row, tok);
+        const int p = axis == 0 ? t.p[0] : axis == 1 ? t.p[1] : t.p[2];
+        const int step = axis == 0 ? a.pairs[0] : axis == 1 ? a.pairs[1] : a.pairs[2];
+        nt = t.turn ? __ldcg(a.table + base + p * step) : make_float2(1.0f, 0.0f);
+        tok += stride;
+        if (tok >= (uint32_t)a.tps) tok -= a.tps;
+    };
+    if (turner) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+            if (blockIdx.x + n * (long long)gridDim.x < a.M) {
+                fetch_angles(blockIdx.x + n * (long long)gridDim.x);
+                turn[n * (a.D / 2) + put] = nt;
             }
     }
-    auto weigh = [&](int k, float (&lo)[8], float (&hi)[8]) {
-        if (!a.weight) return;
-        float w[8];
-        wv[k][0].get(w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) lo[j] *= w[j];
-        wv[k][1].get(w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) hi[j] *= w[j];
-    };
-    int flip = 0;
+    __syncthreads();  // the weight, the first angles
+    int flip = 0, slot = 0, at = 0;  // at: the angles' buffer of this row
+    uint32_t phase = 0;
     for (long long row = blockIdx.x; row < a.M; row += gridDim.x, flip ^= 1) {
-        const long long at = row * a.C;
-        NrVec<DT> xv[UPT][2], gv[BWD ? UPT : 1][2];
-#pragma unroll
-        for (int k = 0; k < UPT; ++k) {
-            if (owned(k)) {
-                const int f = feature(k);
-                xv[k][0].load(a.x, at + f);
-                xv[k][1].load(a.x, at + f + a.D / 2);
-                if (BWD) {
-                    gv[k][0].load(a.dout, at + f);
-                    gv[k][1].load(a.dout, at + f + a.D / 2);
-                }
-            }
-        }
-        if (ROPE) {
-            const NrToken t = nr_token(a, row);
-            for (int i = threadIdx.x; i < a.D / 2; i += blockDim.x) {
-                int base;
-                const int ax = nr_axis(a, i, base);
-                const int p = ax == 0 ? t.p[0] * a.pairs[0] : ax == 1 ? t.p[1] * a.pairs[1] : t.p[2] * a.pairs[2];
-                turn[flip][i] = t.turn ? __ldcg(a.table + base + p) : make_float2(1.0f, 0.0f);
-            }
-        }
+        const long long later = row + 2ll * gridDim.x;
+        if (turner && later < a.M) fetch_angles(later);
+        wait_bar(&full[slot], phase, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
+        const T *const xs = reinterpret_cast<const T *>(ring + slot * slot_bytes);
         // pairs 0-3 of a unit: its features 2j, 2j+1; 4-7 those of its upper
         // vector (HALF: j of both vectors)
         float2 cs[8];
-        auto fetch = [&]() {
+        auto read_angles = [&](float by) {
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                const int pair = HALF ? i0 + j : i0 / 2 + (j & 3) + (j >> 2) * (a.D / 4);
-                const float4 v = *reinterpret_cast<const float4 *>(&turn[flip][pair]);
-                cs[j] = make_float2(v.x, v.y);
-                cs[j + 1] = make_float2(v.z, v.w);
+                const float4 v = reinterpret_cast<const float4 *>(turn + at * (a.D / 2))[(j >> 1) * uph + (i0 >> 3)];
+                cs[j] = mul2(F2(v.x, v.y), F2(by, by)).get();
+                cs[j + 1] = mul2(F2(v.z, v.w), F2(by, by)).get();
             }
         };
-        auto rotate = [&](float (&lo)[8], float (&hi)[8]) {
+        auto rotate = [&](F2 (&lo)[4], F2 (&hi)[4]) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (HALF) nr_turn<BWD>(lo[j], hi[j], cs[j]);
-                else if (j < 4) nr_turn<BWD>(lo[2 * j], lo[2 * j + 1], cs[j]);
-                else nr_turn<BWD>(hi[2 * j - 8], hi[2 * j - 7], cs[j]);
+            for (int j = 0; j < 4; ++j) {
+                float2 x = lo[j].get(), y = hi[j].get();
+                if (HALF) {
+                    nr_turn<BWD>(x.x, y.x, cs[2 * j]);
+                    nr_turn<BWD>(x.y, y.y, cs[2 * j + 1]);
+                } else {
+                    nr_turn<BWD>(x.x, x.y, cs[j]);
+                    nr_turn<BWD>(y.x, y.y, cs[4 + j]);
+                }
+                lo[j] = F2(x.x, x.y), hi[j] = F2(y.x, y.y);
             }
         };
-        if (BWD && ROPE) {
-            __syncthreads();
-            fetch();
-        }
-        // h = w R' dout
-        auto pulled = [&](int k, float (&lo)[8], float (&hi)[8]) {
-            gv[k][0].get(lo);
-            gv[k][1].get(hi);
-            if (ROPE) rotate(lo, hi);
-            weigh(k, lo, hi);
-        };
-        float2 sum = make_float2(0.0f, 0.0f);
+        if (ROPE && BWD) read_angles(1.0f);
+        F2 xl[UPT][4], xh[UPT][4];  // (backward: read again for the result)
+        F2 hl[BWD ? UPT : 1][4], hh[BWD ? UPT : 1][4];  // h = w R' dout
+        F2 s0 = F2(0.0f, 0.0f), s1 = F2(0.0f, 0.0f);
 #pragma unroll
         for (int k = 0; k < UPT; ++k) {
             if (owned(k)) {
-                float lo[8], hi[8];
-                xv[k][0].get(lo);
-                xv[k][1].get(hi);
+                read(xs, k, xl[k], xh[k]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) sum.x += lo[j] * lo[j] + hi[j] * hi[j];
+                for (int j = 0; j < 4; ++j) s0 = fma2(xl[k][j], xl[k][j], fma2(xh[k][j], xh[k][j], s0));
                 if (BWD) {
-                    float gl[8], gh[8];
-                    pulled(k, gl, gh);
+                    read(xs + a.C, k, hl[k], hh[k]);
+                    if (ROPE) rotate(hl[k], hh[k]);
+                    weigh(k, hl[k], hh[k]);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum.y += lo[j] * gl[j] + hi[j] * gh[j];
+                    for (int j = 0; j < 4; ++j) s1 = fma2(xl[k][j], hl[k][j], fma2(xh[k][j], hh[k][j], s1));
                 }
             }
         }
-        sum = nr_block_sum(sum, buf[flip]);
-        const float r = 1.0f / sqrtf(sum.x / (float)a.C + a.eps);
-        const float c2 = BWD ? r * r * (sum.y / (float)a.C) : 0.0f;
-        if (!BWD && ROPE) fetch();
+        float2 sum = make_float2(s0.get().x + s0.get().y, BWD ? s1.get().x + s1.get().y : 0.0f);
+        // behind this barrier the other row's slot and angles have no readers left
+        sum = nr_block_sum<BWD>(sum, buf[flip]);
+        if (turner && later < a.M) turn[(at == 0 ? 2 : at - 1) * (a.D / 2) + put] = nt;
+        if (threadIdx.x == 0 && row > blockIdx.x) {
+            const long long next = row + (long long)(stages - 1) * gridDim.x;
+            if (next < a.M) fill(next, slot == 0 ? stages - 1 : slot - 1);
+        }
+        const float r = rsqrtf(fmaf(sum.x, a.inv_c, a.eps));
+        if (ROPE && !BWD) read_angles(r);
+        T *const out = reinterpret_cast<T *>(a.out) + row * a.C;
 #pragma unroll
         for (int k = 0; k < UPT; ++k) {
             if (owned(k)) {
-                const int f = feature(k);
-                float lo[8], hi[8];
-                xv[k][0].get(lo);
-                xv[k][1].get(hi);
+                F2 lo[4], hi[4];
                 if (BWD) {
-                    float gl[8], gh[8];
-                    pulled(k, gl, gh);
+                    read(xs, k, xl[0], xh[0]);
+                    const float c2 = -r * r * r * (sum.y * a.inv_c);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        lo[j] = r * (gl[j] - lo[j] * c2);
-                        hi[j] = r * (gh[j] - hi[j] * c2);
+                    for (int j = 0; j < 4; ++j) {
+                        lo[j] = fma2(xl[0][j], F2(c2, c2), mul2(hl[k][j], F2(r, r)));
+                        hi[j] = fma2(xh[0][j], F2(c2, c2), mul2(hh[k][j], F2(r, r)));
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) lo[j] *= r, hi[j] *= r;
+                    for (int j = 0; j < 4; ++j) lo[j] = xl[k][j], hi[j] = xh[k][j];
                     weigh(k, lo, hi);
-                    if (ROPE) rotate(lo, hi);
+                    if (ROPE) rotate(lo, hi);  // and times r
+                    else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) lo[j] = mul2(lo[j], F2(r, r)), hi[j] = mul2(hi[j], F2(r, r));
+                    }
                 }
-                NrVec<DT>::store(a.out, at + f, lo);
-                NrVec<DT>::store(a.out, at + f + a.D / 2, hi);
+                nr_write<DT>(out + feat[k], lo);
+                nr_write<DT>(out + feat[k] + a.D / 2, hi);
             }
         }
+        if (++slot == stages) slot = 0, phase ^= 1;
+        if (++at == 3) at = 0;
+    }
+    if (*abort) {  // give the copies in flight time to land before the shared memory goes
+        for (int i = 0; i < 64; ++i) __nanosleep(2000);
     }
 }
 
@@ -309,7 +426,7 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const NormRopeArgs a
         const long long at = row * a.C;
         NrToken t;
         t.turn = false;
-        if (rope) t = nr_token(a, row);
+        if (rope) t = nr_token(a, row, (uint32_t)(row % a.tps));
         // features of item i: a pair of a head, or one feature
         auto where = [&](int i, int &f0, int &f1, float2 &cs) {
             cs = make_float2(1.0f, 0.0f);
@@ -340,7 +457,7 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const NormRopeArgs a
                 sum.y += x0 * (g0 * w_of(f0)) + x1 * (g1 * w_of(f1));
             }
         }
-        sum = nr_block_sum(sum, buf[flip]);
+        sum = nr_block_sum<BWD>(sum, buf[flip]);
         const float r = 1.0f / sqrtf(sum.x / (float)a.C + a.eps);
         const float c2 = BWD ? r * r * (sum.y / (float)a.C) : 0.0f;
         for (int i = threadIdx.x; i < a.C / step; i += blockDim.x) {
