@@ -210,12 +210,14 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
         if (lane == 0) {
             constexpr int ab = DT == DT_BF16 ? 1 : 0;
             constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
-            const uint32_t S = tmem + second * 128, O = tmem + 256 + second * 128, A = sbase + second * G::TILE;
+            const uint32_t S = tmem + second * 128, O = tmem + 256 + second * 128;
+            const uint64_t A = at_desc_k(sbase + second * G::TILE);
             // score operand of a stage (Q, dO), and the other one (dO, Q)
             uint64_t *in_full = second ? g_full : q_full, *in_empty = second ? g_empty : q_empty;
             uint64_t *ot_full = second ? q_full : g_full, *ot_empty = second ? q_empty : g_empty;
             uint64_t *scored = second ? dp_full : s_full, *ready = second ? ds_full : p_full;
-            const uint32_t in_off = second ? G::TILE : 0, ot_off = second ? 0 : G::TILE;
+            const uint64_t in0 = at_desc_k(sbase + G::RING_OFF + (second ? G::TILE : 0)),
+                           ot0 = at_desc_mn(sbase + G::RING_OFF + (second ? 0 : G::TILE));
             uint32_t g = 0, np = 0, nu = 0;
             bool good = true;
             auto scores = [&](uint32_t i) {
@@ -223,9 +225,10 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                 good = good && wait_bar(&in_full[s], (i / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
                 if (!good) return;
                 tc_fence_after();
-                const uint32_t B = sbase + G::RING_OFF + s * G::STAGE + in_off;
+                const uint64_t B = in0 + s * (G::STAGE / 16);
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk) mma_f16_ss(S, at_desc_k(A, kk), at_desc_k(B, kk), id_s, kk > 0);
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_f16_ss(S, A + at_step_k(kk), B + at_step_k(kk), id_s, kk > 0);
                 mma_commit(scored);
                 mma_commit(&in_empty[s]);
             };
@@ -242,10 +245,10 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                     if (i == 0) good = good && wait_bar(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
                     if (!good) break;
                     tc_fence_after();
-                    const uint32_t B = sbase + G::RING_OFF + s * G::STAGE + ot_off;
+                    const uint64_t B = ot0 + s * (G::STAGE / 16);
 #pragma unroll
                     for (int kk = 0; kk < AT_TILE / 16; ++kk)
-                        at_mma_ts(O, S + (kk >> 2) * 64 + (kk & 3) * 8, at_desc_mn(B, kk), id_o, i > 0 || kk > 0);
+                        at_mma_ts(O, S + (kk >> 2) * 64 + (kk & 3) * 8, B + at_step_mn(kk), id_o, i > 0 || kk > 0);
                     mma_commit(&ot_empty[s]);
                     if (i + 1 < w.n) scores(g + 1);
                 }
@@ -529,6 +532,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
         at_fewer_registers();
         if (lane == 0) {
             constexpr uint32_t id_s = idesc_f16(DT == DT_BF16 ? 1 : 0, 0, 0, 128, AT_TILE);
+            const uint64_t Q = at_desc_k(sbase), k0 = at_desc_k(sbase + G::K_OFF);
             uint32_t g = 0, nu = 0;
             bool good = true;
             for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
@@ -541,10 +545,10 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                            wait_bar(&s_empty[t], ((g >> 1) & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
                     if (!good) break;
                     tc_fence_after();
-                    const uint32_t K = sbase + G::K_OFF + s * G::TILE;
+                    const uint64_t K = k0 + s * (G::TILE / 16);
 #pragma unroll
                     for (int kk = 0; kk < DP / 16; ++kk)
-                        mma_f16_ss(tmem + 128 * t, at_desc_k(sbase, kk), at_desc_k(K, kk), id_s, kk > 0);
+                        mma_f16_ss(tmem + 128 * t, Q + at_step_k(kk), K + at_step_k(kk), id_s, kk > 0);
                     mma_commit(&s_full[t]);
                     mma_commit(&k_empty[s]);
                 }
@@ -561,6 +565,8 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
             constexpr int ab = DT == DT_BF16 ? 1 : 0;
             constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
             const uint32_t DS = tmem + 256, O = tmem + 384;
+            const uint64_t dO = at_desc_k(sbase + G::TILE), v0 = at_desc_k(sbase + G::V_OFF),
+                           k0 = at_desc_mn(sbase + G::K_OFF);
             uint32_t g = 0, nu = 0, np = 0;
             bool good = true;
             auto scores = [&](uint32_t i) {
@@ -568,10 +574,10 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                 good = good && wait_bar(&v_full[t], (i / G::NV) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
                 if (!good) return;
                 tc_fence_after();
-                const uint32_t V = sbase + G::V_OFF + t * G::TILE;
+                const uint64_t V = v0 + t * (G::TILE / 16);
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk)
-                    mma_f16_ss(DS, at_desc_k(sbase + G::TILE, kk), at_desc_k(V, kk), id_s, kk > 0);
+                    mma_f16_ss(DS, dO + at_step_k(kk), V + at_step_k(kk), id_s, kk > 0);
                 mma_commit(dp_full);
                 mma_commit(&v_empty[t]);
             };
@@ -588,10 +594,10 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                     if (j == 0) good = good && wait_bar(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
                     if (!good) break;
                     tc_fence_after();
-                    const uint32_t K = sbase + G::K_OFF + s * G::TILE;
+                    const uint64_t K = k0 + s * (G::TILE / 16);
 #pragma unroll
                     for (int kk = 0; kk < AT_TILE / 16; ++kk)
-                        at_mma_ts(O, DS + (kk >> 2) * 64 + (kk & 3) * 8, at_desc_mn(K, kk), id_o, j > 0 || kk > 0);
+                        at_mma_ts(O, DS + (kk >> 2) * 64 + (kk & 3) * 8, K + at_step_mn(kk), id_o, j > 0 || kk > 0);
                     mma_commit(&k_empty[s]);
                     if (j + 1 < w.nk) scores(g + 1);
                 }

@@ -12,13 +12,15 @@ namespace reels {
 
 constexpr int AT_TILE = 128;
 
+// Operand descriptors.  The issuing thread's instructions are the rate of the
+// short MMAs here, so descriptors are formed once per tile and a step only
+// adds a constant to the address field (bytes / 16; no carry, shared memory
+// ends below 2^18).
 // K-major: reduction step kk of 16 features; MN-major: step kk of 16 tokens.
-__device__ __forceinline__ uint64_t at_desc_k(uint32_t tile, int kk) {
-    return sdesc_sw128(tile + (kk >> 2) * (AT_TILE * 128) + (kk & 3) * 32, 16, 1024);
-}
-__device__ __forceinline__ uint64_t at_desc_mn(uint32_t tile, int kk) {
-    return sdesc_sw128(tile + kk * 2048, AT_TILE * 128, 1024);
-}
+__device__ __forceinline__ uint64_t at_desc_k(uint32_t tile) { return sdesc_sw128(tile, 16, 1024); }
+__device__ __forceinline__ uint64_t at_desc_mn(uint32_t tile) { return sdesc_sw128(tile, AT_TILE * 128, 1024); }
+__device__ __forceinline__ constexpr uint64_t at_step_k(int kk) { return (kk >> 2) * (AT_TILE * 128 / 16) + (kk & 3) * 2; }
+__device__ __forceinline__ constexpr uint64_t at_step_mn(int kk) { return kk * 128; }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const void *tmap, int x, int y, int z, int w,
                                             uint64_t *bar) {
@@ -82,6 +84,12 @@ __device__ __forceinline__ float at_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ float at_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 // Probabilities are at most 1 (2^8 before the running maximum catches up) and

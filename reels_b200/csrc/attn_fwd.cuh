@@ -32,8 +32,8 @@ struct AttnFwdGeom {
     static constexpr int NST = DP == 128 ? 5 : 8;  // K and V tiles in flight
     static constexpr int KV_OFF = 2 * TILE;
     static constexpr int BAR_OFF = KV_OFF + NST * TILE;
-    // q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2], mma_done[2], raw, kv_full, kv_empty
-    static constexpr int NBAR = 15 + 2 * NST;
+    // q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], o_empty[2], mma_done[2], turn[2], raw, kv_full, kv_empty
+    static constexpr int NBAR = 19 + 2 * NST;
     static constexpr int MISC_OFF = BAR_OFF + NBAR * 8;
     static constexpr int SMEM_BYTES = MISC_OFF + 16 + 1024;
     static_assert(SMEM_BYTES <= 232448, "shared memory plan exceeds 227 KB");
@@ -73,9 +73,9 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
-    uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 8,
-             *o_empty = bars + 10, *mma_done = bars + 12, *raw = bars + 14, *kv_full = bars + 15,
-             *kv_empty = bars + 15 + G::NST;
+    uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 10,
+             *o_empty = bars + 12, *mma_done = bars + 14, *turn = bars + 16, *raw = bars + 18, *kv_full = bars + 19,
+             *kv_empty = bars + 19 + G::NST;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + G::MISC_OFF);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + G::MISC_OFF + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -85,7 +85,9 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
             mbar_init(&q_full[t], 1);
             mbar_init(&q_empty[t], 1);
             mbar_init(&s_full[t], 1);
-            mbar_init(&p_full[t], 4);
+            mbar_init(&p_full[2 * t], 4);
+            mbar_init(&p_full[2 * t + 1], 4);
+            mbar_init(&turn[t], 1);
             mbar_init(&o_full[t], 1);
             mbar_init(&o_empty[t], 4);
             mbar_init(&mma_done[t], 1);
@@ -169,17 +171,29 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
         if (lane == 0) {
             constexpr int ab = DT == DT_BF16 ? 1 : 0;
             constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
-            const uint32_t S = tmem + t * 128, O = tmem + 256 + t * 128, Q = sbase + t * G::TILE;
-            uint32_t g = 0, np = 0, nu = 0;
+            const uint32_t S = tmem + t * 128, O = tmem + 256 + t * 128;
+            const uint64_t Q = at_desc_k(sbase + t * G::TILE), k0 = at_desc_k(sbase + G::KV_OFF),
+                           v0 = at_desc_mn(sbase + G::KV_OFF);
+            uint32_t g = 0, np = 0, nu = 0, nt = 0;
             bool good = true;
+            // The issuers take turns, tile 0 first: products of both tiles
+            // issued at once would share the tensor core and end together,
+            // and both softmaxes would run, and then wait, at the same time.
+            auto take_turn = [&](bool two) {
+                if (two) good = good && wait_bar(&turn[t], (nt & 1) ^ (t == 0), abort, a.err, DEVERR_TIMEOUT_ACC);
+            };
+            auto pass_turn = [&](bool two) {
+                if (two) mbar_arrive(&turn[t ^ 1]), ++nt;
+            };
             auto wait_kv = [&](uint32_t i) {
                 good = good && wait_bar(&kv_full[i % G::NST], (i / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
                 tc_fence_after();
             };
             auto scores = [&](uint32_t i) {
-                const uint32_t K = sbase + G::KV_OFF + (i % G::NST) * G::TILE;
+                const uint64_t K = k0 + (i % G::NST) * (G::TILE / 16);
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk) mma_f16_ss(S, at_desc_k(Q, kk), at_desc_k(K, kk), id_s, kk > 0);
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_f16_ss(S, Q + at_step_k(kk), K + at_step_k(kk), id_s, kk > 0);
                 mma_commit(&s_full[t]);
                 mma_commit(&kv_empty[i % G::NST]);
             };
@@ -195,25 +209,34 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
                 }
                 good = wait_bar(&q_full[t], nu & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
                 wait_kv(g);
+                take_turn(w.tiles == 2);
                 if (!good) break;
                 scores(g);
+                pass_turn(w.tiles == 2);
                 for (int j = 0; j < w.nk; ++j, g += 2) {
                     if (j == w.nk - 1) mma_commit(&q_empty[t]);  // the last scores were issued
                     wait_kv(g + 1);
-                    good = good && wait_bar(&p_full[t], np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    good = good && wait_bar(&p_full[2 * t], np & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
                     if (j == 0) good = good && wait_bar(&o_empty[t], (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    take_turn(w.tiles == 2);
                     if (!good) break;
                     tc_fence_after();
-                    const uint32_t V = sbase + G::KV_OFF + ((g + 1) % G::NST) * G::TILE;
+                    const uint64_t V = v0 + ((g + 1) % G::NST) * (G::TILE / 16);
 #pragma unroll
-                    for (int kk = 0; kk < AT_TILE / 16; ++kk)
-                        at_mma_ts(O, S + kk * 8, at_desc_mn(V, kk), id_o, j > 0 || kk > 0);
+                    for (int kk = 0; kk < 4; ++kk)
+                        at_mma_ts(O, S + kk * 8, V + at_step_mn(kk), id_o, j > 0 || kk > 0);
+                    good = wait_bar(&p_full[2 * t + 1], np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (!good) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 4; kk < AT_TILE / 16; ++kk) at_mma_ts(O, S + kk * 8, V + at_step_mn(kk), id_o, 1);
                     mma_commit(&kv_empty[(g + 1) % G::NST]);
                     if (j + 1 < w.nk) {
                         wait_kv(g + 2);
                         if (!good) break;
                         scores(g + 2);
                     }
+                    pass_turn(w.tiles == 2);
                 }
                 if (!good) break;
                 mma_commit(&o_full[t]);
@@ -253,7 +276,12 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s[i]);
 #pragma unroll
-                for (int i = 4; i < AT_TILE; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+                for (int i = 4; i < AT_TILE - 4; i += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        mx[e] = at_max3(mx[e], __uint_as_float(s[i + e]), __uint_as_float(s[i + 4 + e]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[AT_TILE - 4 + e]));
                 float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
                 top = (top == -CUDART_INF_F ? 0.0f : top) - AtRange<DT>::FWD_SHIFT;
                 if (j == 0) m = top;
@@ -284,11 +312,13 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
                         sum[2 + (e & 1)] += y;
                     }
                     at_tmem_st16(S + 16 * i, p);
+                    if (i & 1) {  // half of P: its products may start
+                        at_tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_full[2 * t + (i >> 1)]);
+                    }
                 }
-                at_tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[t]);
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
             if (!good) break;
