@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
              *q_full = bars + 10, *q_empty = q_full + G::NST, *g_full = q_empty + G::NST, *g_empty = g_full + G::NST;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + G::MISC_OFF);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + G::MISC_OFF + 4);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         mbar_init(kv_full, 1);
@@ -207,7 +207,8 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
         // ------------------------------------------------- MMAs: 9 S', dV; 10 dP', dK
         at_fewer_registers();
         const int second = warp - 9;
-        if (lane == 0) {
+        {
+            const bool leader = at_elect();
             constexpr int ab = DT == DT_BF16 ? 1 : 0;
             constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
             const uint32_t S = tmem + second * 128, O = tmem + 256 + second * 128;
@@ -222,41 +223,45 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
             bool good = true;
             auto scores = [&](uint32_t i) {
                 const int s = i % G::NST;
-                good = good && wait_bar(&in_full[s], (i / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
+                good = good && at_wait(&in_full[s], (i / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
                 if (!good) return;
                 tc_fence_after();
                 const uint64_t B = in0 + s * (G::STAGE / 16);
+                if (leader) {
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk)
-                    mma_f16_ss(S, A + at_step_k(kk), B + at_step_k(kk), id_s, kk > 0);
-                mma_commit(scored);
-                mma_commit(&in_empty[s]);
+                    for (int kk = 0; kk < DP / 16; ++kk)
+                        mma_f16_ss(S, A + at_step_k(kk), B + at_step_k(kk), id_s, kk > 0);
+                }
+                if (leader) mma_commit(scored);
+                if (leader) mma_commit(&in_empty[s]);
             };
             for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
                 const AttnKvUnit w = attn_kv_unit(a, u);
                 if (w.n == 0) continue;
-                good = wait_bar(kv_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
+                good = at_wait(kv_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
                 scores(g);
                 for (int i = 0; i < w.n && good; ++i, ++g) {
                     const int s = g % G::NST;
-                    if (i == w.n - 1) mma_commit(kv_empty);  // the last scores were issued
-                    good = wait_bar(&ot_full[s], (g / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL) &&
-                           wait_bar(ready, np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                    if (i == 0) good = good && wait_bar(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (leader && i == w.n - 1) mma_commit(kv_empty);  // the last scores were issued
+                    good = at_wait(&ot_full[s], (g / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL) &&
+                           at_wait(ready, np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (i == 0) good = good && at_wait(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
                     if (!good) break;
                     tc_fence_after();
                     const uint64_t B = ot0 + s * (G::STAGE / 16);
+                    if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < AT_TILE / 16; ++kk)
-                        at_mma_ts(O, S + (kk >> 2) * 64 + (kk & 3) * 8, B + at_step_mn(kk), id_o, i > 0 || kk > 0);
-                    mma_commit(&ot_empty[s]);
+                        for (int kk = 0; kk < AT_TILE / 16; ++kk)
+                            at_mma_ts(O, S + (kk >> 2) * 64 + (kk & 3) * 8, B + at_step_mn(kk), id_o, i > 0 || kk > 0);
+                    }
+                    if (leader) mma_commit(&ot_empty[s]);
                     if (i + 1 < w.n) scores(g + 1);
                 }
                 if (!good) break;
-                mma_commit(acc_full);
+                if (leader) mma_commit(acc_full);
                 ++nu;
             }
-            mma_commit(&mma_done[second]);
+            if (leader) mma_commit(&mma_done[second]);
         }
     } else {
         // --------------------------------------------- P', dS' and the output
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
              *k_full = bars + 13, *k_empty = k_full + G::NK, *v_full = k_empty + G::NK, *v_empty = v_full + G::NV;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + G::MISC_OFF);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + G::MISC_OFF + 4);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -530,7 +535,8 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
     } else if (warp == 9) {
         // ---------------------------------------------------------- MMAs: S
         at_fewer_registers();
-        if (lane == 0) {
+        {
+            const bool leader = at_elect();
             constexpr uint32_t id_s = idesc_f16(DT == DT_BF16 ? 1 : 0, 0, 0, 128, AT_TILE);
             const uint64_t Q = at_desc_k(sbase), k0 = at_desc_k(sbase + G::K_OFF);
             uint32_t g = 0, nu = 0;
@@ -538,30 +544,33 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
             for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
                 const AttnQUnit w = attn_q_unit(a, u);
                 if (w.nk == 0) continue;
-                good = wait_bar(q_full, nu++ & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
+                good = at_wait(q_full, nu++ & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
                 for (int j = 0; j < w.nk && good; ++j, ++g) {
                     const int s = g % G::NK, t = g & 1;
-                    good = wait_bar(&k_full[s], (g / G::NK) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL) &&
-                           wait_bar(&s_empty[t], ((g >> 1) & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    good = at_wait(&k_full[s], (g / G::NK) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL) &&
+                           at_wait(&s_empty[t], ((g >> 1) & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
                     if (!good) break;
                     tc_fence_after();
                     const uint64_t K = k0 + s * (G::TILE / 16);
+                    if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < DP / 16; ++kk)
-                        mma_f16_ss(tmem + 128 * t, Q + at_step_k(kk), K + at_step_k(kk), id_s, kk > 0);
-                    mma_commit(&s_full[t]);
-                    mma_commit(&k_empty[s]);
+                        for (int kk = 0; kk < DP / 16; ++kk)
+                            mma_f16_ss(tmem + 128 * t, Q + at_step_k(kk), K + at_step_k(kk), id_s, kk > 0);
+                    }
+                    if (leader) mma_commit(&s_full[t]);
+                    if (leader) mma_commit(&k_empty[s]);
                 }
-                if (good) mma_commit(q_empty);
+                if (leader && good) mma_commit(q_empty);
             }
-            mma_commit(&mma_done[0]);
+            if (leader) mma_commit(&mma_done[0]);
         }
     } else if (warp == 11) {
         at_fewer_registers();  // idle: completes the third group of four warps
     } else if (warp == 10) {
         // ---------------------------------------------------- MMAs: dP and dQ
         at_fewer_registers();
-        if (lane == 0) {
+        {
+            const bool leader = at_elect();
             constexpr int ab = DT == DT_BF16 ? 1 : 0;
             constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
             const uint32_t DS = tmem + 256, O = tmem + 384;
@@ -571,41 +580,45 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
             bool good = true;
             auto scores = [&](uint32_t i) {
                 const int t = i % G::NV;
-                good = good && wait_bar(&v_full[t], (i / G::NV) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
+                good = good && at_wait(&v_full[t], (i / G::NV) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
                 if (!good) return;
                 tc_fence_after();
                 const uint64_t V = v0 + t * (G::TILE / 16);
+                if (leader) {
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk)
-                    mma_f16_ss(DS, dO + at_step_k(kk), V + at_step_k(kk), id_s, kk > 0);
-                mma_commit(dp_full);
-                mma_commit(&v_empty[t]);
+                    for (int kk = 0; kk < DP / 16; ++kk)
+                        mma_f16_ss(DS, dO + at_step_k(kk), V + at_step_k(kk), id_s, kk > 0);
+                }
+                if (leader) mma_commit(dp_full);
+                if (leader) mma_commit(&v_empty[t]);
             };
             for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
                 const AttnQUnit w = attn_q_unit(a, u);
                 if (w.nk == 0) continue;
-                good = wait_bar(q_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
+                good = at_wait(q_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
                 scores(g);
                 for (int j = 0; j < w.nk && good; ++j, ++g) {
                     const int s = g % G::NK;
-                    if (j == w.nk - 1) mma_commit(q_empty);  // the last product with dO was issued
-                    good = wait_bar(&k_full[s], (g / G::NK) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL) &&
-                           wait_bar(ds_full, np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                    if (j == 0) good = good && wait_bar(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (leader && j == w.nk - 1) mma_commit(q_empty);  // the last product with dO was issued
+                    good = at_wait(&k_full[s], (g / G::NK) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL) &&
+                           at_wait(ds_full, np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (j == 0) good = good && at_wait(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
                     if (!good) break;
                     tc_fence_after();
                     const uint64_t K = k0 + s * (G::TILE / 16);
+                    if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < AT_TILE / 16; ++kk)
-                        at_mma_ts(O, DS + (kk >> 2) * 64 + (kk & 3) * 8, K + at_step_mn(kk), id_o, j > 0 || kk > 0);
-                    mma_commit(&k_empty[s]);
+                        for (int kk = 0; kk < AT_TILE / 16; ++kk)
+                            at_mma_ts(O, DS + (kk >> 2) * 64 + (kk & 3) * 8, K + at_step_mn(kk), id_o, j > 0 || kk > 0);
+                    }
+                    if (leader) mma_commit(&k_empty[s]);
                     if (j + 1 < w.nk) scores(g + 1);
                 }
                 if (!good) break;
-                mma_commit(acc_full);
+                if (leader) mma_commit(acc_full);
                 ++nu;
             }
-            mma_commit(&mma_done[1]);
+            if (leader) mma_commit(&mma_done[1]);
         }
     } else {
         // ----------------------------------------------------- dS and the output

@@ -16,8 +16,7 @@
 // the same thread, so its completion also means that O_t may be rescaled.
 //
 // Warps: 0-3 and 4-7 softmax and output of tile 0 and 1 (a thread a row),
-// 8 loads, 9 and 10 the tiles' MMA issuers (one thread cannot issue
-// 128-column MMAs at the rate the tensor core takes them; two can).
+// 8 loads, 9 issues the MMAs.
 // TMEM: S0, S1, O0, O1, 128 columns each.  Persistent, one CTA per SM.
 #pragma once
 #include "attn_common.cuh"
@@ -32,8 +31,8 @@ struct AttnFwdGeom {
     static constexpr int NST = DP == 128 ? 5 : 8;  // K and V tiles in flight
     static constexpr int KV_OFF = 2 * TILE;
     static constexpr int BAR_OFF = KV_OFF + NST * TILE;
-    // q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], o_empty[2], mma_done[2], turn[2], raw, kv_full, kv_empty
-    static constexpr int NBAR = 19 + 2 * NST;
+    // q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], o_empty[2], mma_done, raw, kv_full, kv_empty
+    static constexpr int NBAR = 16 + 2 * NST;
     static constexpr int MISC_OFF = BAR_OFF + NBAR * 8;
     static constexpr int SMEM_BYTES = MISC_OFF + 16 + 1024;
     static_assert(SMEM_BYTES <= 232448, "shared memory plan exceeds 227 KB");
@@ -74,11 +73,11 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
     const uint32_t sbase = smem_u32(smem);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
     uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 10,
-             *o_empty = bars + 12, *mma_done = bars + 14, *turn = bars + 16, *raw = bars + 18, *kv_full = bars + 19,
-             *kv_empty = bars + 19 + G::NST;
+             *o_empty = bars + 12, *mma_done = bars + 14, *raw = bars + 15, *kv_full = bars + 16,
+             *kv_empty = bars + 16 + G::NST;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + G::MISC_OFF);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + G::MISC_OFF + 4);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int t = 0; t < 2; ++t) {
@@ -87,15 +86,14 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[2 * t], 4);
             mbar_init(&p_full[2 * t + 1], 4);
-            mbar_init(&turn[t], 1);
             mbar_init(&o_full[t], 1);
             mbar_init(&o_empty[t], 4);
-            mbar_init(&mma_done[t], 1);
         }
+        mbar_init(mma_done, 1);
         mbar_init(raw, 1);
         for (int s = 0; s < G::NST; ++s) {
             mbar_init(&kv_full[s], 1);
-            mbar_init(&kv_empty[s], 2);
+            mbar_init(&kv_empty[s], 1);
         }
         *abort = 0;
         fence_mbar_init();
@@ -162,87 +160,94 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
                 load_kv(j, true);
             }
         }
-    } else if (warp == 11) {
+    } else if (warp > 9) {
         at_fewer_registers();  // idle: completes the third group of four warps
-    } else if (warp > 8) {
+    } else if (warp == 9) {
         // -------------------------------------------------------------- MMAs
+        // One thread issues for both tiles, in turn: products of both issued
+        // side by side would share the tensor core and end together, and then
+        // both softmaxes would run, and wait, at the same time.
         at_fewer_registers();
-        const int t = warp - 9;
-        if (lane == 0) {
+        {
+            const bool leader = at_elect();
             constexpr int ab = DT == DT_BF16 ? 1 : 0;
             constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
-            const uint32_t S = tmem + t * 128, O = tmem + 256 + t * 128;
-            const uint64_t Q = at_desc_k(sbase + t * G::TILE), k0 = at_desc_k(sbase + G::KV_OFF),
-                           v0 = at_desc_mn(sbase + G::KV_OFF);
-            uint32_t g = 0, np = 0, nu = 0, nt = 0;
+            const uint64_t q0 = at_desc_k(sbase), k0 = at_desc_k(sbase + G::KV_OFF), v0 = at_desc_mn(sbase + G::KV_OFF);
+            uint32_t g = 0, np[2] = {0, 0}, nu[2] = {0, 0};
             bool good = true;
-            // The issuers take turns, tile 0 first: products of both tiles
-            // issued at once would share the tensor core and end together,
-            // and both softmaxes would run, and then wait, at the same time.
-            auto take_turn = [&](bool two) {
-                if (two) good = good && wait_bar(&turn[t], (nt & 1) ^ (t == 0), abort, a.err, DEVERR_TIMEOUT_ACC);
-            };
-            auto pass_turn = [&](bool two) {
-                if (two) mbar_arrive(&turn[t ^ 1]), ++nt;
-            };
             auto wait_kv = [&](uint32_t i) {
-                good = good && wait_bar(&kv_full[i % G::NST], (i / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
+                good = good && at_wait(&kv_full[i % G::NST], (i / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
                 tc_fence_after();
             };
-            auto scores = [&](uint32_t i) {
-                const uint64_t K = k0 + (i % G::NST) * (G::TILE / 16);
+            auto scores = [&](int t, uint64_t K) {
+                const uint64_t Q = q0 + t * (G::TILE / 16);
+                if (leader) {
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk)
-                    mma_f16_ss(S, Q + at_step_k(kk), K + at_step_k(kk), id_s, kk > 0);
-                mma_commit(&s_full[t]);
-                mma_commit(&kv_empty[i % G::NST]);
+                    for (int kk = 0; kk < DP / 16; ++kk)
+                        mma_f16_ss(tmem + t * 128, Q + at_step_k(kk), K + at_step_k(kk), id_s, kk > 0);
+                    mma_commit(&s_full[t]);
+                }
+            };
+            // O_t += P_t V, each half of P when it is there
+            auto mix = [&](int t, uint64_t V, bool first) {
+                const uint32_t S = tmem + t * 128, O = tmem + 256 + t * 128;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    good = good && at_wait(&p_full[2 * t + h], np[t] & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                    if (!good) return;
+                    tc_fence_after();
+                    if (leader) {
+#pragma unroll
+                        for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+                            at_mma_ts(O, S + kk * 8, V + at_step_mn(kk), id_o, !first || kk > 0);
+                    }
+                }
+                ++np[t];
             };
             for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
                 const AttnUnit w = attn_unit(a, u);
                 if (w.nk == 0) continue;
-                if (t >= w.tiles) {  // no second tile: only pass the ring on
-                    for (int j = 0; j < 2 * w.nk && good; ++j, ++g) {
-                        wait_kv(g);
-                        mbar_arrive(&kv_empty[g % G::NST]);
-                    }
-                    continue;
-                }
-                good = wait_bar(&q_full[t], nu & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
+                const bool two = w.tiles == 2;
                 wait_kv(g);
-                take_turn(w.tiles == 2);
-                if (!good) break;
-                scores(g);
-                pass_turn(w.tiles == 2);
-                for (int j = 0; j < w.nk; ++j, g += 2) {
-                    if (j == w.nk - 1) mma_commit(&q_empty[t]);  // the last scores were issued
-                    wait_kv(g + 1);
-                    good = good && wait_bar(&p_full[2 * t], np & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                    if (j == 0) good = good && wait_bar(&o_empty[t], (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                    take_turn(w.tiles == 2);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (t == 1 && !two) continue;
+                    good = good && at_wait(&q_full[t], nu[t] & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
                     if (!good) break;
                     tc_fence_after();
-                    const uint64_t V = v0 + ((g + 1) % G::NST) * (G::TILE / 16);
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        at_mma_ts(O, S + kk * 8, V + at_step_mn(kk), id_o, j > 0 || kk > 0);
-                    good = wait_bar(&p_full[2 * t + 1], np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                    if (!good) break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int kk = 4; kk < AT_TILE / 16; ++kk) at_mma_ts(O, S + kk * 8, V + at_step_mn(kk), id_o, 1);
-                    mma_commit(&kv_empty[(g + 1) % G::NST]);
-                    if (j + 1 < w.nk) {
-                        wait_kv(g + 2);
-                        if (!good) break;
-                        scores(g + 2);
-                    }
-                    pass_turn(w.tiles == 2);
+                    scores(t, k0 + (g % G::NST) * (G::TILE / 16));
+                    if (leader && w.nk == 1) mma_commit(&q_empty[t]);
                 }
-                if (!good) break;
-                mma_commit(&o_full[t]);
-                ++nu;
+                if (leader && good) mma_commit(&kv_empty[g % G::NST]);
+                for (int j = 0; j < w.nk && good; ++j, g += 2) {
+                    const int sv = (g + 1) % G::NST, sk = (g + 2) % G::NST;
+                    const bool more = j + 1 < w.nk;
+                    const uint64_t V = v0 + sv * (G::TILE / 16), K = k0 + sk * (G::TILE / 16);
+                    wait_kv(g + 1);
+                    if (more) wait_kv(g + 2);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (t == 1 && !two) continue;
+                        if (j == 0)
+                            good = good && at_wait(&o_empty[t], (nu[t] & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                        mix(t, V, j == 0);
+                        if (!good) break;
+                        if (more) {
+                            scores(t, K);
+                            if (leader && j + 2 == w.nk) mma_commit(&q_empty[t]);  // the last scores were issued
+                        } else {
+                            if (leader) mma_commit(&o_full[t]);
+                            ++nu[t];
+                        }
+                    }
+                    if (!good) break;
+                    if (leader) {
+                        mma_commit(&kv_empty[sv]);
+                        if (more) mma_commit(&kv_empty[sk]);
+                    }
+                }
             }
-            mma_commit(&mma_done[t]);
+            if (leader) mma_commit(mma_done);
         }
     } else {
         // ------------------------------------------------- softmax and output
@@ -378,13 +383,11 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
     __syncthreads();
     if (warp == 8) {
         tc_fence_after();
-        for (int t = 0; t < 2; ++t) {
-            const long long t0 = clock64();
-            while (!mbar_try_wait(&mma_done[t], 0)) {
-                if (clock64() - t0 > REELS_WAIT_LIMIT_CYCLES) {
-                    if (lane == 0) atomicOr(a.err, DEVERR_TIMEOUT_ACC);
-                    break;
-                }
+        const long long t0 = clock64();
+        while (!mbar_try_wait(mma_done, 0)) {
+            if (clock64() - t0 > REELS_WAIT_LIMIT_CYCLES) {
+                if (lane == 0) atomicOr(a.err, DEVERR_TIMEOUT_ACC);
+                break;
             }
         }
         __syncwarp();
