@@ -495,7 +495,8 @@ int reels_attention_backward(const reels_attn_shape *shape, const void *q, const
     with_dtype(act_dtype, [&](auto t) {
         e = host_launch_pdl(attn_stat_kernel<decltype(t)::value>,
                             dim3((unsigned)std::min<int64_t>(ceil_div(rows, 8), 8ll * call.sms)), dim3(256), 0, st, a,
-                            stat_l, stat_d, range);
+                            stat_l, stat_d, range,
+                            plan.tc ? AtRange<decltype(t)::value>::BWD_SHIFT : 0.0f);
     });
     RA_LAUNCH(e);
     if (!plan.tc) {

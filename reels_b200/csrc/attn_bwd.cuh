@@ -11,16 +11,14 @@
 // where one pass with scattered sums of dQ would need five.
 //
 // In both, the second product's operand (P', dS', dS) is written by the CUDA
-// cores into tensor memory over the scores it came from, which the same
-// issuing thread overwrites only after that product.  Two issuers: S and dV,
-// dP and dK (dQ kernel: S; dP and dQ), whose chains meet only in the
-// elementwise warps.
+// cores into tensor memory over the scores it came from, which the issuing
+// thread overwrites only behind that product.
 #pragma once
 #include "attn_common.cuh"
 
 namespace reels {
 
-constexpr int AB_THREADS = 32 * 12;  // 8 elementwise warps, loads, two MMA issuers, one idle
+constexpr int AB_THREADS = 32 * 12;  // 8 elementwise warps, loads, MMA issue, two idle
 
 // fp16: exponent e with |dS| 2^e <= 2^15, from |dP|, |delta| <= |dO row| |v row|.
 template <int DT>
@@ -53,22 +51,6 @@ __device__ __forceinline__ void ab_store32(const uint32_t (&o)[32], float f, typ
     }
 }
 
-// Waits for both issuers' last commits, then gives the tensor memory back.
-__device__ __forceinline__ void ab_finish(uint32_t tmem, uint64_t *mma_done, unsigned *err) {
-    tc_fence_after();
-    for (int t = 0; t < 2; ++t) {
-        const long long t0 = clock64();
-        while (!mbar_try_wait(&mma_done[t], 0)) {
-            if (clock64() - t0 > REELS_WAIT_LIMIT_CYCLES) {
-                if ((threadIdx.x & 31) == 0) atomicOr(err, DEVERR_TIMEOUT_ACC);
-                break;
-            }
-        }
-    }
-    __syncwarp();
-    tmem_dealloc(tmem, 512);
-}
-
 // ------------------------------------------------------------ dK and dV
 // Unit: a tile of 128 keys of one key head and a range of the walk over the
 // query tiles of the heads that share it.  Everything is computed transposed
@@ -85,8 +67,8 @@ struct AttnKvGeom {
     static constexpr int RING_OFF = 2 * TILE;     // behind K and V
     static constexpr int STAT_OFF = RING_OFF + NST * STAGE;  // per stage: L2[128], delta[128]
     static constexpr int BAR_OFF = STAT_OFF + NST * 1024;
-    // kv_full, kv_empty, s_full, p_full, dp_full, ds_full, acc_full, acc_empty, mma_done[2]; q_full, q_empty, g_full, g_empty
-    static constexpr int NBAR = 10 + 4 * NST;
+    // kv_full, kv_empty, s_full, p_full, dp_full, ds_full, acc_full, acc_empty, mma_done; q_full, q_empty, g_full, g_empty
+    static constexpr int NBAR = 9 + 4 * NST;
     static constexpr int MISC_OFF = BAR_OFF + NBAR * 8;
     static constexpr int SMEM_BYTES = MISC_OFF + 16 + 1024;
     static_assert(SMEM_BYTES <= 232448, "shared memory plan exceeds 227 KB");
@@ -125,27 +107,26 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
     uint64_t *kv_full = bars, *kv_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 3, *dp_full = bars + 4,
              *ds_full = bars + 5, *acc_full = bars + 6, *acc_empty = bars + 7, *mma_done = bars + 8,
-             *q_full = bars + 10, *q_empty = q_full + G::NST, *g_full = q_empty + G::NST, *g_empty = g_full + G::NST;
+             *q_full = bars + 9, *q_empty = q_full + G::NST, *g_full = q_empty + G::NST, *g_empty = g_full + G::NST;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + G::MISC_OFF);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + G::MISC_OFF + 4);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         mbar_init(kv_full, 1);
-        mbar_init(kv_empty, 2);
+        mbar_init(kv_empty, 1);
         mbar_init(s_full, 1);
         mbar_init(p_full, 8);
         mbar_init(dp_full, 1);
         mbar_init(ds_full, 8);
-        mbar_init(acc_full, 2);
+        mbar_init(acc_full, 1);
         mbar_init(acc_empty, 8);
-        mbar_init(&mma_done[0], 1);
-        mbar_init(&mma_done[1], 1);
+        mbar_init(mma_done, 1);
         for (int s = 0; s < G::NST; ++s) {
             mbar_init(&q_full[s], 1);
-            mbar_init(&q_empty[s], 2);
+            mbar_init(&q_empty[s], 1);
             mbar_init(&g_full[s], 1);
-            mbar_init(&g_empty[s], 2);
+            mbar_init(&g_empty[s], 1);
         }
         *abort = 0;
         fence_mbar_init();
@@ -201,68 +182,67 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                 }
             }
         }
-    } else if (warp == 11) {
+    } else if (warp > 9) {
         at_fewer_registers();  // idle: completes the third group of four warps
-    } else if (warp > 8) {
-        // ------------------------------------------------- MMAs: 9 S', dV; 10 dP', dK
+    } else if (warp == 9) {
+        // -------------------------------------------------------------- MMAs
+        // In turn: dV(i), S'(i+1) run under the elementwise dS(i), and dK(i),
+        // dP'(i+1) under the exponentials of step i+1.
         at_fewer_registers();
-        const int second = warp - 9;
-        {
-            const bool leader = at_elect();
-            constexpr int ab = DT == DT_BF16 ? 1 : 0;
-            constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
-            const uint32_t S = tmem + second * 128, O = tmem + 256 + second * 128;
-            const uint64_t A = at_desc_k(sbase + second * G::TILE);
-            // score operand of a stage (Q, dO), and the other one (dO, Q)
-            uint64_t *in_full = second ? g_full : q_full, *in_empty = second ? g_empty : q_empty;
-            uint64_t *ot_full = second ? q_full : g_full, *ot_empty = second ? q_empty : g_empty;
-            uint64_t *scored = second ? dp_full : s_full, *ready = second ? ds_full : p_full;
-            const uint64_t in0 = at_desc_k(sbase + G::RING_OFF + (second ? G::TILE : 0)),
-                           ot0 = at_desc_mn(sbase + G::RING_OFF + (second ? 0 : G::TILE));
-            uint32_t g = 0, np = 0, nu = 0;
-            bool good = true;
-            auto scores = [&](uint32_t i) {
-                const int s = i % G::NST;
-                good = good && at_wait(&in_full[s], (i / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
-                if (!good) return;
-                tc_fence_after();
-                const uint64_t B = in0 + s * (G::STAGE / 16);
-                if (leader) {
+        const bool leader = at_elect();
+        constexpr int ab = DT == DT_BF16 ? 1 : 0;
+        constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
+        const uint64_t kv0 = at_desc_k(sbase), in0 = at_desc_k(sbase + G::RING_OFF),
+                       mn0 = at_desc_mn(sbase + G::RING_OFF);
+        uint32_t g = 0, np = 0, nu = 0;
+        bool good = true;
+        // which = 0: S' = K Q', 1: dP' = V dO'
+        auto scores = [&](int which, uint32_t i) {
+            const int s = i % G::NST;
+            good = good && at_wait(which ? &g_full[s] : &q_full[s], (i / G::NST) & 1, abort, a.err,
+                                   DEVERR_TIMEOUT_AB_FULL);
+            if (!good) return;
+            tc_fence_after();
+            const uint64_t A = kv0 + which * (G::TILE / 16), B = in0 + s * (G::STAGE / 16) + which * (G::TILE / 16);
+            if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < DP / 16; ++kk)
-                        mma_f16_ss(S, A + at_step_k(kk), B + at_step_k(kk), id_s, kk > 0);
-                }
-                if (leader) mma_commit(scored);
-                if (leader) mma_commit(&in_empty[s]);
-            };
-            for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
-                const AttnKvUnit w = attn_kv_unit(a, u);
-                if (w.n == 0) continue;
-                good = at_wait(kv_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
-                scores(g);
-                for (int i = 0; i < w.n && good; ++i, ++g) {
-                    const int s = g % G::NST;
-                    if (leader && i == w.n - 1) mma_commit(kv_empty);  // the last scores were issued
-                    good = at_wait(&ot_full[s], (g / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL) &&
-                           at_wait(ready, np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                    if (i == 0) good = good && at_wait(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                    if (!good) break;
-                    tc_fence_after();
-                    const uint64_t B = ot0 + s * (G::STAGE / 16);
-                    if (leader) {
-#pragma unroll
-                        for (int kk = 0; kk < AT_TILE / 16; ++kk)
-                            at_mma_ts(O, S + (kk >> 2) * 64 + (kk & 3) * 8, B + at_step_mn(kk), id_o, i > 0 || kk > 0);
-                    }
-                    if (leader) mma_commit(&ot_empty[s]);
-                    if (i + 1 < w.n) scores(g + 1);
-                }
-                if (!good) break;
-                if (leader) mma_commit(acc_full);
-                ++nu;
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_f16_ss(tmem + 128 * which, A + at_step_k(kk), B + at_step_k(kk), id_s, kk > 0);
+                mma_commit(which ? dp_full : s_full);
             }
-            if (leader) mma_commit(&mma_done[second]);
+        };
+        // which = 0: dV += P' dO, 1: dK += dS' Q
+        auto mix = [&](int which, uint32_t i, bool first) {
+            const int s = i % G::NST;
+            good = good && at_wait(which ? ds_full : p_full, np & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+            if (!good) return;
+            tc_fence_after();
+            const uint32_t S = tmem + 128 * which, O = tmem + 256 + 128 * which;
+            const uint64_t B = mn0 + s * (G::STAGE / 16) + (which ^ 1) * (G::TILE / 16);
+            if (leader) {
+#pragma unroll
+                for (int kk = 0; kk < AT_TILE / 16; ++kk)
+                    at_mma_ts(O, S + (kk >> 2) * 64 + (kk & 3) * 8, B + at_step_mn(kk), id_o, !first || kk > 0);
+                mma_commit(which ? &q_empty[s] : &g_empty[s]);  // dK is the last to read Q, dV dO
+            }
+        };
+        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+            const AttnKvUnit w = attn_kv_unit(a, u);
+            if (w.n == 0) continue;
+            good = at_wait(kv_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
+            scores(0, g);
+            scores(1, g);
+            if (good) good = at_wait(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+            for (int i = 0; i < w.n && good; ++i, ++g, ++np) {
+                mix(0, g, i == 0);
+                if (i + 1 < w.n) scores(0, g + 1);
+                mix(1, g, i == 0);
+                if (i + 1 < w.n) scores(1, g + 1);
+                else if (leader) mma_commit(kv_empty), mma_commit(acc_full);
+            }
+            ++nu;
         }
+        if (leader) mma_commit(mma_done);
     } else {
         // --------------------------------------------- P', dS' and the output
         at_more_registers();
@@ -270,8 +250,10 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t S = tmem + lanes + 64 * half, DS = S + 128, O = tmem + lanes + 256 + 128 * half;
         const float c = a.scale * CUDART_L2E_F;
+        const F2 c2 = F2(c, c);
         const int e = attn_grad_exp<DT>(a);
-        const float grow = exp2f((float)e - AtRange<DT>::BWD_SHIFT);
+        const float g1 = exp2f((float)e - AtRange<DT>::BWD_SHIFT);
+        const F2 grow = F2(g1, g1);
         const float f = half ? a.scale * exp2f(-(float)e) : exp2f(-AtRange<DT>::BWD_SHIFT);
         uint32_t g = 0, ns = 0, nu = 0;
         bool good = true;
@@ -281,8 +263,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
             const bool live = row < w.rows;
             for (int i = 0; i < w.n; ++i, ++g, ++ns) {
                 const int s = g % G::NST;
-                const float4 *L = reinterpret_cast<const float4 *>(smem + G::STAT_OFF + s * 1024 + half * 256);
-                const float4 *Dl = L + 32;
+                const uint32_t L = sbase + G::STAT_OFF + s * 1024 + half * 256, Dl = L + 512;
                 good = at_wait(&q_full[s], (g / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL) &&
                        at_wait(s_full, ns & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
                 if (!good) break;
@@ -293,20 +274,17 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                 tmem_wait_ld();
                 uint32_t p[32];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const float4 l = L[k];
-                    float v[4];
-                    v[0] = at_exp2(fmaf(__uint_as_float(x[4 * k]), c, AtRange<DT>::BWD_SHIFT - l.x));
-                    v[1] = at_exp2(fmaf(__uint_as_float(x[4 * k + 1]), c, AtRange<DT>::BWD_SHIFT - l.y));
-                    v[2] = at_exp2(fmaf(__uint_as_float(x[4 * k + 2]), c, AtRange<DT>::BWD_SHIFT - l.z));
-                    v[3] = at_exp2(fmaf(__uint_as_float(x[4 * k + 3]), c, AtRange<DT>::BWD_SHIFT - l.w));
+                for (int k = 0; k < 32; k += 2) {
+                    const float4 l = ld_shared_f4(L + 8 * k);
+                    const float2 u = fma2(at_pair(x, k), c2, F2(l.x, l.y)).get();
+                    const float2 v = fma2(at_pair(x, k + 1), c2, F2(l.z, l.w)).get();
+                    x[2 * k] = __float_as_uint(at_exp2(u.x)), x[2 * k + 1] = __float_as_uint(at_exp2(u.y));
+                    x[2 * k + 2] = __float_as_uint(at_exp2(v.x)), x[2 * k + 3] = __float_as_uint(at_exp2(v.y));
+                    p[k] = at_pack<DT>(at_pair(x, k)), p[k + 1] = at_pack<DT>(at_pair(x, k + 1));
+                }
+                if (w.rows < AT_TILE && !live) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (!live) v[j] = 0.0f;
-                        x[4 * k + j] = __float_as_uint(v[j]);
-                    }
-                    p[2 * k] = Elem<DT>::pack2(v[0], v[1]);
-                    p[2 * k + 1] = Elem<DT>::pack2(v[2], v[3]);
+                    for (int k = 0; k < 32; ++k) p[k] = 0u;
                 }
                 at_tmem_st32(S, p);
                 at_tmem_wait_st();
@@ -321,20 +299,16 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                 at_tmem_ld32(DS + 32, y + 32);
                 tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const float4 d = Dl[k];
-                    float v[4];
-                    v[0] = __uint_as_float(x[4 * k]) * (__uint_as_float(y[4 * k]) - d.x);
-                    v[1] = __uint_as_float(x[4 * k + 1]) * (__uint_as_float(y[4 * k + 1]) - d.y);
-                    v[2] = __uint_as_float(x[4 * k + 2]) * (__uint_as_float(y[4 * k + 2]) - d.z);
-                    v[3] = __uint_as_float(x[4 * k + 3]) * (__uint_as_float(y[4 * k + 3]) - d.w);
+                for (int k = 0; k < 32; k += 2) {
+                    const float4 d = ld_shared_f4(Dl + 8 * k);
+                    F2 u = mul2(at_pair(x, k), add2(at_pair(y, k), F2(d.x, d.y)));
+                    F2 v = mul2(at_pair(x, k + 1), add2(at_pair(y, k + 1), F2(d.z, d.w)));
+                    if (DT == DT_F16) u = mul2(u, grow), v = mul2(v, grow);
+                    p[k] = at_pack<DT>(u), p[k + 1] = at_pack<DT>(v);
+                }
+                if (w.rows < AT_TILE && !live) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (DT == DT_F16) v[j] *= grow;
-                        if (!live) v[j] = 0.0f;
-                    }
-                    p[2 * k] = Elem<DT>::pack2(v[0], v[1]);
-                    p[2 * k + 1] = Elem<DT>::pack2(v[2], v[3]);
+                    for (int k = 0; k < 32; ++k) p[k] = 0u;
                 }
                 at_tmem_st32(DS, p);
                 at_tmem_wait_st();
@@ -381,7 +355,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) ab_finish(tmem, mma_done, a.err);
+    if (warp == 8) at_finish(tmem, mma_done, a.err);
 }
 
 // Adds the partial dK and dV of the split walk in order.
@@ -411,8 +385,8 @@ struct AttnQGeom {
     static constexpr int K_OFF = 2 * TILE;  // behind Q and dO
     static constexpr int V_OFF = K_OFF + NK * TILE;
     static constexpr int BAR_OFF = V_OFF + NV * TILE;
-    // q_full, q_empty, s_full[2], s_empty[2], dp_full, ds_full, acc_full, acc_empty, raw, mma_done[2]; rings
-    static constexpr int NBAR = 13 + 2 * (NK + NV);
+    // q_full, q_empty, s_full[2], s_empty[2], dp_full, ds_full, acc_full, acc_empty, raw, mma_done; rings
+    static constexpr int NBAR = 12 + 2 * (NK + NV);
     static constexpr int MISC_OFF = BAR_OFF + NBAR * 8;
     static constexpr int SMEM_BYTES = MISC_OFF + 16 + 1024;
     static_assert(SMEM_BYTES <= 232448, "shared memory plan exceeds 227 KB");
@@ -446,27 +420,27 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
     uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *s_empty = bars + 4, *dp_full = bars + 6,
              *ds_full = bars + 7, *acc_full = bars + 8, *acc_empty = bars + 9, *raw = bars + 10, *mma_done = bars + 11,
-             *k_full = bars + 13, *k_empty = k_full + G::NK, *v_full = k_empty + G::NK, *v_empty = v_full + G::NV;
+             *k_full = bars + 12, *k_empty = k_full + G::NK, *v_full = k_empty + G::NK, *v_empty = v_full + G::NV;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + G::MISC_OFF);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + G::MISC_OFF + 4);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
-        mbar_init(q_empty, 2);
+        mbar_init(q_empty, 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&s_full[s], 1);
             mbar_init(&s_empty[s], 8);
-            mbar_init(&mma_done[s], 1);
         }
         mbar_init(dp_full, 1);
         mbar_init(ds_full, 8);
         mbar_init(acc_full, 1);
         mbar_init(acc_empty, 8);
+        mbar_init(mma_done, 1);
         mbar_init(raw, 1);
         for (int s = 0; s < G::NK; ++s) {
             mbar_init(&k_full[s], 1);
-            mbar_init(&k_empty[s], 2);
+            mbar_init(&k_empty[s], 1);
         }
         for (int s = 0; s < G::NV; ++s) {
             mbar_init(&v_full[s], 1);
@@ -532,94 +506,76 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                 }
             }
         }
-    } else if (warp == 9) {
-        // ---------------------------------------------------------- MMAs: S
-        at_fewer_registers();
-        {
-            const bool leader = at_elect();
-            constexpr uint32_t id_s = idesc_f16(DT == DT_BF16 ? 1 : 0, 0, 0, 128, AT_TILE);
-            const uint64_t Q = at_desc_k(sbase), k0 = at_desc_k(sbase + G::K_OFF);
-            uint32_t g = 0, nu = 0;
-            bool good = true;
-            for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
-                const AttnQUnit w = attn_q_unit(a, u);
-                if (w.nk == 0) continue;
-                good = at_wait(q_full, nu++ & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
-                for (int j = 0; j < w.nk && good; ++j, ++g) {
-                    const int s = g % G::NK, t = g & 1;
-                    good = at_wait(&k_full[s], (g / G::NK) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL) &&
-                           at_wait(&s_empty[t], ((g >> 1) & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                    if (!good) break;
-                    tc_fence_after();
-                    const uint64_t K = k0 + s * (G::TILE / 16);
-                    if (leader) {
-#pragma unroll
-                        for (int kk = 0; kk < DP / 16; ++kk)
-                            mma_f16_ss(tmem + 128 * t, Q + at_step_k(kk), K + at_step_k(kk), id_s, kk > 0);
-                    }
-                    if (leader) mma_commit(&s_full[t]);
-                    if (leader) mma_commit(&k_empty[s]);
-                }
-                if (leader && good) mma_commit(q_empty);
-            }
-            if (leader) mma_commit(&mma_done[0]);
-        }
-    } else if (warp == 11) {
+    } else if (warp > 9) {
         at_fewer_registers();  // idle: completes the third group of four warps
-    } else if (warp == 10) {
-        // ---------------------------------------------------- MMAs: dP and dQ
+    } else if (warp == 9) {
+        // -------------------------------------------------------------- MMAs
+        // In turn: dQ(j), dP(j+1), S(j+2); the scores run two tiles ahead of
+        // the elementwise warps' dS.
         at_fewer_registers();
-        {
-            const bool leader = at_elect();
-            constexpr int ab = DT == DT_BF16 ? 1 : 0;
-            constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
-            const uint32_t DS = tmem + 256, O = tmem + 384;
-            const uint64_t dO = at_desc_k(sbase + G::TILE), v0 = at_desc_k(sbase + G::V_OFF),
-                           k0 = at_desc_mn(sbase + G::K_OFF);
-            uint32_t g = 0, nu = 0, np = 0;
-            bool good = true;
-            auto scores = [&](uint32_t i) {
-                const int t = i % G::NV;
-                good = good && at_wait(&v_full[t], (i / G::NV) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
-                if (!good) return;
+        const bool leader = at_elect();
+        constexpr int ab = DT == DT_BF16 ? 1 : 0;
+        constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
+        const uint32_t DS = tmem + 256, O = tmem + 384;
+        const uint64_t Q = at_desc_k(sbase), dO = at_desc_k(sbase + G::TILE), k0 = at_desc_k(sbase + G::K_OFF),
+                       v0 = at_desc_k(sbase + G::V_OFF), mn0 = at_desc_mn(sbase + G::K_OFF);
+        uint32_t g = 0, nu = 0, np = 0;
+        bool good = true;
+        auto scores = [&](uint32_t i) {
+            const int s = i % G::NK, t = i & 1;
+            good = good && at_wait(&k_full[s], (i / G::NK) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL) &&
+                   at_wait(&s_empty[t], ((i >> 1) & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+            if (!good) return;
+            tc_fence_after();
+            const uint64_t K = k0 + s * (G::TILE / 16);
+            if (leader) {
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_f16_ss(tmem + 128 * t, Q + at_step_k(kk), K + at_step_k(kk), id_s, kk > 0);
+                mma_commit(&s_full[t]);
+            }
+        };
+        auto grads = [&](uint32_t i) {  // dP
+            const int t = i % G::NV;
+            good = good && at_wait(&v_full[t], (i / G::NV) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
+            if (!good) return;
+            tc_fence_after();
+            const uint64_t V = v0 + t * (G::TILE / 16);
+            if (leader) {
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_f16_ss(DS, dO + at_step_k(kk), V + at_step_k(kk), id_s, kk > 0);
+                mma_commit(dp_full);
+                mma_commit(&v_empty[t]);
+            }
+        };
+        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+            const AttnQUnit w = attn_q_unit(a, u);
+            if (w.nk == 0) continue;
+            good = at_wait(q_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
+            scores(g);
+            grads(g);
+            if (w.nk > 1) scores(g + 1);
+            if (good) good = at_wait(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+            for (int j = 0; j < w.nk && good; ++j, ++g, ++np) {
+                const int s = g % G::NK;
+                good = at_wait(ds_full, np & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
+                if (!good) break;
                 tc_fence_after();
-                const uint64_t V = v0 + t * (G::TILE / 16);
+                const uint64_t K = mn0 + s * (G::TILE / 16);
                 if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < DP / 16; ++kk)
-                        mma_f16_ss(DS, dO + at_step_k(kk), V + at_step_k(kk), id_s, kk > 0);
+                    for (int kk = 0; kk < AT_TILE / 16; ++kk)
+                        at_mma_ts(O, DS + (kk >> 2) * 64 + (kk & 3) * 8, K + at_step_mn(kk), id_o, j > 0 || kk > 0);
+                    mma_commit(&k_empty[s]);  // dQ is the last to read K
                 }
-                if (leader) mma_commit(dp_full);
-                if (leader) mma_commit(&v_empty[t]);
-            };
-            for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
-                const AttnQUnit w = attn_q_unit(a, u);
-                if (w.nk == 0) continue;
-                good = at_wait(q_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
-                scores(g);
-                for (int j = 0; j < w.nk && good; ++j, ++g) {
-                    const int s = g % G::NK;
-                    if (leader && j == w.nk - 1) mma_commit(q_empty);  // the last product with dO was issued
-                    good = at_wait(&k_full[s], (g / G::NK) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL) &&
-                           at_wait(ds_full, np++ & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                    if (j == 0) good = good && at_wait(acc_empty, (nu & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                    if (!good) break;
-                    tc_fence_after();
-                    const uint64_t K = k0 + s * (G::TILE / 16);
-                    if (leader) {
-#pragma unroll
-                        for (int kk = 0; kk < AT_TILE / 16; ++kk)
-                            at_mma_ts(O, DS + (kk >> 2) * 64 + (kk & 3) * 8, K + at_step_mn(kk), id_o, j > 0 || kk > 0);
-                    }
-                    if (leader) mma_commit(&k_empty[s]);
-                    if (j + 1 < w.nk) scores(g + 1);
-                }
-                if (!good) break;
-                if (leader) mma_commit(acc_full);
-                ++nu;
+                if (j + 1 < w.nk) grads(g + 1);
+                else if (leader) mma_commit(q_empty), mma_commit(acc_full);
+                if (j + 2 < w.nk) scores(g + 2);
             }
-            if (leader) mma_commit(&mma_done[1]);
+            ++nu;
         }
+        if (leader) mma_commit(mma_done);
     } else {
         // ----------------------------------------------------- dS and the output
         at_more_registers();
@@ -628,14 +584,17 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
         const uint32_t DS = tmem + lanes + 256 + 64 * half, O = tmem + lanes + 384;
         const float c = a.scale * CUDART_L2E_F;
         const int e = attn_grad_exp<DT>(a);
-        const float grow = exp2f((float)e), f = a.scale * exp2f(-(float)e);
+        const F2 c2 = F2(c, c);
+        const float g1 = exp2f((float)e - AtRange<DT>::BWD_SHIFT), f = a.scale * exp2f(-(float)e);
+        const F2 grow = F2(g1, g1);
         uint32_t g = 0, nu = 0;
         bool good = true;
         for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
             const AttnQUnit w = attn_q_unit(a, u);
             const int row = w.q0 + (warp & 3) * 32 + lane;
             const long long st = ((long long)w.b * a.H + w.h) * a.Sqp + row;
-            const float L = __ldcg(a.stat_l + st), delta = __ldcg(a.stat_d + st);
+            const float sl = __ldcg(a.stat_l + st), sd = __ldcg(a.stat_d + st);
+            const F2 L = F2(sl, sl), delta = F2(sd, sd);
             for (int j = 0; j < w.nk; ++j, ++g) {
                 const int t = g & 1;
                 good = at_wait(&s_full[t], (g >> 1) & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
@@ -649,7 +608,10 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s_empty[t]);
 #pragma unroll
-                for (int k = 0; k < 64; ++k) x[k] = __float_as_uint(at_exp2(fmaf(__uint_as_float(x[k]), c, -L)));
+                for (int k = 0; k < 32; ++k) {
+                    const float2 u = fma2(at_pair(x, k), c2, L).get();
+                    x[2 * k] = __float_as_uint(at_exp2(u.x)), x[2 * k + 1] = __float_as_uint(at_exp2(u.y));
+                }
                 good = at_wait(dp_full, g & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
                 if (!good) break;
                 tc_fence_after();
@@ -658,21 +620,20 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                 at_tmem_ld32(DS + 32, y + 32);
                 tmem_wait_ld();
                 const int rows = w.len - j * AT_TILE - 64 * half;
+                uint32_t p[32];
 #pragma unroll
-                for (int k = 0; k < 64; ++k) {
-                    float v = __uint_as_float(x[k]) * (__uint_as_float(y[k]) - delta);
-                    if (DT == DT_F16) v *= grow;
-                    y[k] = __float_as_uint(v);
+                for (int k = 0; k < 32; ++k) {
+                    F2 u = mul2(at_pair(x, k), add2(at_pair(y, k), delta));
+                    if (DT == DT_F16) u = mul2(u, grow);
+                    p[k] = at_pack<DT>(u);
                 }
                 if (rows < 64) {
 #pragma unroll
-                    for (int k = 0; k < 64; ++k)
-                        if (k >= rows) y[k] = 0u;
+                    for (int k = 0; k < 32; ++k) {  // keys 2k, 2k + 1
+                        if (2 * k >= rows) p[k] = 0u;
+                        else if (2 * k + 1 >= rows) p[k] &= 0xffffu;
+                    }
                 }
-                uint32_t p[32];
-#pragma unroll
-                for (int k = 0; k < 32; ++k)
-                    p[k] = Elem<DT>::pack2(__uint_as_float(y[2 * k]), __uint_as_float(y[2 * k + 1]));
                 at_tmem_st32(DS, p);
                 at_tmem_wait_st();
                 tc_fence_before();
@@ -715,7 +676,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) ab_finish(tmem, mma_done, a.err);
+    if (warp == 8) at_finish(tmem, mma_done, a.err);
 }
 
 }  // namespace reels

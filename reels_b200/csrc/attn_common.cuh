@@ -99,6 +99,16 @@ __device__ __forceinline__ float at_max3(float a, float b, float c) {
     return d;
 }
 
+// A pair of neighbouring accumulator columns.
+__device__ __forceinline__ F2 at_pair(const uint32_t *r, int k) {
+    return F2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1]));
+}
+template <int DT>
+__device__ __forceinline__ uint32_t at_pack(F2 v) {
+    const float2 f = v.get();
+    return Elem<DT>::pack2(f.x, f.y);
+}
+
 // Probabilities are at most 1 (2^8 before the running maximum catches up) and
 // fall to 2^-15 and below on long rows.  bf16 holds that range as it is; fp16
 // gets them multiplied by a power of two that uses its range up to 2^15 and
@@ -121,6 +131,20 @@ __device__ __forceinline__ bool at_wait(uint64_t *bar, uint32_t parity, volatile
                                         unsigned code) {
     const bool ok = wait_bar(bar, parity, abort, err, code);
     return __all_sync(0xffffffffu, ok);
+}
+
+// Waits for the issuer's last commit, then gives the tensor memory back.
+__device__ __forceinline__ void at_finish(uint32_t tmem, uint64_t *mma_done, unsigned *err) {
+    tc_fence_after();
+    const long long t0 = clock64();
+    while (!mbar_try_wait(mma_done, 0)) {
+        if (clock64() - t0 > REELS_WAIT_LIMIT_CYCLES) {
+            if ((threadIdx.x & 31) == 0) atomicOr(err, DEVERR_TIMEOUT_ACC);
+            break;
+        }
+    }
+    __syncwarp();
+    tmem_dealloc(tmem, 512);
 }
 
 // Zeroes rows from `first` on of an operand tile: keys behind a sample's

@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t S = tmem + t * 128 + lanes, O = tmem + 256 + t * 128 + lanes;
         const float c = a.scale * CUDART_L2E_F;
+        const F2 c2 = F2(c, c);
         uint32_t ns = 0, nu = 0;
         bool good = true;
         for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
@@ -304,17 +305,17 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
                         at_tmem_st32(O + 32 * i, o);
                     }
                 }
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const F2 m2 = F2(-m, -m);
+                F2 sum[2] = {F2(0.0f, 0.0f), F2(0.0f, 0.0f)};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t p[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float x = at_exp2(fmaf(__uint_as_float(s[32 * i + 2 * e]), c, -m));
-                        const float y = at_exp2(fmaf(__uint_as_float(s[32 * i + 2 * e + 1]), c, -m));
-                        p[e] = Elem<DT>::pack2(x, y);
-                        sum[e & 1] += x;
-                        sum[2 + (e & 1)] += y;
+                        const float2 u = fma2(at_pair(s + 32 * i, e), c2, m2).get();
+                        const F2 v = F2(at_exp2(u.x), at_exp2(u.y));
+                        p[e] = at_pack<DT>(v);
+                        sum[e & 1] = add2(sum[e & 1], v);
                     }
                     at_tmem_st16(S + 16 * i, p);
                     if (i & 1) {  // half of P: its products may start
@@ -324,7 +325,8 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
                         if (lane == 0) mbar_arrive(&p_full[2 * t + (i >> 1)]);
                     }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                const float2 total = add2(sum[0], sum[1]).get();
+                l += total.x + total.y;
             }
             if (!good) break;
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
@@ -381,18 +383,7 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
-        tc_fence_after();
-        const long long t0 = clock64();
-        while (!mbar_try_wait(mma_done, 0)) {
-            if (clock64() - t0 > REELS_WAIT_LIMIT_CYCLES) {
-                if (lane == 0) atomicOr(a.err, DEVERR_TIMEOUT_ACC);
-                break;
-            }
-        }
-        __syncwarp();
-        tmem_dealloc(tmem, 512);
-    }
+    if (warp == 8) at_finish(tmem, mma_done, a.err);
 }
 
 }  // namespace reels

@@ -34,7 +34,7 @@ struct AttnArgs {
     float *part_o, *part_lse;                // [splits][B][H][Sq][D], [splits][B][H][Sq]
     // backward
     const void *dout;                        // [B][Sq][H][D]
-    const float *stat_l, *stat_d;            // [B][H][Sqp]: L in log2 units (+inf: no part), delta
+    const float *stat_l, *stat_d;            // [B][H][Sqp]: -L in log2 units (-inf: no part), -delta
     int Sqp;                                 // Sq rounded up to whole tiles
     void *dq, *dk, *dv;                      // contiguous, in the layout of q, k and v
     const unsigned *range;                   // fp16: largest |dO row|, |v row| (float bits)
@@ -204,18 +204,19 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
     }
 }
 
-// Row statistics of the gradient: (L in log2 units, delta) of every query row,
-// padded to Sqp rows a head.  Rows without keys and padding get L = +inf, so
-// their probabilities come out as exp2(-inf) = 0.  One warp a row.
+// Row statistics of the gradient, as the terms that are added: -L in log2
+// units plus `shift` (fp16, see AtRange) and -delta of every query row, padded
+// to Sqp rows a head.  Rows without keys and padding get -inf, so that their
+// probabilities come out as exp2(-inf) = 0.  One warp a row.
 template <int DT>
-__global__ void __launch_bounds__(256) attn_stat_kernel(const AttnArgs a, float *stat_l, float *stat_d, unsigned *range) {
+__global__ void __launch_bounds__(256) attn_stat_kernel(const AttnArgs a, float *stat_l, float *stat_d, unsigned *range, float shift) {
     griddep_wait();
     const int lane = threadIdx.x & 31;
     const long long rows = (long long)a.B * a.H * a.Sqp;
     float top = 0.0f;  // fp16: largest |dO row|^2
     for (long long row = blockIdx.x * 8ll + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8ll) {
         const int q = (int)(row % a.Sqp), h = (int)(row / a.Sqp % a.H), b = (int)(row / a.Sqp / a.H);
-        float2 st = make_float2(CUDART_INF_F, 0.0f);
+        float2 st = make_float2(-CUDART_INF_F, 0.0f);
         if (q < a.Sq) {
             const long long at = (((long long)b * a.Sq + q) * a.H + h) * a.D;
             float delta = 0.0f, n2 = 0.0f;
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(256) attn_stat_kernel(const AttnArgs a, float 
                 n2 += __shfl_xor_sync(0xffffffffu, n2, w);
             }
             const float lse = __ldcg(a.lse + ((long long)b * a.H + h) * a.Sq + q);
-            if (lse != -CUDART_INF_F) st = make_float2(lse * CUDART_L2E_F, delta);
+            if (lse != -CUDART_INF_F) st = make_float2(shift - lse * CUDART_L2E_F, -delta);
             top = fmaxf(top, n2);
         }
         if (lane == 0) {
@@ -293,11 +294,11 @@ __device__ __forceinline__ void as_grad_tile(const AttnArgs &a, const float *Q, 
         const float2 st = make_float2(__ldcg(a.stat_l + stat_at + 2 * ty + i), __ldcg(a.stat_d + stat_at + 2 * ty + i));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const bool in = k0 + tx + 8 * j < len && st.x != CUDART_INF_F;
-            const float p = in ? exp2f(s[i][j] * a.scale * CUDART_L2E_F - st.x) : 0.0f;
+            const bool in = k0 + tx + 8 * j < len && st.x != -CUDART_INF_F;
+            const float p = in ? exp2f(s[i][j] * a.scale * CUDART_L2E_F + st.x) : 0.0f;
             const int at = (2 * ty + i) * (AS_T + 1) + tx + 8 * j;
             P[at] = p;
-            S[at] = in ? p * (dp[i][j] - st.y) : 0.0f;
+            S[at] = in ? p * (dp[i][j] + st.y) : 0.0f;
         }
     }
 }

@@ -103,28 +103,6 @@ __device__ __forceinline__ int nr_axis(const NormRopeArgs &a, int i, int &base) 
     return 2;
 }
 
-// Two fp32 values in one register pair, and the packed arithmetic on them.
-struct F2 {
-    unsigned long long v;
-    __device__ __forceinline__ F2() {}
-    __device__ __forceinline__ F2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
-    __device__ __forceinline__ float2 get() const {
-        float2 r;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-        return r;
-    }
-};
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-
 // Eight consecutive elements, from memory to four packed pairs and back.
 template <int DT>
 __device__ __forceinline__ void nr_read(const typename Elem<DT>::T *p, F2 (&v)[4]) {
