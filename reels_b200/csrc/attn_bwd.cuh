@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) at_finish(tmem, mma_done, a.err);
+    if (warp == 8) at_finish(tmem, mma_done, 1, a.err);
 }
 
 // Adds the partial dK and dV of the split walk in order.
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) at_finish(tmem, mma_done, a.err);
+    if (warp == 8) at_finish(tmem, mma_done, 1, a.err);
 }
 
 }  // namespace reels

@@ -133,14 +133,16 @@ __device__ __forceinline__ bool at_wait(uint64_t *bar, uint32_t parity, volatile
     return __all_sync(0xffffffffu, ok);
 }
 
-// Waits for the issuer's last commit, then gives the tensor memory back.
-__device__ __forceinline__ void at_finish(uint32_t tmem, uint64_t *mma_done, unsigned *err) {
+// Waits for the issuers' last commits, then gives the tensor memory back.
+__device__ __forceinline__ void at_finish(uint32_t tmem, uint64_t *mma_done, int issuers, unsigned *err) {
     tc_fence_after();
-    const long long t0 = clock64();
-    while (!mbar_try_wait(mma_done, 0)) {
-        if (clock64() - t0 > REELS_WAIT_LIMIT_CYCLES) {
-            if ((threadIdx.x & 31) == 0) atomicOr(err, DEVERR_TIMEOUT_ACC);
-            break;
+    for (int t = 0; t < issuers; ++t) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&mma_done[t], 0)) {
+            if (clock64() - t0 > REELS_WAIT_LIMIT_CYCLES) {
+                if ((threadIdx.x & 31) == 0) atomicOr(err, DEVERR_TIMEOUT_ACC);
+                break;
+            }
         }
     }
     __syncwarp();

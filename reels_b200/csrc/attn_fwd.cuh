@@ -16,7 +16,7 @@
 // the same thread, so its completion also means that O_t may be rescaled.
 //
 // Warps: 0-3 and 4-7 softmax and output of tile 0 and 1 (a thread a row),
-// 8 loads, 9 issues the MMAs.
+// 8 loads, 9 and 10 issue the tiles' MMAs.
 // TMEM: S0, S1, O0, O1, 128 columns each.  Persistent, one CTA per SM.
 #pragma once
 #include "attn_common.cuh"
@@ -31,8 +31,8 @@ struct AttnFwdGeom {
     static constexpr int NST = DP == 128 ? 5 : 8;  // K and V tiles in flight
     static constexpr int KV_OFF = 2 * TILE;
     static constexpr int BAR_OFF = KV_OFF + NST * TILE;
-    // q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], o_empty[2], mma_done, raw, kv_full, kv_empty
-    static constexpr int NBAR = 16 + 2 * NST;
+    // q_full[2], q_empty[2], s_full[2], p_full[2][2], o_full[2], o_empty[2], mma_done[2], turn[2], raw, kv_full, kv_empty
+    static constexpr int NBAR = 19 + 2 * NST;
     static constexpr int MISC_OFF = BAR_OFF + NBAR * 8;
     static constexpr int SMEM_BYTES = MISC_OFF + 16 + 1024;
     static_assert(SMEM_BYTES <= 232448, "shared memory plan exceeds 227 KB");
@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
     const uint32_t sbase = smem_u32(smem);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
     uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 10,
-             *o_empty = bars + 12, *mma_done = bars + 14, *raw = bars + 15, *kv_full = bars + 16,
-             *kv_empty = bars + 16 + G::NST;
+             *o_empty = bars + 12, *mma_done = bars + 14, *turn = bars + 16, *raw = bars + 18, *kv_full = bars + 19,
+             *kv_empty = bars + 19 + G::NST;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + G::MISC_OFF);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + G::MISC_OFF + 4);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -86,14 +86,15 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[2 * t], 4);
             mbar_init(&p_full[2 * t + 1], 4);
+            mbar_init(&turn[t], 1);
+            mbar_init(&mma_done[t], 1);
             mbar_init(&o_full[t], 1);
             mbar_init(&o_empty[t], 4);
         }
-        mbar_init(mma_done, 1);
         mbar_init(raw, 1);
         for (int s = 0; s < G::NST; ++s) {
             mbar_init(&kv_full[s], 1);
-            mbar_init(&kv_empty[s], 1);
+            mbar_init(&kv_empty[s], 2);
         }
         *abort = 0;
         fence_mbar_init();
@@ -160,95 +161,97 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
                 load_kv(j, true);
             }
         }
-    } else if (warp > 9) {
+    } else if (warp == 11) {
         at_fewer_registers();  // idle: completes the third group of four warps
-    } else if (warp == 9) {
+    } else if (warp > 8) {
         // -------------------------------------------------------------- MMAs
-        // One thread issues for both tiles, in turn: products of both issued
-        // side by side would share the tensor core and end together, and then
-        // both softmaxes would run, and wait, at the same time.
+        // An issuer for each tile, so that one's waits run beside the other's
+        // products, and in turn: products of both tiles issued side by side
+        // would share the tensor core and end together, and then both
+        // softmaxes would run, and wait, at the same time.
         at_fewer_registers();
-        {
-            const bool leader = at_elect();
-            constexpr int ab = DT == DT_BF16 ? 1 : 0;
-            constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
-            const uint64_t q0 = at_desc_k(sbase), k0 = at_desc_k(sbase + G::KV_OFF), v0 = at_desc_mn(sbase + G::KV_OFF);
-            uint32_t g = 0, np[2] = {0, 0}, nu[2] = {0, 0};
-            bool good = true;
-            auto wait_kv = [&](uint32_t i) {
-                good = good && at_wait(&kv_full[i % G::NST], (i / G::NST) & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
+        const int t = warp - 9;
+        const bool leader = at_elect();
+        constexpr int ab = DT == DT_BF16 ? 1 : 0;
+        constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
+        const uint32_t S = tmem + t * 128, O = tmem + 256 + t * 128;
+        const uint64_t Q = at_desc_k(sbase + t * G::TILE), k0 = at_desc_k(sbase + G::KV_OFF),
+                       v0 = at_desc_mn(sbase + G::KV_OFF);
+        uint32_t g = 0, np = 0, nu = 0, nt = 0;
+        bool good = true;
+        auto wait = [&](uint64_t *bar, uint32_t parity, unsigned code) {
+            good = good && at_wait(bar, parity, abort, a.err, code);
+        };
+        auto wait_kv = [&](uint32_t i) { wait(&kv_full[i % G::NST], (i / G::NST) & 1, DEVERR_TIMEOUT_W_FULL); };
+        auto scores = [&](uint32_t i) {
+            const uint64_t K = k0 + (i % G::NST) * (G::TILE / 16);
+            if (leader) {
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk)
+                    mma_f16_ss(S, Q + at_step_k(kk), K + at_step_k(kk), id_s, kk > 0);
+                mma_commit(&s_full[t]);
+                mma_commit(&kv_empty[i % G::NST]);
+            }
+        };
+        auto take_turn = [&](bool two) {
+            if (two) wait(&turn[t], (nt & 1) ^ (t == 0), DEVERR_TIMEOUT_ACC);
+        };
+        auto pass_turn = [&](bool two) {
+            if (!two) return;
+            if (leader) mbar_arrive(&turn[t ^ 1]);
+            ++nt;
+        };
+        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+            const AttnUnit w = attn_unit(a, u);
+            if (w.nk == 0) continue;
+            const bool two = w.tiles == 2;
+            if (t >= w.tiles) {  // no second tile: only pass the ring on
+                for (int j = 0; j < 2 * w.nk && good; ++j, ++g) {
+                    wait_kv(g);
+                    if (leader && good) mbar_arrive(&kv_empty[g % G::NST]);
+                }
+                continue;
+            }
+            wait(&q_full[t], nu & 1, DEVERR_TIMEOUT_AB_FULL);
+            wait_kv(g);
+            take_turn(two);
+            if (!good) break;
+            tc_fence_after();
+            scores(g);
+            pass_turn(two);
+            for (int j = 0; j < w.nk; ++j, g += 2) {
+                const int sv = (g + 1) % G::NST;
+                const bool more = j + 1 < w.nk;
+                const uint64_t V = v0 + sv * (G::TILE / 16);
+                if (leader && !more) mma_commit(&q_empty[t]);  // the last scores were issued
+                wait_kv(g + 1);
+                if (more) wait_kv(g + 2);
+                if (j == 0) wait(&o_empty[t], (nu & 1) ^ 1, DEVERR_TIMEOUT_ACC);
+                // O += P V, each half of P when it is there
+                wait(&p_full[2 * t], np & 1, DEVERR_TIMEOUT_ACC);
+                take_turn(two);
+                if (!good) break;
                 tc_fence_after();
-            };
-            auto scores = [&](int t, uint64_t K) {
-                const uint64_t Q = q0 + t * (G::TILE / 16);
                 if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < DP / 16; ++kk)
-                        mma_f16_ss(tmem + t * 128, Q + at_step_k(kk), K + at_step_k(kk), id_s, kk > 0);
-                    mma_commit(&s_full[t]);
+                    for (int kk = 0; kk < 4; ++kk)
+                        at_mma_ts(O, S + kk * 8, V + at_step_mn(kk), id_o, j > 0 || kk > 0);
                 }
-            };
-            // O_t += P_t V, each half of P when it is there
-            auto mix = [&](int t, uint64_t V, bool first) {
-                const uint32_t S = tmem + t * 128, O = tmem + 256 + t * 128;
+                wait(&p_full[2 * t + 1], np++ & 1, DEVERR_TIMEOUT_ACC);
+                if (!good) break;
+                tc_fence_after();
+                if (leader) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    good = good && at_wait(&p_full[2 * t + h], np[t] & 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                    if (!good) return;
-                    tc_fence_after();
-                    if (leader) {
-#pragma unroll
-                        for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
-                            at_mma_ts(O, S + kk * 8, V + at_step_mn(kk), id_o, !first || kk > 0);
-                    }
+                    for (int kk = 4; kk < AT_TILE / 16; ++kk) at_mma_ts(O, S + kk * 8, V + at_step_mn(kk), id_o, 1);
+                    mma_commit(more ? &kv_empty[sv] : &o_full[t]);
+                    if (!more) mma_commit(&kv_empty[sv]);
                 }
-                ++np[t];
-            };
-            for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
-                const AttnUnit w = attn_unit(a, u);
-                if (w.nk == 0) continue;
-                const bool two = w.tiles == 2;
-                wait_kv(g);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (t == 1 && !two) continue;
-                    good = good && at_wait(&q_full[t], nu[t] & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
-                    if (!good) break;
-                    tc_fence_after();
-                    scores(t, k0 + (g % G::NST) * (G::TILE / 16));
-                    if (leader && w.nk == 1) mma_commit(&q_empty[t]);
-                }
-                if (leader && good) mma_commit(&kv_empty[g % G::NST]);
-                for (int j = 0; j < w.nk && good; ++j, g += 2) {
-                    const int sv = (g + 1) % G::NST, sk = (g + 2) % G::NST;
-                    const bool more = j + 1 < w.nk;
-                    const uint64_t V = v0 + sv * (G::TILE / 16), K = k0 + sk * (G::TILE / 16);
-                    wait_kv(g + 1);
-                    if (more) wait_kv(g + 2);
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (t == 1 && !two) continue;
-                        if (j == 0)
-                            good = good && at_wait(&o_empty[t], (nu[t] & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_ACC);
-                        mix(t, V, j == 0);
-                        if (!good) break;
-                        if (more) {
-                            scores(t, K);
-                            if (leader && j + 2 == w.nk) mma_commit(&q_empty[t]);  // the last scores were issued
-                        } else {
-                            if (leader) mma_commit(&o_full[t]);
-                            ++nu[t];
-                        }
-                    }
-                    if (!good) break;
-                    if (leader) {
-                        mma_commit(&kv_empty[sv]);
-                        if (more) mma_commit(&kv_empty[sk]);
-                    }
-                }
+                if (more) scores(g + 2);
+                pass_turn(two);
             }
-            if (leader) mma_commit(mma_done);
+            ++nu;
         }
+        if (leader) mma_commit(&mma_done[t]);
     } else {
         // ------------------------------------------------- softmax and output
         at_more_registers();
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) at_finish(tmem, mma_done, a.err);
+    if (warp == 8) at_finish(tmem, mma_done, 2, a.err);
 }
 
 }  // namespace reels
