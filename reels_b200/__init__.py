@@ -3,10 +3,10 @@
 The compute lives in libreels_lowvram.so (include/reels_lowvram.h); this
 package is the Python-side mirror of the reference's layer API
 (:mod:`reels_b200.lowvram`), the attention between its projections
-(:mod:`reels_b200.attention`) and its data-parallel gradient all-reduce
+(:mod:`reels_b200.attn`) and its data-parallel gradient all-reduce
 (:mod:`reels_b200.distributed`).
 """
-from .attention import (  # noqa: F401
+from .attn import (  # noqa: F401
     AttentionFunction,
     RMSNormRopeFunction,
     RopeTable,

@@ -17,7 +17,16 @@ from typing import Optional, Sequence
 import torch
 
 from . import _native as nat
-from .lowvram import _check_numel, _dt, _flat, _ptr, _require_cuda, _stream
+from .lowvram import _check_numel, _dt, _ptr, _require_cuda
+
+# These calls are a few microseconds of GPU work on small clips, so the host's
+# way to the launch counts: the raw stream handle without a Stream object, and
+# no view or copy of what is contiguous already.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _stream(device) -> int:
+    return _raw_stream(device.index)
 
 
 # ------------------------------------------------------ norm and rotation
@@ -81,12 +90,15 @@ def _norm_rope_args(x, heads, weight, rope, tokens_per_sample, positions):
     _require_cuda(x, weight)
     C = x.shape[-1]
     heads = int(heads)
-    if heads <= 0 or C % heads:
+    if heads <= 0 or C == 0 or C % heads:
         raise ValueError("the features must be heads * head_dim")
-    xf = _flat(x, C)
-    M = xf.shape[0]
-    _check_numel(weight, C, "norm weight", x.device)
-    w = weight.contiguous().to(x.dtype) if weight is not None else None
+    xf = x if x.is_contiguous() else x.contiguous()
+    M = x.numel() // C
+    w = weight
+    if w is not None:
+        _check_numel(w, C, "norm weight", x.device)
+        if w.dtype != x.dtype or not w.is_contiguous():
+            w = w.contiguous().to(x.dtype)
     if tokens_per_sample is None:
         tps = x.shape[-2] if x.dim() >= 2 else 1
     else:
@@ -134,7 +146,7 @@ def rms_norm_rope(x: torch.Tensor, heads: int, weight: Optional[torch.Tensor] = 
     code = nat.lib().reels_rms_norm_rope(xf.data_ptr(), M, heads, D, _ptr(w), r, tps, float(epsilon), _dt(x.dtype),
                                          out.data_ptr(), _stream(x.device))
     nat.check("rms_norm_rope", code)
-    return out.view(x.shape)
+    return out
 
 
 def rms_norm_rope_backward(x: torch.Tensor, dout: torch.Tensor, heads: int, weight: Optional[torch.Tensor] = None,
@@ -146,12 +158,12 @@ def rms_norm_rope_backward(x: torch.Tensor, dout: torch.Tensor, heads: int, weig
     if dout.shape != x.shape or dout.dtype != x.dtype or dout.device != x.device:
         raise ValueError("dout must have the shape, dtype and device of x")
     xf, M, heads, D, w, r, tps, pos = _norm_rope_args(x, heads, weight, rope, tokens_per_sample, positions)
-    df = _flat(dout, xf.shape[1])
+    df = dout if dout.is_contiguous() else dout.contiguous()
     dx = torch.empty_like(xf)
     code = nat.lib().reels_rms_norm_rope_backward(xf.data_ptr(), df.data_ptr(), M, heads, D, _ptr(w), r, tps,
                                                   float(epsilon), _dt(x.dtype), dx.data_ptr(), _stream(x.device))
     nat.check("rms_norm_rope_backward", code)
-    return dx.view(x.shape)
+    return dx
 
 
 class RMSNormRopeFunction(torch.autograd.Function):
@@ -184,41 +196,65 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _attention_args(q, k, v, scale, kv_lengths):
-    _require_cuda(q, k, v, kv_lengths)
+_I3 = ctypes.c_int64 * 3
+# Checked sizes, strides and types -> (head_dim ** -0.5, the C shape, scratch
+# bytes forward and backward, whether the strides can be read): the host side
+# of a call is mostly this, and a program repeats few of them.
+_SHAPES = {}
+
+
+def _attention_shape(q, k, v):
+    key = (q.shape, k.shape, v.shape, q.stride(), k.stride(), v.stride(), q.dtype, k.dtype, v.dtype)
+    hit = _SHAPES.get(key)
+    if hit is not None:
+        return hit
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("q, k and v must be (batch, tokens, heads, head_dim)")
     B, Sq, H, D = q.shape
     if k.shape != v.shape:
         raise ValueError("k and v must have the same shape")
-    if k.shape[0] != B or k.shape[3] != D:
+    KB, Sk, HK, KD = k.shape
+    if KB != B or KD != D:
         raise ValueError("q, k and v must agree in batch and head_dim")
-    HK = k.shape[2]
     if HK == 0 or H % HK:
         raise ValueError("heads must be a multiple of kv_heads")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("q, k and v must have the same dtype")
-    if k.device != q.device or v.device != q.device:
+    dt = _dt(q.dtype)
+    shape = nat.AttnShape(B, H, HK, Sq, Sk, D, _I3(*q.stride()[:3]), _I3(*k.stride()[:3]), _I3(*v.stride()[:3]))
+    ws = [nat.lib().reels_attention_workspace_bytes(ctypes.byref(shape), dt, p)
+          for p in (nat.PASS_FORWARD, nat.PASS_BACKWARD)]
+    hit = (D ** -0.5 if D else 1.0, shape, *ws, all(_readable(t) is t for t in (q, k, v)))
+    if len(_SHAPES) >= 4096:
+        _SHAPES.clear()
+    _SHAPES[key] = hit
+    return hit
+
+
+def _attention_args(q, k, v, scale, kv_lengths):
+    _require_cuda(q, k, v, kv_lengths)
+    device = q.device
+    if k.device != device or v.device != device:
         raise ValueError("q, k and v must be on the same device")
+    known = _attention_shape(q, k, v)
+    if not known[4]:
+        q, k, v = _readable(q), _readable(k), _readable(v)
+        known = _attention_shape(q, k, v)
     if kv_lengths is not None:
-        if kv_lengths.dtype not in (torch.int32, torch.int64) or kv_lengths.shape != (B,):
+        if kv_lengths.dtype not in (torch.int32, torch.int64) or kv_lengths.shape != (q.shape[0],):
             raise ValueError("kv_lengths must be one integer per sample")
-        if kv_lengths.device != q.device:
-            raise ValueError(f"kv_lengths is on {kv_lengths.device}, the input on {q.device}")
-        kv_lengths = kv_lengths.clamp(0, k.shape[1]) if kv_lengths.dtype == torch.int64 else kv_lengths
-        kv_lengths = kv_lengths.to(torch.int32).contiguous()
-    scale = D ** -0.5 if scale is None else float(scale)
-    q, k, v = _readable(q), _readable(k), _readable(v)
-    i3 = ctypes.c_int64 * 3
-    shape = nat.AttnShape(B, H, HK, Sq, k.shape[1], D, i3(*q.stride()[:3]), i3(*k.stride()[:3]), i3(*v.stride()[:3]))
-    return q, k, v, kv_lengths, scale, shape
+        if kv_lengths.device != device:
+            raise ValueError(f"kv_lengths is on {kv_lengths.device}, the input on {device}")
+        if kv_lengths.dtype == torch.int64:
+            kv_lengths = kv_lengths.clamp(0, k.shape[1]).to(torch.int32)
+        kv_lengths = kv_lengths.contiguous()
+    return q, k, v, kv_lengths, known[0] if scale is None else float(scale), known
 
 
-def _attention_workspace(device, shape, dt, which):
+def _scratch(nbytes, device):
     """Scratch of one call, from the caching allocator: calls on different
     streams and captured graphs each have their own."""
-    n = nat.lib().reels_attention_workspace_bytes(ctypes.byref(shape), dt, which)
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional[float] = None,
@@ -234,14 +270,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     Returns out (batch, tokens, heads, head_dim), contiguous, and with
     ``return_lse`` also the fp32 log-sum-exp (batch, heads, tokens) that
     :func:`attention_backward` needs."""
-    q, k, v, lengths, scale, shape = _attention_args(q, k, v, scale, kv_lengths)
+    q, k, v, lengths, scale, known = _attention_args(q, k, v, scale, kv_lengths)
     B, Sq, H, D = q.shape
-    dt = _dt(q.dtype)
-    out = torch.empty((B, Sq, H, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
-    ws = _attention_workspace(q.device, shape, dt, nat.PASS_FORWARD)
-    code = nat.lib().reels_attention_forward(ctypes.byref(shape), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                             _ptr(lengths), scale, dt, out.data_ptr(), lse.data_ptr(), _ptr(ws),
+    out = q.new_empty((B, Sq, H, D))
+    lse = q.new_empty((B, H, Sq), dtype=torch.float32)
+    ws = _scratch(known[2], q.device)
+    code = nat.lib().reels_attention_forward(ctypes.byref(known[1]), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                             _ptr(lengths), scale, _dt(q.dtype), out.data_ptr(), lse.data_ptr(), _ptr(ws),
                                              0 if ws is None else ws.numel(), _stream(q.device))
     nat.check("attention", code)
     return (out, lse) if return_lse else out
@@ -252,24 +287,22 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     """Pullback of :func:`attention`: ``(dq, dk, dv)``, contiguous, with the
     probabilities recomputed from q, k and ``lse``.  ``out`` and ``lse`` are
     the forward's.  Repeated calls give the same bits."""
+    _require_cuda(dout, out, lse)
+    q, k, v, lengths, scale, known = _attention_args(q, k, v, scale, kv_lengths)
     if out.shape != q.shape or dout.shape != q.shape:
         raise ValueError("out and dout must have the shape of q")
     if out.dtype != q.dtype or dout.dtype != q.dtype:
         raise ValueError("out and dout must have the dtype of q")
-    _require_cuda(dout, out, lse)
     if dout.device != q.device or out.device != q.device or lse.device != q.device:
         raise ValueError("dout, out and lse must be on q's device")
     if lse.dtype != torch.float32 or tuple(lse.shape) != (q.shape[0], q.shape[2], q.shape[1]):
         raise ValueError("lse must be the forward's fp32 (batch, heads, tokens)")
-    q, k, v, lengths, scale, shape = _attention_args(q, k, v, scale, kv_lengths)
     out, dout, lse = out.contiguous(), dout.contiguous(), lse.contiguous()
-    dt = _dt(q.dtype)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
-    ws = _attention_workspace(q.device, shape, dt, nat.PASS_BACKWARD)
-    code = nat.lib().reels_attention_backward(ctypes.byref(shape), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                                              out.data_ptr(), lse.data_ptr(), dout.data_ptr(), _ptr(lengths), scale, dt,
-                                              dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws),
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape)
+    ws = _scratch(known[3], q.device)
+    code = nat.lib().reels_attention_backward(ctypes.byref(known[1]), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                              out.data_ptr(), lse.data_ptr(), dout.data_ptr(), _ptr(lengths), scale,
+                                              _dt(q.dtype), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws),
                                               0 if ws is None else ws.numel(), _stream(q.device))
     nat.check("attention_backward", code)
     return dq, dk, dv

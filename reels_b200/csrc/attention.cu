@@ -178,7 +178,7 @@ int check_shape(const reels_attn_shape *s, int dt) {
         return host_fail("head_dim must be between 1 and " + std::to_string(AT_MAX_D));
     const int64_t lim = INT32_MAX - 256;
     if (s->batch > lim || s->heads > lim || s->q_tokens > lim || s->k_tokens > lim ||
-        s->batch * s->heads > lim || ceil_div(std::max(s->q_tokens, s->k_tokens), AS_T) > lim / std::max<int64_t>(1, s->batch * s->heads))
+        s->batch * s->heads > lim || ceil_div(std::max(s->q_tokens, s->k_tokens), AS_T) > lim / 2 / std::max<int64_t>(1, s->batch * s->heads))
         return host_fail("attention shape too large");
     for (int i = 0; i < 3; ++i)
         if (s->q_stride[i] < 0 || s->k_stride[i] < 0 || s->v_stride[i] < 0) return host_fail("negative stride");
@@ -195,11 +195,11 @@ AttnPlan plan_attention(const reels_attn_shape &s, int dt, const void *q, const 
            tma_strides(s.k_stride, nk) && tma_strides(s.v_stride, nk) && aligned16(q) && aligned16(k) && aligned16(v);
     p.Sqp = (int)(ceil_div(s.q_tokens, AT_TILE) * AT_TILE);
     // Forward: few rows leave SMs idle, so the keys are split over them and
-    // joined; a split keeps at least four tiles of keys.
+    // joined; a split keeps at least four tiles of keys (two on the CUDA cores).
     const int tile = p.tc ? AT_TILE : AS_T;
     const int64_t rows = ceil_div(s.q_tokens, p.tc ? 2 * AT_TILE : AS_T) * s.batch * s.heads;
     const int64_t tiles = std::max<int64_t>(1, ceil_div(s.k_tokens, tile));
-    int64_t want = rows > 0 ? std::min<int64_t>((p.tc ? 1 : 4) * kPlanSms / std::max<int64_t>(rows, 1), tiles / 4) : 1;
+    int64_t want = rows > 0 ? std::min<int64_t>((p.tc ? 1 : 4) * kPlanSms / rows, tiles / (p.tc ? 4 : 2)) : 1;
     want = std::max<int64_t>(1, std::min<int64_t>(want, 1024));
     const int64_t per = ceil_div(tiles, want);
     p.splits = (int)ceil_div(tiles, per);
@@ -290,8 +290,7 @@ cudaError_t big_smem(K kern, int bytes) {
 template <int DT, int DP>
 cudaError_t simt_attrs() {
     cudaError_t e = big_smem(attn_simt_fwd_kernel<DT, DP>, as_smem_bytes(DP, 3));
-    if (e == cudaSuccess) e = big_smem(attn_simt_dkdv_kernel<DT, DP>, as_smem_bytes(DP, 4));
-    if (e == cudaSuccess) e = big_smem(attn_simt_dq_kernel<DT, DP>, as_smem_bytes(DP, 4));
+    if (e == cudaSuccess) e = big_smem(attn_simt_bwd_kernel<DT, DP>, as_smem_bytes(DP, 4));
     return e;
 }
 template <int DT, int DP>
@@ -492,28 +491,31 @@ int reels_attention_backward(const reels_attn_shape *shape, const void *q, const
         if (e != cudaSuccess) return host_fail_dev(std::string("cudaMemsetAsync: ") + cudaGetErrorString(e));
     }
     const int64_t rows = s.batch * s.heads * plan.Sqp, keys = s.batch * s.kv_heads * s.k_tokens;
-    with_dtype(act_dtype, [&](auto t) {
-        e = host_launch_pdl(attn_stat_kernel<decltype(t)::value>,
-                            dim3((unsigned)std::min<int64_t>(ceil_div(rows, 8), 8ll * call.sms)), dim3(256), 0, st, a,
-                            stat_l, stat_d, range,
-                            plan.tc ? AtRange<decltype(t)::value>::BWD_SHIFT : 0.0f);
-    });
+    if (!plan.tc)
+        with_dtype(act_dtype, [&](auto t) {
+            e = host_launch_pdl(attn_stat_kernel<decltype(t)::value>,
+                                dim3((unsigned)std::min<int64_t>(ceil_div(rows, 8), 8ll * call.sms)), dim3(256), 0, st,
+                                a, stat_l, stat_d);
+        });
+    else
+        with_tc_type(act_dtype, s.head_dim, [&](auto t, auto d) {
+            constexpr int DT = decltype(t)::value, G = decltype(d)::value / 8;
+            const int64_t blocks = ceil_div(s.batch * s.q_tokens * s.heads, 256 / G * 4);
+            e = host_launch_pdl(attn_stat_vec_kernel<DT, G>, dim3((unsigned)std::min<int64_t>(blocks, 8ll * call.sms)),
+                                dim3(256), 0, st, a, stat_l, stat_d, range, AtRange<DT>::BWD_SHIFT);
+        });
     RA_LAUNCH(e);
     if (!plan.tc) {
         with_dtype(act_dtype, [&](auto t) {
             with_simt_dim(s.head_dim, [&](auto d) {
                 constexpr int DT = decltype(t)::value, DP = decltype(d)::value;
-                e = host_launch_pdl(attn_simt_dkdv_kernel<DT, DP>,
-                                    dim3((unsigned)(ceil_div(s.k_tokens, AS_T) * s.batch * s.kv_heads)),
-                                    dim3(AS_THREADS), as_smem_bytes(DP, 4), st, a);
-                if (e == cudaSuccess)
-                    e = host_launch_pdl(attn_simt_dq_kernel<DT, DP>,
-                                        dim3((unsigned)(ceil_div(s.q_tokens, AS_T) * s.batch * s.heads)),
-                                        dim3(AS_THREADS), as_smem_bytes(DP, 4), st, a);
+                const int64_t blocks = ceil_div(s.k_tokens, AS_T) * s.batch * s.kv_heads +
+                                       ceil_div(s.q_tokens, AS_T) * s.batch * s.heads;
+                e = host_launch_pdl(attn_simt_bwd_kernel<DT, DP>, dim3((unsigned)blocks), dim3(AS_THREADS),
+                                    as_smem_bytes(DP, 4), st, a);
             });
         });
         RA_LAUNCH(e);
-        host_count_launch();
         return host_ok(REELS_PATH_CUDACORE);
     }
     if (range) {

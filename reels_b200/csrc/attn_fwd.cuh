@@ -281,17 +281,20 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
                     for (int i = 0; i < AT_TILE; ++i)
                         if (i >= rows) s[i] = 0xff800000u;  // -inf
                 }
-                float mx[4];
+                float mx[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s[i]);
+                for (int i = 0; i < 8; ++i)
+                    mx[i] = at_max3(__uint_as_float(s[i]), __uint_as_float(s[i + 8]), __uint_as_float(s[i + 16]));
 #pragma unroll
-                for (int i = 4; i < AT_TILE - 4; i += 8)
+                for (int i = 24; i < 120; i += 16)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        mx[e] = at_max3(mx[e], __uint_as_float(s[i + e]), __uint_as_float(s[i + 4 + e]));
+                    for (int e = 0; e < 8; ++e)
+                        mx[e] = at_max3(mx[e], __uint_as_float(s[i + e]), __uint_as_float(s[i + 8 + e]));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[AT_TILE - 4 + e]));
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[120 + e]));
+                mx[0] = at_max3(mx[0], mx[1], mx[2]);
+                mx[3] = at_max3(mx[3], mx[4], mx[5]);
+                float top = fmaxf(at_max3(mx[0], mx[3], mx[6]), mx[7]) * c;
                 top = (top == -CUDART_INF_F ? 0.0f : top) - AtRange<DT>::FWD_SHIFT;
                 if (j == 0) m = top;
                 else if (__any_sync(0xffffffffu, top - m > 8.0f)) {

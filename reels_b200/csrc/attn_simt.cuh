@@ -9,8 +9,10 @@
 //   dV = P' dO,  dQ = scale dS k,  dK = scale dS' q
 // A row without keys has O = 0, L = -inf and no part in any gradient.
 //
-// 32 x 32 tiles of S in registers (2 x 4 a thread, 128 threads), operands in
-// shared memory as fp32; every sum is fp32 and in a fixed order.
+// 32 x 32 tiles of S in registers (2 x 2 a thread, 256 threads), operands in
+// shared memory as fp32; every sum is fp32 and in a fixed order.  Small fp32
+// clips are the use: a few tiles a block, so a block's latency counts, and dQ
+// runs beside dK and dV in one launch.
 #pragma once
 #include <math_constants.h>
 
@@ -20,7 +22,7 @@ namespace reels {
 
 constexpr int AT_MAX_D = 256;  // head size
 constexpr int AS_T = 32;       // tile of the CUDA-core kernels
-constexpr int AS_THREADS = 128;
+constexpr int AS_THREADS = 256;
 
 struct AttnArgs {
     const void *q, *k, *v;                   // [batch][token][head][D] by strides, D contiguous
@@ -50,45 +52,64 @@ __device__ __forceinline__ int attn_keys(const AttnArgs &a, int b) {
     return n < 0 ? 0 : (n < a.Sk ? n : a.Sk);
 }
 
-// 32 rows of D elements into dst[32][DP + 4], rows from `n` on and features from D on as zeros.
+// 32 rows of D elements into dst[32][DP + 4], rows from `n` on and features
+// from D on as zeros.  fp32 rows that allow it in 16-byte pieces.
 template <int DT, int DP>
 __device__ __forceinline__ void as_load(float *dst, const void *src, long long at, long long pitch, int n, int D) {
+    if (DT == DT_F32 && ((reinterpret_cast<uintptr_t>(src) & 15) | ((at | pitch | D) & 3)) == 0) {
+        const float *p = reinterpret_cast<const float *>(src) + at;
+        float4 v[DP / 32];
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+            const int x = threadIdx.x + i * AS_THREADS, r = x / (DP / 4), d = x % (DP / 4) * 4;
+            v[i] = (r < n && d < D) ? __ldcg(reinterpret_cast<const float4 *>(p + r * pitch + d))
+                                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+            const int x = threadIdx.x + i * AS_THREADS, r = x / (DP / 4), d = x % (DP / 4) * 4;
+            *reinterpret_cast<float4 *>(dst + r * (DP + 4) + d) = v[i];
+        }
+        return;
+    }
+#pragma unroll 8
     for (int i = threadIdx.x; i < AS_T * DP; i += AS_THREADS) {
         const int r = i / DP, d = i - r * DP;
         dst[r * (DP + 4) + d] = (r < n && d < D) ? load_act(src, at + r * pitch + d, DT) : 0.0f;
     }
 }
-// acc[i][j] = A[2 ty + i] . B[tx + 8 j]
+// acc[i][j] = A[2 ty + i] . B[tx + 16 j]
 template <int DP>
-__device__ __forceinline__ void as_dot(const float *A, const float *B, int ty, int tx, float (&acc)[2][4]) {
+__device__ __forceinline__ void as_dot(const float *A, const float *B, int ty, int tx, float (&acc)[2][2]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-#pragma unroll 4
+        for (int j = 0; j < 2; ++j) acc[i][j] = 0.0f;
+#pragma unroll 8
     for (int d = 0; d < DP; d += 4) {
-        float4 x[2], y[4];
+        float4 x[2], y[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) x[i] = *reinterpret_cast<const float4 *>(A + (2 * ty + i) * (DP + 4) + d);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4 *>(B + (tx + 8 * j) * (DP + 4) + d);
+        for (int i = 0; i < 2; ++i) {
+            x[i] = *reinterpret_cast<const float4 *>(A + (2 * ty + i) * (DP + 4) + d);
+            y[i] = *reinterpret_cast<const float4 *>(B + (tx + 16 * i) * (DP + 4) + d);
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 2; ++j)
                 acc[i][j] += x[i].x * y[j].x + x[i].y * y[j].y + x[i].z * y[j].z + x[i].w * y[j].w;
     }
 }
-// acc[i][c][.] += sum_n W(2 ty + i, n) B[n][4 tx + 32 c ..]; W(r, n) = w[r * rs + n * ns]
+// acc[i][c][.] += sum_n W(2 ty + i, n) B[n][4 tx + 64 c ..]; W(r, n) = w[r * rs + n * ns]
 template <int DP>
 __device__ __forceinline__ void as_mix(const float *w, int rs, int ns, const float *B, int ty, int tx,
-                                       float (&acc)[2][DP / 32][4]) {
-#pragma unroll 2
+                                       float (&acc)[2][DP / 64][4]) {
+#pragma unroll 4
     for (int n = 0; n < AS_T; ++n) {
         const float w0 = w[(2 * ty) * rs + n * ns], w1 = w[(2 * ty + 1) * rs + n * ns];
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-            const float4 b = *reinterpret_cast<const float4 *>(B + n * (DP + 4) + 4 * tx + 32 * c);
+        for (int c = 0; c < DP / 64; ++c) {
+            const float4 b = *reinterpret_cast<const float4 *>(B + n * (DP + 4) + 4 * tx + 64 * c);
             acc[0][c][0] += w0 * b.x, acc[0][c][1] += w0 * b.y, acc[0][c][2] += w0 * b.z, acc[0][c][3] += w0 * b.w;
             acc[1][c][0] += w1 * b.x, acc[1][c][1] += w1 * b.y, acc[1][c][2] += w1 * b.z, acc[1][c][3] += w1 * b.w;
         }
@@ -104,46 +125,46 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(const AttnArg
     extern __shared__ float sm[];
     float *Q = sm, *K = Q + AS_T * (DP + 4), *V = K + AS_T * (DP + 4), *P = V + AS_T * (DP + 4);
     griddep_wait();
-    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int tiles = (a.Sq + AS_T - 1) / AS_T, bh = (int)(blockIdx.x / tiles);
     const int q0 = (int)(blockIdx.x % tiles) * AS_T, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.HK);
     const int len = attn_keys(a, b);
     const int k_begin = min(len, (int)blockIdx.y * a.split_keys), k_end = min(len, k_begin + a.split_keys);
     as_load<DT, DP>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
-    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.0f, 0.0f}, o[2][DP / 32][4] = {};
+    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.0f, 0.0f}, o[2][DP / 64][4] = {};
     for (int k0 = k_begin; k0 < k_end; k0 += AS_T) {
         __syncthreads();
         as_load<DT, DP>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], k_end - k0, a.D);
         as_load<DT, DP>(V, a.v, b * a.vs[0] + k0 * a.vs[1] + hk * a.vs[2], a.vs[1], k_end - k0, a.D);
         __syncthreads();
-        float s[2][4];
+        float s[2][2];
         as_dot<DP>(Q, K, ty, tx, s);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float mx = -CUDART_INF_F;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[i][j] = k0 + tx + 8 * j < k_end ? s[i][j] * a.scale : -CUDART_INF_F;
+            for (int j = 0; j < 2; ++j) {
+                s[i][j] = k0 + tx + 16 * j < k_end ? s[i][j] * a.scale : -CUDART_INF_F;
                 mx = fmaxf(mx, s[i][j]);
             }
 #pragma unroll
-            for (int w = 1; w < 8; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+            for (int w = 1; w < 16; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
             mx = fmaxf(m[i], mx);
             const float ref = mx == -CUDART_INF_F ? 0.0f : mx;
             const float keep = expf(m[i] - ref);
             float sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 const float p = expf(s[i][j] - ref);
-                P[(2 * ty + i) * (AS_T + 1) + tx + 8 * j] = p;
+                P[(2 * ty + i) * (AS_T + 1) + tx + 16 * j] = p;
                 sum += p;
             }
 #pragma unroll
-            for (int w = 1; w < 8; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+            for (int w = 1; w < 16; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
             l[i] = l[i] * keep + sum;
             m[i] = mx;
 #pragma unroll
-            for (int c = 0; c < DP / 32; ++c)
+            for (int c = 0; c < DP / 64; ++c)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[i][c][e] *= keep;
         }
@@ -159,10 +180,10 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(const AttnArg
         const long long at = ((long long)blockIdx.y * a.B + b) * a.H + h;
         if (tx == 0) (a.splits > 1 ? a.part_lse : a.lse)[at * a.Sq + q] = lse;
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c)
+        for (int c = 0; c < DP / 64; ++c)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int d = 4 * tx + 32 * c + e;
+                const int d = 4 * tx + 64 * c + e;
                 if (d >= a.D) continue;
                 const float v = o[i][c][e] * inv;
                 if (a.splits > 1) a.part_o[(at * a.Sq + q) * a.D + d] = v;
@@ -205,56 +226,105 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
 }
 
 // Row statistics of the gradient, as the terms that are added: -L in log2
-// units plus `shift` (fp16, see AtRange) and -delta of every query row, padded
-// to Sqp rows a head.  Rows without keys and padding get -inf, so that their
-// probabilities come out as exp2(-inf) = 0.  One warp a row.
+// units and -delta of every query row, padded to Sqp rows a head.  Rows
+// without keys and padding get -inf, so that their probabilities come out as
+// exp2(-inf) = 0.  One warp a row.
 template <int DT>
-__global__ void __launch_bounds__(256) attn_stat_kernel(const AttnArgs a, float *stat_l, float *stat_d, unsigned *range, float shift) {
+__global__ void __launch_bounds__(256) attn_stat_kernel(const AttnArgs a, float *stat_l, float *stat_d) {
     griddep_wait();
     const int lane = threadIdx.x & 31;
     const long long rows = (long long)a.B * a.H * a.Sqp;
-    float top = 0.0f;  // fp16: largest |dO row|^2
     for (long long row = blockIdx.x * 8ll + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8ll) {
         const int q = (int)(row % a.Sqp), h = (int)(row / a.Sqp % a.H), b = (int)(row / a.Sqp / a.H);
         float2 st = make_float2(-CUDART_INF_F, 0.0f);
         if (q < a.Sq) {
             const long long at = (((long long)b * a.Sq + q) * a.H + h) * a.D;
-            float delta = 0.0f, n2 = 0.0f;
-            if (DT != DT_F32 && (a.D & 7) == 0) {
-                for (int d = 8 * lane; d < a.D; d += 256) {
-                    const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(
-                        reinterpret_cast<const typename Elem<DT>::T *>(a.dout) + at + d));
-                    const uint4 y = __ldcg(reinterpret_cast<const uint4 *>(
-                        reinterpret_cast<const typename Elem<DT>::T *>(a.out) + at + d));
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float g = load_act(&x, j, DT);
-                        delta += g * load_act(&y, j, DT);
-                        n2 += g * g;
-                    }
-                }
-            } else {
-                for (int d = lane; d < a.D; d += 32) {
-                    const float g = load_act(a.dout, at + d, DT);
-                    delta += g * load_act(a.out, at + d, DT);
-                    n2 += g * g;
-                }
+            float delta = 0.0f;
+            for (int d = lane; d < a.D; d += 32) {
+                const float g = load_act(a.dout, at + d, DT);
+                delta += g * load_act(a.out, at + d, DT);
             }
 #pragma unroll
-            for (int w = 16; w > 0; w >>= 1) {
-                delta += __shfl_xor_sync(0xffffffffu, delta, w);
-                n2 += __shfl_xor_sync(0xffffffffu, n2, w);
-            }
+            for (int w = 16; w > 0; w >>= 1) delta += __shfl_xor_sync(0xffffffffu, delta, w);
             const float lse = __ldcg(a.lse + ((long long)b * a.H + h) * a.Sq + q);
-            if (lse != -CUDART_INF_F) st = make_float2(shift - lse * CUDART_L2E_F, -delta);
-            top = fmaxf(top, n2);
+            if (lse != -CUDART_INF_F) st = make_float2(-lse * CUDART_L2E_F, -delta);
         }
         if (lane == 0) {
             stat_l[row] = st.x;
             stat_d[row] = st.y;
         }
     }
-    if (range && lane == 0) atomicMax(range, __float_as_uint(sqrtf(top)));
+}
+
+// The same for 16-bit rows of D = 8 n features up to 8 G, as the tensor-core
+// kernels take them: G lanes a row with 16 bytes each, four rows in flight,
+// rows in memory order (the heads of a token side by side).  `shift` is added
+// to -L (fp16, see AtRange); `range` receives the largest |dO row| (fp16; a
+// maximum does not depend on the order of its atomics).  Bound: HBM, out and
+// dO once.
+template <int DT, int G>
+__global__ void __launch_bounds__(256) attn_stat_vec_kernel(const AttnArgs a, float *stat_l, float *stat_d,
+                                                            unsigned *range, float shift) {
+    griddep_wait();
+    using T = typename Elem<DT>::T;
+    constexpr int R = 4;
+    const int sub = threadIdx.x % G;
+    const long long rows = (long long)a.B * a.Sq * a.H, step = (long long)gridDim.x * (256 / G) * R;
+    float top = 0.0f;  // largest |dO row|^2
+    for (long long r0 = ((long long)blockIdx.x * (256 / G) + threadIdx.x / G) * R, any = (long long)blockIdx.x * (256 / G) * R;
+         any < rows; r0 += step, any += step) {  // (a block stays together for its shuffles)
+        uint4 x[R], y[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            x[i] = y[i] = make_uint4(0, 0, 0, 0);
+            if (r0 + i < rows && 8 * sub < a.D) {
+                x[i] = __ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.dout) + (r0 + i) * a.D) + sub);
+                y[i] = __ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.out) + (r0 + i) * a.D) + sub);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            float delta = 0.0f, n2 = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float g = load_act(&x[i], j, DT);
+                delta += g * load_act(&y[i], j, DT);
+                if (DT == DT_F16) n2 += g * g;
+            }
+#pragma unroll
+            for (int w = G / 2; w > 0; w >>= 1) {
+                delta += __shfl_xor_sync(0xffffffffu, delta, w);
+                if (DT == DT_F16) n2 += __shfl_xor_sync(0xffffffffu, n2, w);
+            }
+            top = fmaxf(top, n2);
+            if (sub == 0 && r0 + i < rows) {
+                int b, q, h;
+                if (rows <= 0x7fffffff) {  // (64-bit divisions would cost more than the rows)
+                    const uint32_t r = (uint32_t)(r0 + i), tok = r / (uint32_t)a.H;
+                    h = (int)(r - tok * a.H), b = (int)(tok / (uint32_t)a.Sq), q = (int)(tok - b * (uint32_t)a.Sq);
+                } else {
+                    const long long tok = (r0 + i) / a.H;
+                    h = (int)((r0 + i) - tok * a.H), b = (int)(tok / a.Sq), q = (int)(tok - (long long)b * a.Sq);
+                }
+                const long long bh = (long long)b * a.H + h;
+                const float lse = __ldcg(a.lse + bh * a.Sq + q);
+                const bool dead = lse == -CUDART_INF_F;
+                stat_l[bh * a.Sqp + q] = dead ? -CUDART_INF_F : shift - lse * CUDART_L2E_F;
+                stat_d[bh * a.Sqp + q] = dead ? 0.0f : -delta;
+            }
+        }
+    }
+    const int pad = a.Sqp - a.Sq;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < (long long)a.B * a.H * pad; i += gridDim.x * 256ll) {
+        const long long at = i / pad * a.Sqp + a.Sq + i % pad;
+        stat_l[at] = -CUDART_INF_F;
+        stat_d[at] = 0.0f;
+    }
+    if (DT == DT_F16) {
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        if ((threadIdx.x & 31) == 0) atomicMax(range, __float_as_uint(sqrtf(top)));
+    }
 }
 
 // fp16: the largest |v row|, so that the gradients' operands can be held in
@@ -286,37 +356,35 @@ template <int DP>
 __device__ __forceinline__ void as_grad_tile(const AttnArgs &a, const float *Q, const float *K, const float *V,
                                              const float *G, float *P, float *S, long long stat_at, int k0, int len,
                                              int ty, int tx) {
-    float s[2][4], dp[2][4];
+    float s[2][2], dp[2][2];
     as_dot<DP>(Q, K, ty, tx, s);
     as_dot<DP>(G, V, ty, tx, dp);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const float2 st = make_float2(__ldcg(a.stat_l + stat_at + 2 * ty + i), __ldcg(a.stat_d + stat_at + 2 * ty + i));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bool in = k0 + tx + 8 * j < len && st.x != -CUDART_INF_F;
+        for (int j = 0; j < 2; ++j) {
+            const bool in = k0 + tx + 16 * j < len && st.x != -CUDART_INF_F;
             const float p = in ? exp2f(s[i][j] * a.scale * CUDART_L2E_F + st.x) : 0.0f;
-            const int at = (2 * ty + i) * (AS_T + 1) + tx + 8 * j;
+            const int at = (2 * ty + i) * (AS_T + 1) + tx + 16 * j;
             P[at] = p;
             S[at] = in ? p * (dp[i][j] + st.y) : 0.0f;
         }
     }
 }
 
-// dK and dV of a tile of keys: all query tiles of all heads that share it.  grid: key tiles * B * HK
+// dK and dV of a tile of keys: all query tiles of all heads that share it.
 template <int DT, int DP>
-__global__ void __launch_bounds__(AS_THREADS) attn_simt_dkdv_kernel(const AttnArgs a) {
-    extern __shared__ float sm[];
+__device__ __forceinline__ void as_dkdv(const AttnArgs &a, float *sm, unsigned block) {
     constexpr int T = AS_T * (DP + 4);
     float *K = sm, *V = K + T, *Q = V + T, *G = Q + T, *P = G + T, *S = P + AS_T * (AS_T + 1);
-    griddep_wait();
-    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
-    const int tiles = (a.Sk + AS_T - 1) / AS_T, bh = (int)(blockIdx.x / tiles);
-    const int k0 = (int)(blockIdx.x % tiles) * AS_T, b = bh / a.HK, hk = bh % a.HK, group = a.H / a.HK;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int tiles = (a.Sk + AS_T - 1) / AS_T, bh = (int)(block / tiles);
+    const int k0 = (int)(block % tiles) * AS_T, b = bh / a.HK, hk = bh % a.HK, group = a.H / a.HK;
     const int len = attn_keys(a, b);
     as_load<DT, DP>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], len - k0, a.D);
     as_load<DT, DP>(V, a.v, b * a.vs[0] + k0 * a.vs[1] + hk * a.vs[2], a.vs[1], len - k0, a.D);
-    float dk[2][DP / 32][4] = {}, dv[2][DP / 32][4] = {};
+    float dk[2][DP / 64][4] = {}, dv[2][DP / 64][4] = {};
     for (int h = hk * group; h < (hk + 1) * group && k0 < len; ++h)
         for (int q0 = 0; q0 < a.Sq; q0 += AS_T) {
             __syncthreads();
@@ -334,10 +402,10 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dkdv_kernel(const AttnAr
         const int t = k0 + 2 * ty + i;
         if (t >= a.Sk) continue;
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c)
+        for (int c = 0; c < DP / 64; ++c)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int d = 4 * tx + 32 * c + e;
+                const int d = 4 * tx + 64 * c + e;
                 if (d >= a.D) continue;
                 const long long at = (((long long)b * a.Sk + t) * a.HK + hk) * a.D + d;
                 store_act(a.dk, at, DT, t < len ? dk[i][c][e] * a.scale : 0.0f);
@@ -346,20 +414,18 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dkdv_kernel(const AttnAr
     }
 }
 
-// dQ of a tile of queries.  grid: query tiles * B * H
+// dQ of a tile of queries.
 template <int DT, int DP>
-__global__ void __launch_bounds__(AS_THREADS) attn_simt_dq_kernel(const AttnArgs a) {
-    extern __shared__ float sm[];
+__device__ __forceinline__ void as_dq(const AttnArgs &a, float *sm, unsigned block) {
     constexpr int T = AS_T * (DP + 4);
     float *K = sm, *V = K + T, *Q = V + T, *G = Q + T, *P = G + T, *S = P + AS_T * (AS_T + 1);
-    griddep_wait();
-    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
-    const int tiles = (a.Sq + AS_T - 1) / AS_T, bh = (int)(blockIdx.x / tiles);
-    const int q0 = (int)(blockIdx.x % tiles) * AS_T, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.HK);
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int tiles = (a.Sq + AS_T - 1) / AS_T, bh = (int)(block / tiles);
+    const int q0 = (int)(block % tiles) * AS_T, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.HK);
     const int len = attn_keys(a, b);
     as_load<DT, DP>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
     as_load<DT, DP>(G, a.dout, (((long long)b * a.Sq + q0) * a.H + h) * a.D, (long long)a.H * a.D, a.Sq - q0, a.D);
-    float dq[2][DP / 32][4] = {};
+    float dq[2][DP / 64][4] = {};
     for (int k0 = 0; k0 < len; k0 += AS_T) {
         __syncthreads();
         as_load<DT, DP>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], len - k0, a.D);
@@ -374,14 +440,24 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_dq_kernel(const AttnArgs
         const int t = q0 + 2 * ty + i;
         if (t >= a.Sq) continue;
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c)
+        for (int c = 0; c < DP / 64; ++c)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int d = 4 * tx + 32 * c + e;
+                const int d = 4 * tx + 64 * c + e;
                 if (d < a.D)
                     store_act(a.dq, (((long long)b * a.Sq + t) * a.H + h) * a.D + d, DT, dq[i][c][e] * a.scale);
             }
     }
+}
+
+// grid: key tiles * B * HK blocks for dK and dV, then query tiles * B * H for dQ
+template <int DT, int DP>
+__global__ void __launch_bounds__(AS_THREADS) attn_simt_bwd_kernel(const AttnArgs a) {
+    extern __shared__ float sm[];
+    griddep_wait();
+    const unsigned first = (unsigned)((a.Sk + AS_T - 1) / AS_T) * a.B * a.HK;
+    if (blockIdx.x < first) as_dkdv<DT, DP>(a, sm, blockIdx.x);
+    else as_dq<DT, DP>(a, sm, blockIdx.x - first);
 }
 
 }  // namespace reels
