@@ -155,6 +155,7 @@ int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t head
 
 // ---------------------------------------------------------------- attention
 constexpr int kPlanSms = 148;
+constexpr int kStatBlocks = 8 * kPlanSms;  // most blocks of the statistics kernel
 
 struct AttnPlan {
     bool tc = false;
@@ -204,17 +205,19 @@ AttnPlan plan_attention(const reels_attn_shape &s, int dt, const void *q, const 
     const int64_t per = ceil_div(tiles, want);
     p.splits = (int)ceil_div(tiles, per);
     p.split_keys = (int)std::min<int64_t>(per * tile, INT32_MAX - 256);
-    // dK, dV: the walk over queries is split where whole walks would leave
-    // SMs idle in the last round.  Steps of a round, and the partial sums'
-    // way through memory, in units of a step (about 1.2 us).
+    // Backward: one launch of the dK, dV walks and then the dQ walks, 1.9 and
+    // 1.35 us a step.  The first are split where a whole one would outlast the
+    // average SM: the launch ends about half a unit behind the average, and the
+    // partial sums pass through memory twice (about 5 TB/s) and a launch.
     if (p.tc && s.q_tokens > 0 && s.k_tokens > 0) {
-        const int64_t units = ceil_div(s.k_tokens, AT_TILE) * s.batch * s.kv_heads;
+        const double q_tiles = (double)(p.Sqp / AT_TILE), k_tiles = (double)ceil_div(s.k_tokens, AT_TILE);
         const int64_t steps = s.heads / s.kv_heads * (p.Sqp / AT_TILE);
-        const double mb = 2.0 * 2.0 * 4.0 * (double)(s.batch * s.k_tokens * s.kv_heads * s.head_dim) / 5e6;
+        const double work = (double)(s.batch * s.heads) * q_tiles * k_tiles * (1.9 + 1.35) / kPlanSms;
+        const double part = 2.0 * 2.0 * 4.0 * (double)(s.batch * s.k_tokens * s.kv_heads * s.head_dim) / 5e6;
         double best = 1e300;
         for (int64_t n = 1; n <= std::min<int64_t>(steps, 32); ++n) {
-            const double cost = (double)ceil_div(units * n, kPlanSms) * (double)(ceil_div(steps, n) + 3) +
-                                (n > 1 ? 4.0 + mb * (double)n / 1.2 : 0.0);
+            const double unit = 1.9 * (double)ceil_div(steps, n) + 4.0;
+            const double cost = std::max(work, unit) + 0.5 * unit + (n > 1 ? 4.0 + part * (double)n : 0.0);
             if (cost < best * 0.97) best = cost, p.red_splits = (int)n;
         }
         p.red_splits = (int)ceil_div(steps, ceil_div(steps, p.red_splits));
@@ -243,7 +246,7 @@ AttnWs attn_ws(const reels_attn_shape &s, const AttnPlan &p, bool bwd) {
         const size_t rows = (size_t)s.batch * s.heads * p.Sqp;
         w.stat_l = take(rows * 4);
         w.stat_d = take(rows * 4);
-        w.range = take(8);
+        w.range = take(kStatBlocks * 8);
         if (p.red_splits > 1) {
             const size_t n = (size_t)p.red_splits * s.batch * s.k_tokens * s.kv_heads * s.head_dim * 4;
             w.part_k = take(n);
@@ -296,8 +299,9 @@ cudaError_t simt_attrs() {
 template <int DT, int DP>
 cudaError_t tc_attrs() {
     cudaError_t e = big_smem(attn_fwd_kernel<DT, DP>, AttnFwdGeom<DP>::SMEM_BYTES);
-    if (e == cudaSuccess) e = big_smem(attn_dkdv_kernel<DT, DP>, AttnKvGeom<DP>::SMEM_BYTES);
-    if (e == cudaSuccess) e = big_smem(attn_dq_kernel<DT, DP>, AttnQGeom<DP>::SMEM_BYTES);
+    if (e == cudaSuccess) e = big_smem(attn_bwd_kernel<DT, DP, 0>, AttnBwdGeom<DP>::SMEM_BYTES);
+    if (e == cudaSuccess) e = big_smem(attn_bwd_kernel<DT, DP, 1>, AttnBwdGeom<DP>::SMEM_BYTES);
+    if (e == cudaSuccess) e = big_smem(attn_bwd_kernel<DT, DP, 2>, AttnBwdGeom<DP>::SMEM_BYTES);
     return e;
 }
 // Shared-memory sizes of the kernels, once per device (which is current).
@@ -482,14 +486,7 @@ int reels_attention_backward(const reels_attn_shape *shape, const void *q, const
     float *stat_l = reinterpret_cast<float *>(ws + w.stat_l), *stat_d = reinterpret_cast<float *>(ws + w.stat_d);
     a.stat_l = stat_l, a.stat_d = stat_d;
     a.part_k = reinterpret_cast<float *>(ws + w.part_k), a.part_v = reinterpret_cast<float *>(ws + w.part_v);
-    unsigned *range = nullptr;
     cudaError_t e = cudaSuccess;
-    if (plan.tc && act_dtype == REELS_F16) {
-        range = reinterpret_cast<unsigned *>(ws + w.range);
-        a.range = range;
-        e = cudaMemsetAsync(range, 0, 8, st);
-        if (e != cudaSuccess) return host_fail_dev(std::string("cudaMemsetAsync: ") + cudaGetErrorString(e));
-    }
     const int64_t rows = s.batch * s.heads * plan.Sqp, keys = s.batch * s.kv_heads * s.k_tokens;
     if (!plan.tc)
         with_dtype(act_dtype, [&](auto t) {
@@ -501,8 +498,11 @@ int reels_attention_backward(const reels_attn_shape *shape, const void *q, const
         with_tc_type(act_dtype, s.head_dim, [&](auto t, auto d) {
             constexpr int DT = decltype(t)::value, G = decltype(d)::value / 8;
             const int64_t blocks = ceil_div(s.batch * s.q_tokens * s.heads, 256 / G * 4);
-            e = host_launch_pdl(attn_stat_vec_kernel<DT, G>, dim3((unsigned)std::min<int64_t>(blocks, 8ll * call.sms)),
-                                dim3(256), 0, st, a, stat_l, stat_d, range, AtRange<DT>::BWD_SHIFT);
+            float2 *range = reinterpret_cast<float2 *>(ws + w.range);
+            a.range = range;
+            a.ranges = (int)std::min<int64_t>(blocks, kStatBlocks);
+            e = host_launch_pdl(attn_stat_vec_kernel<DT, G>, dim3((unsigned)a.ranges), dim3(256), 0, st, a, stat_l,
+                                stat_d, range, AtRange<DT>::BWD_SHIFT);
         });
     RA_LAUNCH(e);
     if (!plan.tc) {
@@ -518,14 +518,6 @@ int reels_attention_backward(const reels_attn_shape *shape, const void *q, const
         RA_LAUNCH(e);
         return host_ok(REELS_PATH_CUDACORE);
     }
-    if (range) {
-        with_dtype(act_dtype, [&](auto t) {
-            e = host_launch_pdl(attn_range_kernel<decltype(t)::value>,
-                                dim3((unsigned)std::min<int64_t>(ceil_div(keys, 8), 8ll * call.sms)), dim3(256), 0, st,
-                                a, range + 1);
-        });
-        RA_LAUNCH(e);
-    }
     const int64_t og[3] = {s.q_tokens * s.heads * s.head_dim, s.heads * s.head_dim, s.head_dim};
     CUtensorMap mq, mk, mv, mg;
     if ((rc = attn_map(&mq, q, act_dtype, s.batch, s.q_tokens, s.heads, s.head_dim, s.q_stride)) ||
@@ -533,27 +525,45 @@ int reels_attention_backward(const reels_attn_shape *shape, const void *q, const
         (rc = attn_map(&mv, v, act_dtype, s.batch, s.k_tokens, s.kv_heads, s.head_dim, s.v_stride)) ||
         (rc = attn_map(&mg, dout, act_dtype, s.batch, s.q_tokens, s.heads, s.head_dim, og)))
         return rc;
-    const long long kv_units = ceil_div(s.k_tokens, AT_TILE) * s.batch * s.kv_heads * plan.red_splits;
-    const long long q_units = (long long)(plan.Sqp / AT_TILE) * s.batch * s.heads;
+    AttnBwdUnits n = {};
+    const int64_t q_tiles = plan.Sqp / AT_TILE, k_tiles = ceil_div(s.k_tokens, AT_TILE);
+    n.kv = k_tiles * s.batch * s.kv_heads * plan.red_splits;
+    n.q = q_tiles * s.batch * s.heads;
+    // A block's start and end take some 3 us.  With many units of each kind a
+    // block stays on its SM and the walks are launched one after the other (2 x
+    // 6144 tokens, 32 heads: 3160 us; together, in blocks of two units, 3274);
+    // with few, blocks of about 32 steps of both let the SMs even out (8190
+    // queries over 512 keys, 40 heads: 352 us together, 381 one by one).
+    const bool apart = std::min(n.kv, n.q) >= 8ll * call.sms;
+    const int64_t fill = ceil_div(n.kv + n.q, call.sms);
+    auto blocks_of = [&](int64_t units, int64_t steps) {
+        return ceil_div(units, std::max<int64_t>(1, std::min<int64_t>(32 / std::max<int64_t>(steps, 1), fill)));
+    };
+    n.kv_blocks = (unsigned)blocks_of(n.kv, ceil_div(s.heads / s.kv_heads * q_tiles, plan.red_splits));
+    const int64_t blocks = n.kv_blocks + blocks_of(n.q, k_tiles);
     with_tc_type(act_dtype, s.head_dim, [&](auto t, auto d) {
-        constexpr int DT = decltype(t)::value, DP = decltype(d)::value;
-        e = host_launch_pdl(attn_dkdv_kernel<DT, DP>, dim3((unsigned)std::min<long long>(kv_units, call.sms)),
-                            dim3(AB_THREADS), AttnKvGeom<DP>::SMEM_BYTES, st, mq, mk, mv, mg, a, kv_units);
-        if (e == cudaSuccess && plan.red_splits > 1) {
-            const long long n = (long long)keys * s.head_dim;
-            const dim3 grid((unsigned)std::min<long long>(ceil_div(n, 1024), 8ll * call.sms));
-            e = host_launch_pdl(attn_sum_kernel<DT>, grid, dim3(256), 0, st, (const float *)a.part_k, n,
-                                plan.red_splits, a.dk);
+        constexpr int DT = decltype(t)::value, DP = decltype(d)::value, SM = AttnBwdGeom<DP>::SMEM_BYTES;
+        const dim3 block(AB_THREADS), all((unsigned)call.sms);
+        if (apart) {
+            e = host_launch_pdl(attn_bwd_kernel<DT, DP, 1>, all, block, SM, st, mq, mk, mv, mg, a, n);
             if (e == cudaSuccess)
-                e = host_launch_pdl(attn_sum_kernel<DT>, grid, dim3(256), 0, st, (const float *)a.part_v, n,
-                                    plan.red_splits, a.dv);
+                e = host_launch_pdl(attn_bwd_kernel<DT, DP, 2>, all, block, SM, st, mq, mk, mv, mg, a, n);
+        } else {
+            e = host_launch_pdl(attn_bwd_kernel<DT, DP, 0>, dim3((unsigned)blocks), block, SM, st, mq, mk, mv, mg, a,
+                                n);
         }
-        if (e == cudaSuccess)
-            e = host_launch_pdl(attn_dq_kernel<DT, DP>, dim3((unsigned)std::min<long long>(q_units, call.sms)),
-                                dim3(AB_THREADS), AttnQGeom<DP>::SMEM_BYTES, st, mq, mk, mv, mg, a, q_units);
     });
     RA_LAUNCH(e);
-    for (int i = 0; i < (plan.red_splits > 1 ? 3 : 1); ++i) host_count_launch();
+    if (apart) host_count_launch();
+    if (plan.red_splits > 1) {
+        const long long values = (long long)keys * s.head_dim;
+        const dim3 grid((unsigned)std::min<long long>(ceil_div(values, 1024), 4ll * call.sms), 2);
+        if (act_dtype == REELS_BF16)
+            e = host_launch_pdl(attn_sum_kernel<DT_BF16>, grid, dim3(256), 0, st, a, values, plan.red_splits);
+        else
+            e = host_launch_pdl(attn_sum_kernel<DT_F16>, grid, dim3(256), 0, st, a, values, plan.red_splits);
+        RA_LAUNCH(e);
+    }
     return host_ok(REELS_PATH_TENSORCORE);
 }
 

@@ -5,10 +5,10 @@
 //   dS = P (dP - delta),  dP = dO V',  delta = rowsum(dO * O)
 //   dV = P' dO,   dK = scale dS' Q,   dQ = scale dS K
 //
-// Two kernels, each a sum in registers' order with no atomics, so repeated
-// calls give the same bits: one walks the queries of a key tile (dK, dV; four
-// products a step), one the keys of a query tile (dQ; three).  Seven products
-// where one pass with scattered sums of dQ would need five.
+// Two walks, each a sum in a fixed order with no atomics, so repeated calls
+// give the same bits: one over the queries of a key tile (dK, dV; four products
+// a step), one over the keys of a query tile (dQ; three).  Seven products where
+// one walk with scattered sums of dQ would need five.
 //
 // In both, the second product's operand (P', dS', dS) is written by the CUDA
 // cores into tensor memory over the scores it came from, which the issuing
@@ -19,12 +19,25 @@
 namespace reels {
 
 constexpr int AB_THREADS = 32 * 12;  // 8 elementwise warps, loads, MMA issue, two idle
+using AbRegisters = AtRegisters<216>;
 
-// fp16: exponent e with |dS| 2^e <= 2^15, from |dP|, |delta| <= |dO row| |v row|.
+// fp16: exponent e with |dS| 2^e <= 2^15, from |dP|, |delta| <= |dO row| |v row|
+// whose largest values the blocks of the statistics kernel left.  Called by
+// whole warps.
 template <int DT>
 __device__ __forceinline__ int attn_grad_exp(const AttnArgs &a) {
     if (DT != DT_F16) return 0;
-    const float top = __uint_as_float(__ldcg(a.range)) * __uint_as_float(__ldcg(a.range + 1));
+    float g = 0.0f, v = 0.0f;
+    for (int i = threadIdx.x & 31; i < a.ranges; i += 32) {
+        const float2 r = __ldcg(a.range + i);
+        g = fmaxf(g, r.x), v = fmaxf(v, r.y);
+    }
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) {
+        g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, w));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, w));
+    }
+    const float top = g * v;
     if (!(top > 1e-30f) || !(top < 1e30f)) return 0;
     return 13 - ilogbf(top);
 }
@@ -96,13 +109,10 @@ __device__ __forceinline__ AttnKvUnit attn_kv_unit(const AttnArgs &a, long long 
 }
 
 template <int DT, int DP>
-__global__ void __launch_bounds__(AB_THREADS, 1)
-    attn_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG,
-                     const AttnArgs a, const long long units) {
+__device__ __forceinline__ void attn_dkdv(const CUtensorMap &tmQ, const CUtensorMap &tmK, const CUtensorMap &tmV,
+                                          const CUtensorMap &tmG, const AttnArgs &a, uint8_t *smem, long long u0,
+                                          long long units, unsigned step) {
     using G = AttnKvGeom<DP>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
     uint64_t *kv_full = bars, *kv_empty = bars + 1, *s_full = bars + 2, *p_full = bars + 3, *dp_full = bars + 4,
@@ -146,16 +156,15 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    griddep_wait();
     const int nqt = a.Sqp / AT_TILE, group = a.H / a.HK;
 
     if (warp == 8) {
         // ------------------------------------------------------------ loads
-        at_fewer_registers();
+        AbRegisters::fewer();
         if (lane == 0) {
             uint32_t g = 0, nu = 0;
             bool good = true;
-            for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+            for (long long u = u0; u < units && good; u += step) {
                 const AttnKvUnit w = attn_kv_unit(a, u);
                 if (w.n == 0) continue;
                 good = wait_bar(kv_empty, (nu++ & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_W_EMPTY);
@@ -183,12 +192,12 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
             }
         }
     } else if (warp > 9) {
-        at_fewer_registers();  // idle: completes the third group of four warps
+        AbRegisters::fewer();  // idle: completes the third group of four warps
     } else if (warp == 9) {
         // -------------------------------------------------------------- MMAs
         // In turn: dV(i), S'(i+1) run under the elementwise dS(i), and dK(i),
         // dP'(i+1) under the exponentials of step i+1.
-        at_fewer_registers();
+        AbRegisters::fewer();
         const bool leader = at_elect();
         constexpr int ab = DT == DT_BF16 ? 1 : 0;
         constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
@@ -226,7 +235,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                 mma_commit(which ? &q_empty[s] : &g_empty[s]);  // dK is the last to read Q, dV dO
             }
         };
-        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+        for (long long u = u0; u < units && good; u += step) {
             const AttnKvUnit w = attn_kv_unit(a, u);
             if (w.n == 0) continue;
             good = at_wait(kv_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_W_FULL);
@@ -245,7 +254,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
         if (leader) mma_commit(mma_done);
     } else {
         // --------------------------------------------- P', dS' and the output
-        at_more_registers();
+        AbRegisters::more();
         const int half = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t S = tmem + lanes + 64 * half, DS = S + 128, O = tmem + lanes + 256 + 128 * half;
@@ -257,7 +266,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
         const float f = half ? a.scale * exp2f(-(float)e) : exp2f(-AtRange<DT>::BWD_SHIFT);
         uint32_t g = 0, ns = 0, nu = 0;
         bool good = true;
-        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+        for (long long u = u0; u < units && good; u += step) {
             const AttnKvUnit w = attn_kv_unit(a, u);
             const int row = (warp & 3) * 32 + lane;
             const bool live = row < w.rows;
@@ -358,10 +367,12 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
     if (warp == 8) at_finish(tmem, mma_done, 1, a.err);
 }
 
-// Adds the partial dK and dV of the split walk in order.
+// Adds the partial dK (blockIdx.y = 0) and dV of the split walk in order.
 template <int DT>
-__global__ void __launch_bounds__(256) attn_sum_kernel(const float *part, long long n, int splits, void *out) {
+__global__ void __launch_bounds__(256) attn_sum_kernel(const AttnArgs a, long long n, int splits) {
     griddep_wait();
+    const float *part = blockIdx.y ? a.part_v : a.part_k;
+    void *out = blockIdx.y ? a.dv : a.dk;
     for (long long i = 4ll * (blockIdx.x * 256ll + threadIdx.x); i < n; i += 1024ll * gridDim.x) {
         float4 s = __ldcg(reinterpret_cast<const float4 *>(part + i));
         for (int k = 1; k < splits; ++k) {
@@ -409,13 +420,10 @@ __device__ __forceinline__ AttnQUnit attn_q_unit(const AttnArgs &a, long long u)
 }
 
 template <int DT, int DP>
-__global__ void __launch_bounds__(AB_THREADS, 1)
-    attn_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const AttnArgs a,
-                   const long long units) {
+__device__ __forceinline__ void attn_dq(const CUtensorMap &tmQ, const CUtensorMap &tmK, const CUtensorMap &tmV,
+                                        const CUtensorMap &tmG, const AttnArgs &a, uint8_t *smem, long long u0,
+                                        long long units, unsigned step) {
     using G = AttnQGeom<DP>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + G::BAR_OFF);
     uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *s_empty = bars + 4, *dp_full = bars + 6,
@@ -464,14 +472,13 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    griddep_wait();
 
     if (warp == 8) {
         // ------------------------------------------------------------ loads
-        at_fewer_registers();
+        AbRegisters::fewer();
         uint32_t g = 0, nu = 0, nraw = 0;
         bool good = true;
-        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+        for (long long u = u0; u < units && good; u += step) {
             const AttnQUnit w = attn_q_unit(a, u);
             if (w.nk == 0) continue;
             good = at_wait(q_empty, (nu++ & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_AB_EMPTY);
@@ -507,12 +514,12 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
             }
         }
     } else if (warp > 9) {
-        at_fewer_registers();  // idle: completes the third group of four warps
+        AbRegisters::fewer();  // idle: completes the third group of four warps
     } else if (warp == 9) {
         // -------------------------------------------------------------- MMAs
         // In turn: dQ(j), dP(j+1), S(j+2); the scores run two tiles ahead of
         // the elementwise warps' dS.
-        at_fewer_registers();
+        AbRegisters::fewer();
         const bool leader = at_elect();
         constexpr int ab = DT == DT_BF16 ? 1 : 0;
         constexpr uint32_t id_s = idesc_f16(ab, 0, 0, 128, AT_TILE), id_o = idesc_f16(ab, 0, 1, 128, DP);
@@ -549,7 +556,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
                 mma_commit(&v_empty[t]);
             }
         };
-        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+        for (long long u = u0; u < units && good; u += step) {
             const AttnQUnit w = attn_q_unit(a, u);
             if (w.nk == 0) continue;
             good = at_wait(q_full, nu & 1, abort, a.err, DEVERR_TIMEOUT_AB_FULL);
@@ -578,7 +585,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
         if (leader) mma_commit(mma_done);
     } else {
         // ----------------------------------------------------- dS and the output
-        at_more_registers();
+        AbRegisters::more();
         const int half = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t DS = tmem + lanes + 256 + 64 * half, O = tmem + lanes + 384;
@@ -589,7 +596,7 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
         const F2 grow = F2(g1, g1);
         uint32_t g = 0, nu = 0;
         bool good = true;
-        for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
+        for (long long u = u0; u < units && good; u += step) {
             const AttnQUnit w = attn_q_unit(a, u);
             const int row = w.q0 + (warp & 3) * 32 + lane;
             const long long st = ((long long)w.b * a.H + w.h) * a.Sqp + row;
@@ -677,6 +684,41 @@ __global__ void __launch_bounds__(AB_THREADS, 1)
     tc_fence_before();
     __syncthreads();
     if (warp == 8) at_finish(tmem, mma_done, 1, a.err);
+}
+
+// One launch for both: kv_blocks blocks for the units of dK and dV, the long
+// ones, then blocks for those of dQ, which fill the SMs that come free.  A block
+// takes every kv_blocks-th unit (likewise for dQ), so that blocks running side by
+// side are at neighbouring units and read the same keys or queries from L2 (a
+// run of neighbouring units for each block instead: 3213 to 3460 us at
+// 2 x 6144 tokens, 32 heads).
+template <int DP>
+struct AttnBwdGeom {
+    static constexpr int SMEM_BYTES = AttnKvGeom<DP>::SMEM_BYTES > AttnQGeom<DP>::SMEM_BYTES
+                                          ? AttnKvGeom<DP>::SMEM_BYTES
+                                          : AttnQGeom<DP>::SMEM_BYTES;
+};
+struct AttnBwdUnits {
+    long long kv, q;  // units
+    unsigned kv_blocks;
+};
+
+// PART: 0 both, 1 dK and dV alone, 2 dQ alone (large calls, where nothing is
+// left to even out and each walk compiled by itself is 2% faster).
+template <int DT, int DP, int PART>
+__global__ void __launch_bounds__(AB_THREADS, 1)
+    attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmG, const AttnArgs a,
+                    const AttnBwdUnits n) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    griddep_wait();
+    if constexpr (PART == 1) attn_dkdv<DT, DP>(tmQ, tmK, tmV, tmG, a, smem, blockIdx.x, n.kv, gridDim.x);
+    else if constexpr (PART == 2) attn_dq<DT, DP>(tmQ, tmK, tmV, tmG, a, smem, blockIdx.x, n.q, gridDim.x);
+    else if (blockIdx.x < n.kv_blocks)
+        attn_dkdv<DT, DP>(tmQ, tmK, tmV, tmG, a, smem, blockIdx.x, n.kv, n.kv_blocks);
+    else
+        attn_dq<DT, DP>(tmQ, tmK, tmV, tmG, a, smem, blockIdx.x - n.kv_blocks, n.q, gridDim.x - n.kv_blocks);
 }
 
 }  // namespace reels

@@ -121,10 +121,15 @@ struct AtRange {
 
 // The kernels are launched with 12 warps of 168 registers a thread.  The
 // eight elementwise warps (two groups of four) hold a row of scores each and
-// take 216, the other four keep 72: 256 * 216 + 128 * 72 = 384 * 168.  Called
-// at the head of each role, so that the compiler knows which count holds.
-__device__ __forceinline__ void at_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
-__device__ __forceinline__ void at_fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
+// take MORE, the other four keep FEWER: 256 MORE + 128 FEWER = 384 * 168.
+// Called at the head of each role, so that the compiler knows which count holds.
+template <int MORE>
+struct AtRegisters {
+    static constexpr int FEWER = 504 - 2 * MORE;
+    static_assert(MORE % 8 == 0 && FEWER % 8 == 0 && FEWER >= 24, "register counts come in eights");
+    static __device__ __forceinline__ void more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MORE)); }
+    static __device__ __forceinline__ void fewer() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEWER)); }
+};
 
 // A wait of a whole warp on one barrier.
 __device__ __forceinline__ bool at_wait(uint64_t *bar, uint32_t parity, volatile int *abort, unsigned *err,

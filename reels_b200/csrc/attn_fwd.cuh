@@ -24,6 +24,7 @@
 namespace reels {
 
 constexpr int AF_THREADS = 32 * 12;
+using AfRegisters = AtRegisters<224>;
 
 template <int DP>
 struct AttnFwdGeom {
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
 
     if (warp == 8) {
         // ------------------------------------------------------------ loads
-        at_fewer_registers();
+        AfRegisters::fewer();
         uint32_t g = 0, qn[2] = {0, 0}, nraw = 0;
         bool good = true;
         for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
@@ -162,14 +163,14 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
             }
         }
     } else if (warp == 11) {
-        at_fewer_registers();  // idle: completes the third group of four warps
+        AfRegisters::fewer();  // idle: completes the third group of four warps
     } else if (warp > 8) {
         // -------------------------------------------------------------- MMAs
         // An issuer for each tile, so that one's waits run beside the other's
         // products, and in turn: products of both tiles issued side by side
         // would share the tensor core and end together, and then both
         // softmaxes would run, and wait, at the same time.
-        at_fewer_registers();
+        AfRegisters::fewer();
         const int t = warp - 9;
         const bool leader = at_elect();
         constexpr int ab = DT == DT_BF16 ? 1 : 0;
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
         if (leader) mma_commit(&mma_done[t]);
     } else {
         // ------------------------------------------------- softmax and output
-        at_more_registers();
+        AfRegisters::more();
         const int t = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t S = tmem + t * 128 + lanes, O = tmem + 256 + t * 128 + lanes;

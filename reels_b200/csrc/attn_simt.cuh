@@ -39,7 +39,8 @@ struct AttnArgs {
     const float *stat_l, *stat_d;            // [B][H][Sqp]: -L in log2 units (-inf: no part), -delta
     int Sqp;                                 // Sq rounded up to whole tiles
     void *dq, *dk, *dv;                      // contiguous, in the layout of q, k and v
-    const unsigned *range;                   // fp16: largest |dO row|, |v row| (float bits)
+    const float2 *range;                     // fp16: [ranges] largest |dO row| and |v row| of a block
+    int ranges;
     int red_splits;                          // dK, dV: ranges of the (head, query tile) walk
     float *part_k, *part_v;                  // [red_splits][B][Sk][HK][D]
     unsigned *err;
@@ -256,64 +257,77 @@ __global__ void __launch_bounds__(256) attn_stat_kernel(const AttnArgs a, float 
     }
 }
 
-// The same for 16-bit rows of D = 8 n features up to 8 G, as the tensor-core
-// kernels take them: G lanes a row with 16 bytes each, four rows in flight,
-// rows in memory order (the heads of a token side by side).  `shift` is added
-// to -L (fp16, see AtRange); `range` receives the largest |dO row| (fp16; a
-// maximum does not depend on the order of its atomics).  Bound: HBM, out and
-// dO once.
-template <int DT, int G>
-__global__ void __launch_bounds__(256) attn_stat_vec_kernel(const AttnArgs a, float *stat_l, float *stat_d,
-                                                            unsigned *range, float shift) {
-    griddep_wait();
+// The largest |row|^2 and, with `y`, x . y of rows of D = 8 n <= 8 G features:
+// G lanes a row with 16 bytes each, four rows in flight.
+template <int DT, int G, typename At, typename Use>
+__device__ __forceinline__ void as_rows(const void *x, const void *y, long long rows, int D, At at, Use use,
+                                        float &top) {
     using T = typename Elem<DT>::T;
     constexpr int R = 4;
     const int sub = threadIdx.x % G;
-    const long long rows = (long long)a.B * a.Sq * a.H, step = (long long)gridDim.x * (256 / G) * R;
-    float top = 0.0f;  // largest |dO row|^2
-    for (long long r0 = ((long long)blockIdx.x * (256 / G) + threadIdx.x / G) * R, any = (long long)blockIdx.x * (256 / G) * R;
-         any < rows; r0 += step, any += step) {  // (a block stays together for its shuffles)
-        uint4 x[R], y[R];
+    const long long step = (long long)gridDim.x * (256 / G) * R;
+    // (the bound is the block's first row: a block stays together for its shuffles)
+    for (long long first = (long long)blockIdx.x * (256 / G) * R; first < rows; first += step) {
+        const long long r0 = first + threadIdx.x / G * R;
+        uint4 u[R], v[R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            x[i] = y[i] = make_uint4(0, 0, 0, 0);
-            if (r0 + i < rows && 8 * sub < a.D) {
-                x[i] = __ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.dout) + (r0 + i) * a.D) + sub);
-                y[i] = __ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.out) + (r0 + i) * a.D) + sub);
+            u[i] = v[i] = make_uint4(0, 0, 0, 0);
+            if (r0 + i < rows && 8 * sub < D) {
+                const long long o = at(r0 + i);
+                if (o >= 0) {
+                    u[i] = __ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(x) + o) + sub);
+                    if (y) v[i] = __ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(y) + o) + sub);
+                }
             }
         }
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            float delta = 0.0f, n2 = 0.0f;
+            float dot = 0.0f, n2 = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float g = load_act(&x[i], j, DT);
-                delta += g * load_act(&y[i], j, DT);
+                const float g = load_act(&u[i], j, DT);
+                if (y) dot += g * load_act(&v[i], j, DT);
                 if (DT == DT_F16) n2 += g * g;
             }
 #pragma unroll
             for (int w = G / 2; w > 0; w >>= 1) {
-                delta += __shfl_xor_sync(0xffffffffu, delta, w);
+                if (y) dot += __shfl_xor_sync(0xffffffffu, dot, w);
                 if (DT == DT_F16) n2 += __shfl_xor_sync(0xffffffffu, n2, w);
             }
             top = fmaxf(top, n2);
-            if (sub == 0 && r0 + i < rows) {
-                int b, q, h;
-                if (rows <= 0x7fffffff) {  // (64-bit divisions would cost more than the rows)
-                    const uint32_t r = (uint32_t)(r0 + i), tok = r / (uint32_t)a.H;
-                    h = (int)(r - tok * a.H), b = (int)(tok / (uint32_t)a.Sq), q = (int)(tok - b * (uint32_t)a.Sq);
-                } else {
-                    const long long tok = (r0 + i) / a.H;
-                    h = (int)((r0 + i) - tok * a.H), b = (int)(tok / a.Sq), q = (int)(tok - (long long)b * a.Sq);
-                }
-                const long long bh = (long long)b * a.H + h;
-                const float lse = __ldcg(a.lse + bh * a.Sq + q);
-                const bool dead = lse == -CUDART_INF_F;
-                stat_l[bh * a.Sqp + q] = dead ? -CUDART_INF_F : shift - lse * CUDART_L2E_F;
-                stat_d[bh * a.Sqp + q] = dead ? 0.0f : -delta;
-            }
+            if (sub == 0 && r0 + i < rows) use(r0 + i, dot);
         }
     }
+}
+
+// The same for the tensor-core kernels: rows in memory order (the heads of a
+// token side by side), `shift` added to -L (fp16, see AtRange), and for fp16
+// each block's largest |dO row| and |v row|.  Bound: HBM, out and dO once.
+template <int DT, int G>
+__global__ void __launch_bounds__(256) attn_stat_vec_kernel(const AttnArgs a, float *stat_l, float *stat_d,
+                                                            float2 *range, float shift) {
+    griddep_wait();
+    const long long rows = (long long)a.B * a.Sq * a.H;
+    float top = 0.0f, top_v = 0.0f;
+    as_rows<DT, G>(
+        a.dout, a.out, rows, a.D, [&](long long r) { return r * a.D; },
+        [&](long long r, float delta) {
+            int b, q, h;
+            if (rows <= 0x7fffffff) {  // (64-bit divisions would cost more than the rows)
+                const uint32_t tok = (uint32_t)r / (uint32_t)a.H;
+                h = (int)((uint32_t)r - tok * a.H), b = (int)(tok / (uint32_t)a.Sq), q = (int)(tok - b * (uint32_t)a.Sq);
+            } else {
+                const long long tok = r / a.H;
+                h = (int)(r - tok * a.H), b = (int)(tok / a.Sq), q = (int)(tok - (long long)b * a.Sq);
+            }
+            const long long bh = (long long)b * a.H + h;
+            const float lse = __ldcg(a.lse + bh * a.Sq + q);
+            const bool dead = lse == -CUDART_INF_F;
+            stat_l[bh * a.Sqp + q] = dead ? -CUDART_INF_F : shift - lse * CUDART_L2E_F;
+            stat_d[bh * a.Sqp + q] = dead ? 0.0f : -delta;
+        },
+        top);
     const int pad = a.Sqp - a.Sq;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < (long long)a.B * a.H * pad; i += gridDim.x * 256ll) {
         const long long at = i / pad * a.Sqp + a.Sq + i % pad;
@@ -321,34 +335,33 @@ __global__ void __launch_bounds__(256) attn_stat_vec_kernel(const AttnArgs a, fl
         stat_d[at] = 0.0f;
     }
     if (DT == DT_F16) {
+        __shared__ float2 warps[8];
+        as_rows<DT, G>(
+            a.v, nullptr, (long long)a.B * a.Sk * a.HK, a.D,
+            [&](long long r) {
+                int h, t, b;
+                if ((long long)a.B * a.Sk * a.HK <= 0x7fffffff) {
+                    const uint32_t tok = (uint32_t)r / (uint32_t)a.HK;
+                    h = (int)((uint32_t)r - tok * a.HK), b = (int)(tok / (uint32_t)a.Sk);
+                    t = (int)(tok - b * (uint32_t)a.Sk);
+                } else {
+                    h = (int)(r % a.HK), t = (int)(r / a.HK % a.Sk), b = (int)(r / a.HK / a.Sk);
+                }
+                return t < attn_keys(a, b) ? b * a.vs[0] + t * a.vs[1] + h * a.vs[2] : -1ll;
+            },
+            [](long long, float) {}, top_v);
 #pragma unroll
-        for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-        if ((threadIdx.x & 31) == 0) atomicMax(range, __float_as_uint(sqrtf(top)));
-    }
-}
-
-// fp16: the largest |v row|, so that the gradients' operands can be held in
-// range.  A maximum does not depend on the order of its atomics.
-template <int DT>
-__global__ void __launch_bounds__(256) attn_range_kernel(const AttnArgs a, unsigned *range) {
-    griddep_wait();
-    const int lane = threadIdx.x & 31;
-    const long long rows = (long long)a.B * a.HK * a.Sk;
-    float top = 0.0f;
-    for (long long row = blockIdx.x * 8ll + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8ll) {
-        const int h = (int)(row % a.HK), t = (int)(row / a.HK % a.Sk), b = (int)(row / a.HK / a.Sk);
-        if (t >= attn_keys(a, b)) continue;
-        const long long at = b * a.vs[0] + t * a.vs[1] + h * a.vs[2];
-        float n2 = 0.0f;
-        for (int d = lane; d < a.D; d += 32) {
-            const float x = load_act(a.v, at + d, DT);
-            n2 += x * x;
+        for (int w = 16; w > 0; w >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, w));
         }
-#pragma unroll
-        for (int w = 16; w > 0; w >>= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, w);
-        top = fmaxf(top, n2);
+        if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = make_float2(top, top_v);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < 8; ++w) top = fmaxf(top, warps[w].x), top_v = fmaxf(top_v, warps[w].y);
+            range[blockIdx.x] = make_float2(sqrtf(top), sqrtf(top_v));
+        }
     }
-    if (lane == 0) atomicMax(range, __float_as_uint(sqrtf(top)));
 }
 
 // P and dS of one 32 x 32 tile into shared memory, [query][key].
