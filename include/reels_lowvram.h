@@ -378,8 +378,10 @@ int reels_rms_norm_rope_backward(const void *x, const void *dout, int64_t M, int
  * place.  heads is a multiple of kv_heads: query head h reads key head
  * h / (heads / kv_heads).  head_dim <= 256.
  * 16-bit tensors with head_dim a multiple of 8 up to 128, 16-byte aligned
- * pointers and positive strides in multiples of 8 run on the tcgen05 path;
- * every other case runs on CUDA-core kernels. */
+ * pointers and positive strides in multiples of 8 run on the tcgen05 path
+ * (the forward with up to 8 query rows a key head, which is bound by reading
+ * the keys, on a CUDA-core kernel of its own); every other case runs on
+ * CUDA-core kernels. */
 typedef struct reels_attn_shape {
     int64_t batch, heads, kv_heads, q_tokens, k_tokens, head_dim;
     int64_t q_stride[3], k_stride[3], v_stride[3];
@@ -390,7 +392,7 @@ typedef struct reels_attn_shape {
 size_t reels_attention_workspace_bytes(const reels_attn_shape *shape, int act_dtype, int pass);
 
 /* The plan for aligned pointers, for diagnostics and tests; no device work.
- * info[0] path, info[1] key splits of the forward, info[2] keys per split,
+ * info[0] the forward's path, info[1] its key splits, info[2] keys per split,
  * info[3] splits of the walk over the queries for dk and dv. */
 int reels_attention_plan(const reels_attn_shape *shape, int act_dtype, int64_t *info);
 

@@ -159,6 +159,7 @@ constexpr int kStatBlocks = 8 * kPlanSms;  // most blocks of the statistics kern
 
 struct AttnPlan {
     bool tc = false;
+    int few = 0;                     // > 0: rows of a key head, few enough for attn_rows_kernel (forward)
     int splits = 1, split_keys = 1;  // forward
     int red_splits = 1;              // backward, dK and dV
     int Sqp = 0;
@@ -195,12 +196,17 @@ AttnPlan plan_attention(const reels_attn_shape &s, int dt, const void *q, const 
     p.tc = dt != REELS_F32 && s.head_dim % 8 == 0 && s.head_dim <= 128 && tma_strides(s.q_stride, nq) &&
            tma_strides(s.k_stride, nk) && tma_strides(s.v_stride, nk) && aligned16(q) && aligned16(k) && aligned16(v);
     p.Sqp = (int)(ceil_div(s.q_tokens, AT_TILE) * AT_TILE);
+    const int64_t shared = s.q_tokens * (s.heads / s.kv_heads);
+    if (p.tc && shared <= 8) p.few = (int)std::max<int64_t>(shared, 1);
     // Forward: few rows leave SMs idle, so the keys are split over them and
     // joined; a split keeps at least four tiles of keys (two on the CUDA cores).
-    const int tile = p.tc ? AT_TILE : AS_T;
-    const int64_t rows = ceil_div(s.q_tokens, p.tc ? 2 * AT_TILE : AS_T) * s.batch * s.heads;
+    // Blocks beside each other on an SM: 1 of the tensor-core kernel, 2 of the
+    // few-row kernel, 4 others.
+    const int tile = p.tc && !p.few ? AT_TILE : p.few ? 64 : AS_T;
+    const int64_t rows = p.few ? (int64_t)s.batch * s.kv_heads
+                               : ceil_div(s.q_tokens, p.tc ? 2 * AT_TILE : AS_T) * s.batch * s.heads;
     const int64_t tiles = std::max<int64_t>(1, ceil_div(s.k_tokens, tile));
-    int64_t want = rows > 0 ? std::min<int64_t>((p.tc ? 1 : 4) * kPlanSms / rows, tiles / (p.tc ? 4 : 2)) : 1;
+    int64_t want = rows > 0 ? std::min<int64_t>((p.few ? 2 : p.tc ? 1 : 4) * kPlanSms / rows, tiles / (p.tc ? 4 : 2)) : 1;
     want = std::max<int64_t>(1, std::min<int64_t>(want, 1024));
     const int64_t per = ceil_div(tiles, want);
     p.splits = (int)ceil_div(tiles, per);
@@ -372,7 +378,7 @@ int reels_attention_plan(const reels_attn_shape *shape, int act_dtype, int64_t *
     if (rc) return rc;
     if (!info) return host_fail("null info");
     const AttnPlan p = plan_attention(*shape, act_dtype, nullptr, nullptr, nullptr);
-    info[0] = p.tc ? REELS_PATH_TENSORCORE : REELS_PATH_CUDACORE;
+    info[0] = p.tc && !p.few ? REELS_PATH_TENSORCORE : REELS_PATH_CUDACORE;
     info[1] = p.splits;
     info[2] = p.split_keys;
     info[3] = p.red_splits;
@@ -409,7 +415,16 @@ int reels_attention_forward(const reels_attn_shape *shape, const void *q, const 
         a.part_lse = reinterpret_cast<float *>(reinterpret_cast<char *>(workspace) + w.part_lse);
     }
     cudaError_t e = cudaSuccess;
-    if (tc) {
+    if (tc && plan.few) {
+        const dim3 grid((unsigned)(s.batch * s.kv_heads), (unsigned)plan.splits);
+        with_tc_type(act_dtype, s.head_dim, [&](auto t, auto d) {
+            constexpr int DT = decltype(t)::value, G = decltype(d)::value / 8;
+            if (plan.few == 1) e = host_launch_pdl(attn_rows_kernel<DT, G, 1>, grid, dim3(256), 0, st, a);
+            else if (plan.few == 2) e = host_launch_pdl(attn_rows_kernel<DT, G, 2>, grid, dim3(256), 0, st, a);
+            else if (plan.few <= 4) e = host_launch_pdl(attn_rows_kernel<DT, G, 4>, grid, dim3(256), 0, st, a);
+            else e = host_launch_pdl(attn_rows_kernel<DT, G, 8>, grid, dim3(256), 0, st, a);
+        });
+    } else if (tc) {
         CUtensorMap mq, mk, mv;
         if ((rc = attn_map(&mq, q, act_dtype, s.batch, s.q_tokens, s.heads, s.head_dim, s.q_stride)) ||
             (rc = attn_map(&mk, k, act_dtype, s.batch, s.k_tokens, s.kv_heads, s.head_dim, s.k_stride)) ||
@@ -434,13 +449,15 @@ int reels_attention_forward(const reels_attn_shape *shape, const void *q, const 
     if (plan.splits > 1) {
         const int64_t rows = s.batch * s.heads * s.q_tokens;
         with_dtype(act_dtype, [&](auto t) {
-            e = host_launch_pdl(attn_join_kernel<decltype(t)::value>,
-                                dim3((unsigned)std::min<int64_t>(ceil_div(rows, 8), 8ll * call.sms)), dim3(256), 0, st,
-                                a);
+            with_simt_dim(s.head_dim, [&](auto d) {
+                e = host_launch_pdl(attn_join_kernel<decltype(t)::value, decltype(d)::value / 32>,
+                                    dim3((unsigned)std::min<int64_t>(ceil_div(rows, 4), 16ll * call.sms)), dim3(128), 0,
+                                    st, a);
+            });
         });
         RA_LAUNCH(e);
     }
-    return host_ok(tc ? REELS_PATH_TENSORCORE : REELS_PATH_CUDACORE);
+    return host_ok(tc && !plan.few ? REELS_PATH_TENSORCORE : REELS_PATH_CUDACORE);
 }
 
 int reels_attention_backward(const reels_attn_shape *shape, const void *q, const void *k, const void *v,

@@ -193,36 +193,185 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(const AttnArg
     }
 }
 
-// Joins the key splits of a row: weights exp(L_i - L), splits in order.  One warp a row.
-template <int DT>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
+__device__ __forceinline__ float as_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Forward for few rows (up to R = 8 queries and heads that share a key head, as
+// with single tokens): the keys and values pass once through registers at HBM
+// rate, where the tensor-core kernel would spend a whole 128-row softmax on
+// them (one row over 32760 keys of 12 heads: 44 us there).  A group of G lanes
+// takes a key, 16 bytes of it a lane; groups keep a running maximum, sum and
+// output of their own over every (256 / G)-th key, four keys at a time, and
+// are joined in a fixed order at the end.  P is not rounded here.
+// grid: B * HK, splits
+template <int DT, int G, int R>
+__global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a) {
+    using T = typename Elem<DT>::T;
+    constexpr int U = 4, GROUPS = 256 / G, DP = 8 * G;
+    __shared__ float sm[8][R][DP + 2];
+    griddep_wait();
+    const int lane = threadIdx.x & 31, sub = lane % G, grp = threadIdx.x / G;
+    const int b = blockIdx.x / a.HK, hk = blockIdx.x % a.HK, group = a.H / a.HK, rows = a.Sq * group;
+    const int len = attn_keys(a, b);
+    const int k_begin = min(len, (int)blockIdx.y * a.split_keys), k_end = min(len, k_begin + a.split_keys);
+    const bool live = 8 * sub < a.D;
+    float q[R][8], acc[R][8] = {}, m[R], l[R] = {};
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = -CUDART_INF_F;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < rows && live) {
+            const int h = hk * group + r / a.Sq, t = r % a.Sq;
+            x = __ldcg(reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.q) + b * a.qs[0] + t * a.qs[1] +
+                                                       h * a.qs[2]) + sub);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[r][j] = load_act(&x, j, DT) * (a.scale * CUDART_L2E_F);
+    }
+    const T *K = reinterpret_cast<const T *>(a.k) + b * a.ks[0] + hk * a.ks[2];
+    const T *V = reinterpret_cast<const T *>(a.v) + b * a.vs[0] + hk * a.vs[2];
+    uint4 nx[U], ny[U];  // the next keys and values, on their way
+    auto fetch = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int t = base + u * GROUPS + grp;
+            nx[u] = ny[u] = make_uint4(0, 0, 0, 0);
+            if (t < k_end && live) {
+                nx[u] = __ldcg(reinterpret_cast<const uint4 *>(K + t * a.ks[1]) + sub);
+                ny[u] = __ldcg(reinterpret_cast<const uint4 *>(V + t * a.vs[1]) + sub);
+            }
+        }
+    };
+    fetch(k_begin);
+    for (int base = k_begin; base < k_end; base += U * GROUPS) {
+        uint4 x[U], y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = nx[u], y[u] = ny[u];
+        fetch(base + U * GROUPS);
+        float s[U][R];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float k[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) k[j] = load_act(&x[u], j, DT);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float d = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d += q[r][j] * k[j];
+#pragma unroll
+                for (int w = G / 2; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
+                s[u][r] = base + u * GROUPS + grp < k_end ? d : -CUDART_INF_F;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float mx = m[r];
+#pragma unroll
+            for (int u = 0; u < U; ++u) mx = fmaxf(mx, s[u][r]);
+            const float ref = mx == -CUDART_INF_F ? 0.0f : mx, keep = as_exp2(m[r] - ref);
+            m[r] = mx;
+            l[r] *= keep;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[r][j] *= keep;
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[u][r] = as_exp2(s[u][r] - ref), l[r] += s[u][r];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = load_act(&y[u], j, DT);
+#pragma unroll
+                for (int r = 0; r < R; ++r) acc[r][j] += s[u][r] * v;
+            }
+    }
+    // the groups of a warp, then the warps
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int w = G; w < 32; w <<= 1) {
+            const float om = __shfl_xor_sync(0xffffffffu, m[r], w), mx = fmaxf(m[r], om);
+            const float ref = mx == -CUDART_INF_F ? 0.0f : mx, f = exp2f(m[r] - ref), g = exp2f(om - ref);
+            m[r] = mx;
+            l[r] = l[r] * f + __shfl_xor_sync(0xffffffffu, l[r], w) * g;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[r][j] = acc[r][j] * f + __shfl_xor_sync(0xffffffffu, acc[r][j], w) * g;
+        }
+        if (lane < G) {
+            float *at = sm[threadIdx.x >> 5][r];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) at[8 * sub + j] = acc[r][j];
+            if (sub == 0) at[DP] = m[r], at[DP + 1] = l[r];
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * DP; i += 256) {
+        const int r = i / DP, d = i % DP;
+        if (r >= rows || d >= a.D) continue;
+        float mx = -CUDART_INF_F, total = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) mx = fmaxf(mx, sm[w][r][DP]);
+        const float ref = mx == -CUDART_INF_F ? 0.0f : mx;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            const float f = exp2f(sm[w][r][DP] - ref);
+            total += f * sm[w][r][DP + 1];
+            o += f * sm[w][r][d];
+        }
+        const int h = hk * group + r / a.Sq, t = r % a.Sq;
+        const long long at = (((long long)blockIdx.y * a.B + b) * a.H + h) * a.Sq + t;
+        o *= total > 0.0f || total != total ? 1.0f / total : 0.0f;
+        if (d == 0) (a.splits > 1 ? a.part_lse : a.lse)[at] = (ref + log2f(total)) * CUDART_LN2_F;
+        if (a.splits > 1) a.part_o[at * a.D + d] = o;
+        else store_act(a.out, (((long long)b * a.Sq + t) * a.H + h) * a.D + d, DT, o);
+    }
+}
+
+// Joins the key splits of a row: weights exp(L_i - L), splits in order.  One
+// warp a row; the lanes hold a weight each and pass them on.  NC: 32-feature
+// pieces of a row; eight splits are read at a time.
+template <int DT, int NC>
+__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a) {
     griddep_wait();
     const int lane = threadIdx.x & 31;
     const long long rows = (long long)a.B * a.H * a.Sq;
-    for (long long row = blockIdx.x * 8ll + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8ll) {
+    for (long long row = blockIdx.x * 4ll + (threadIdx.x >> 5); row < rows; row += gridDim.x * 4ll) {
         float m = -CUDART_INF_F;
-        bool nan = false;
-        for (int s = lane; s < a.splits; s += 32) {
-            const float x = __ldcg(a.part_lse + s * rows + row);
-            m = fmaxf(m, x);
-            nan |= x != x;
-        }
+        for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, __ldcg(a.part_lse + s * rows + row));
 #pragma unroll
         for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-        if (__any_sync(0xffffffffu, nan)) m = CUDART_NAN_F;
         const float ref = m == -CUDART_INF_F ? 0.0f : m;
-        float total = 0.0f;
-        for (int s = 0; s < a.splits; ++s) total += expf(__ldcg(a.part_lse + s * rows + row) - ref);
+        float total = 0.0f, acc[NC] = {}, f = 0.0f;
+        for (int s0 = 0; s0 < a.splits; s0 += 8) {
+            float v[8][NC];
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+                    v[s][c] = s0 + s < a.splits && 32 * c + lane < a.D
+                                  ? __ldcg(a.part_o + ((s0 + s) * rows + row) * a.D + 32 * c + lane)
+                                  : 0.0f;
+            if ((s0 & 31) == 0)
+                f = s0 + lane < a.splits ? expf(__ldcg(a.part_lse + (s0 + lane) * rows + row) - ref) : 0.0f;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const float g = __shfl_sync(0xffffffffu, f, (s0 & 31) + s);
+                total += g;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) acc[c] += g * v[s][c];
+            }
+        }
         const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
         if (lane == 0) a.lse[row] = ref + logf(total);
         const int q = (int)(row % a.Sq), h = (int)(row / a.Sq % a.H), b = (int)(row / a.Sq / a.H);
-        for (int d = lane; d < a.D; d += 32) {
-            float acc = 0.0f;
-#pragma unroll 4
-            for (int s = 0; s < a.splits; ++s)
-                acc += expf(__ldcg(a.part_lse + s * rows + row) - ref) * __ldcg(a.part_o + (s * rows + row) * a.D + d);
-            store_act(a.out, (((long long)b * a.Sq + q) * a.H + h) * a.D + d, DT, acc * inv);
-        }
+        const long long at = (((long long)b * a.Sq + q) * a.H + h) * a.D;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if (32 * c + lane < a.D) store_act(a.out, at + 32 * c + lane, DT, acc[c] * inv);
     }
 }
 

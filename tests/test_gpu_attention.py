@@ -23,6 +23,12 @@ CASES = [
     (1, 256, 384, 2, 2, 64, HF, None, False),
     (1, 1, 1, 1, 1, 128, BF, None, False),
     (2, 1, 4097, 3, 3, 128, BF, None, False),     # one row, key splits
+    (3, 2, 300, 2, 2, 64, HF, [300, 0, 65], False),  # few rows: 2, 3, 4, 5, 8 a key head
+    (1, 1, 129, 6, 2, 128, HF, None, False),
+    (2, 2, 5000, 4, 2, 40, BF, [5000, 77], False),
+    (1, 5, 63, 1, 1, 96, BF, None, False),
+    (1, 4, 1000, 2, 1, 128, BF, [999], False),
+    (1, 3, 3, 2, 2, 64, BF, None, True),
     (1, 130, 2051, 2, 1, 64, HF, None, False),    # few rows, key splits, shared heads
     (2, 129, 131, 3, 3, 128, HF, [131, 3], False),   # one past a tile; a short sample
     (3, 200, 300, 4, 2, 128, BF, [0, 300, 128], False),  # no keys; a whole tile exactly
@@ -49,7 +55,7 @@ def test_parity(torch, B, Sq, Sk, H, HK, D, dtype, lengths, packed):
     c = ac.Case(B, Sq, Sk, H, HK, D, getattr(torch, dtype), lengths, packed, seed=Sq + Sk)
     out, lse = attention(c.q, c.k, c.v, kv_lengths=c.lengths, return_lse=True)
     check_device_status()
-    tc = dtype != FL and D % 8 == 0 and D <= 128
+    tc = dtype != FL and D % 8 == 0 and D <= 128 and Sq * H // HK > 8
     assert nat.last_path() == (nat.PATH_TENSORCORE if tc else nat.PATH_CUDACORE)
     want = ac.reference(c)
     ac.check("out", out, want["out"])
