@@ -160,6 +160,7 @@ constexpr int kStatBlocks = 8 * kPlanSms;  // most blocks of the statistics kern
 struct AttnPlan {
     bool tc = false;
     int few = 0;                     // > 0: rows of a key head, few enough for attn_rows_kernel (forward)
+    int tile = 32;                   // of the CUDA-core kernels: 64 where the blocks fill the GPU twice
     int splits = 1, split_keys = 1;  // forward
     int red_splits = 1;              // backward, dK and dV
     int Sqp = 0;
@@ -180,7 +181,7 @@ int check_shape(const reels_attn_shape *s, int dt) {
         return host_fail("head_dim must be between 1 and " + std::to_string(AT_MAX_D));
     const int64_t lim = INT32_MAX - 256;
     if (s->batch > lim || s->heads > lim || s->q_tokens > lim || s->k_tokens > lim ||
-        s->batch * s->heads > lim || ceil_div(std::max(s->q_tokens, s->k_tokens), AS_T) > lim / 2 / std::max<int64_t>(1, s->batch * s->heads))
+        s->batch * s->heads > lim || ceil_div(std::max(s->q_tokens, s->k_tokens), 32) > lim / 2 / std::max<int64_t>(1, s->batch * s->heads))
         return host_fail("attention shape too large");
     for (int i = 0; i < 3; ++i)
         if (s->q_stride[i] < 0 || s->k_stride[i] < 0 || s->v_stride[i] < 0) return host_fail("negative stride");
@@ -202,9 +203,10 @@ AttnPlan plan_attention(const reels_attn_shape &s, int dt, const void *q, const 
     // joined; a split keeps at least four tiles of keys (two on the CUDA cores).
     // Blocks beside each other on an SM: 1 of the tensor-core kernel, 2 of the
     // few-row kernel, 4 others.
-    const int tile = p.tc && !p.few ? AT_TILE : p.few ? 64 : AS_T;
+    if (s.head_dim <= 128 && ceil_div(s.q_tokens, 64) * s.batch * s.heads >= 2 * kPlanSms) p.tile = 64;
+    const int tile = p.few ? 64 : p.tc ? AT_TILE : p.tile;
     const int64_t rows = p.few ? (int64_t)s.batch * s.kv_heads
-                               : ceil_div(s.q_tokens, p.tc ? 2 * AT_TILE : AS_T) * s.batch * s.heads;
+                               : ceil_div(s.q_tokens, p.tc ? 2 * AT_TILE : p.tile) * s.batch * s.heads;
     const int64_t tiles = std::max<int64_t>(1, ceil_div(s.k_tokens, tile));
     int64_t want = rows > 0 ? std::min<int64_t>((p.few ? 2 : p.tc ? 1 : 4) * kPlanSms / rows, tiles / (p.tc ? 4 : 2)) : 1;
     want = std::max<int64_t>(1, std::min<int64_t>(want, 1024));
@@ -296,10 +298,17 @@ template <typename K>
 cudaError_t big_smem(K kern, int bytes) {
     return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
+template <int DT, int DP, int T>
+cudaError_t simt_tile_attrs() {
+    cudaError_t e = big_smem(attn_simt_fwd_kernel<DT, DP, T>, as_smem_bytes(DP, T, 3));
+    if (e == cudaSuccess) e = big_smem(attn_simt_bwd_kernel<DT, DP, T>, as_smem_bytes(DP, T, 4));
+    return e;
+}
 template <int DT, int DP>
 cudaError_t simt_attrs() {
-    cudaError_t e = big_smem(attn_simt_fwd_kernel<DT, DP>, as_smem_bytes(DP, 3));
-    if (e == cudaSuccess) e = big_smem(attn_simt_bwd_kernel<DT, DP>, as_smem_bytes(DP, 4));
+    cudaError_t e = simt_tile_attrs<DT, DP, 32>();
+    if constexpr (DP <= 128)
+        if (e == cudaSuccess) e = simt_tile_attrs<DT, DP, 64>();
     return e;
 }
 template <int DT, int DP>
@@ -335,6 +344,16 @@ void with_simt_dim(int64_t D, F &&f) {
     if (D <= 64) f(std::integral_constant<int, 64>{});
     else if (D <= 128) f(std::integral_constant<int, 128>{});
     else f(std::integral_constant<int, 256>{});
+}
+// The head size as the kernels' and the tile of the CUDA-core kernels.
+template <typename F>
+void with_simt_tile(int64_t D, int tile, F &&f) {
+    using T32 = std::integral_constant<int, 32>;
+    using T64 = std::integral_constant<int, 64>;
+    if (D <= 64) tile == 64 ? f(std::integral_constant<int, 64>{}, T64{}) : f(std::integral_constant<int, 64>{}, T32{});
+    else if (D <= 128)
+        tile == 64 ? f(std::integral_constant<int, 128>{}, T64{}) : f(std::integral_constant<int, 128>{}, T32{});
+    else f(std::integral_constant<int, 256>{}, T32{});
 }
 template <typename F>
 void with_tc_type(int dt, int64_t D, F &&f) {
@@ -437,11 +456,12 @@ int reels_attention_forward(const reels_attn_shape *shape, const void *q, const 
                                 dim3(AF_THREADS), AttnFwdGeom<DP>::SMEM_BYTES, st, mq, mk, mv, a, units);
         });
     } else {
-        const dim3 grid((unsigned)(ceil_div(s.q_tokens, AS_T) * s.batch * s.heads), (unsigned)plan.splits);
+        const dim3 grid((unsigned)(ceil_div(s.q_tokens, plan.tile) * s.batch * s.heads), (unsigned)plan.splits);
         with_dtype(act_dtype, [&](auto t) {
-            with_simt_dim(s.head_dim, [&](auto d) {
-                constexpr int DT = decltype(t)::value, DP = decltype(d)::value;
-                e = host_launch_pdl(attn_simt_fwd_kernel<DT, DP>, grid, dim3(AS_THREADS), as_smem_bytes(DP, 3), st, a);
+            with_simt_tile(s.head_dim, plan.tile, [&](auto d, auto tile) {
+                constexpr int DT = decltype(t)::value, DP = decltype(d)::value, T = decltype(tile)::value;
+                e = host_launch_pdl(attn_simt_fwd_kernel<DT, DP, T>, grid, dim3(AS_THREADS), as_smem_bytes(DP, T, 3),
+                                    st, a);
             });
         });
     }
@@ -524,12 +544,12 @@ int reels_attention_backward(const reels_attn_shape *shape, const void *q, const
     RA_LAUNCH(e);
     if (!plan.tc) {
         with_dtype(act_dtype, [&](auto t) {
-            with_simt_dim(s.head_dim, [&](auto d) {
-                constexpr int DT = decltype(t)::value, DP = decltype(d)::value;
-                const int64_t blocks = ceil_div(s.k_tokens, AS_T) * s.batch * s.kv_heads +
-                                       ceil_div(s.q_tokens, AS_T) * s.batch * s.heads;
-                e = host_launch_pdl(attn_simt_bwd_kernel<DT, DP>, dim3((unsigned)blocks), dim3(AS_THREADS),
-                                    as_smem_bytes(DP, 4), st, a);
+            with_simt_tile(s.head_dim, plan.tile, [&](auto d, auto tile) {
+                constexpr int DT = decltype(t)::value, DP = decltype(d)::value, T = decltype(tile)::value;
+                const int64_t blocks =
+                    ceil_div(s.k_tokens, T) * s.batch * s.kv_heads + ceil_div(s.q_tokens, T) * s.batch * s.heads;
+                e = host_launch_pdl(attn_simt_bwd_kernel<DT, DP, T>, dim3((unsigned)blocks), dim3(AS_THREADS),
+                                    as_smem_bytes(DP, T, 4), st, a);
             });
         });
         RA_LAUNCH(e);

@@ -9,10 +9,11 @@
 //   dV = P' dO,  dQ = scale dS k,  dK = scale dS' q
 // A row without keys has O = 0, L = -inf and no part in any gradient.
 //
-// 32 x 32 tiles of S in registers (2 x 2 a thread, 256 threads), operands in
-// shared memory as fp32; every sum is fp32 and in a fixed order.  Small fp32
-// clips are the use: a few tiles a block, so a block's latency counts, and dQ
-// runs beside dK and dV in one launch.
+// T x T tiles of S in registers (T / 16 squared a thread, 256 threads), operands
+// in shared memory as fp32; every sum is fp32 and in a fixed order.  T = 32 for
+// small clips, where a block's latency counts, 64 where the blocks fill the GPU
+// (half the shared-memory reads a product); dQ runs beside dK and dV in one
+// launch.
 #pragma once
 #include <math_constants.h>
 
@@ -21,7 +22,6 @@
 namespace reels {
 
 constexpr int AT_MAX_D = 256;  // head size
-constexpr int AS_T = 32;       // tile of the CUDA-core kernels
 constexpr int AS_THREADS = 256;
 
 struct AttnArgs {
@@ -53,98 +53,110 @@ __device__ __forceinline__ int attn_keys(const AttnArgs &a, int b) {
     return n < 0 ? 0 : (n < a.Sk ? n : a.Sk);
 }
 
-// 32 rows of D elements into dst[32][DP + 4], rows from `n` on and features
+// T rows of D elements into dst[T][DP + 4], rows from `n` on and features
 // from D on as zeros.  fp32 rows that allow it in 16-byte pieces.
-template <int DT, int DP>
+template <int DT, int DP, int T>
 __device__ __forceinline__ void as_load(float *dst, const void *src, long long at, long long pitch, int n, int D) {
     if (DT == DT_F32 && ((reinterpret_cast<uintptr_t>(src) & 15) | ((at | pitch | D) & 3)) == 0) {
         const float *p = reinterpret_cast<const float *>(src) + at;
-        float4 v[DP / 32];
+        constexpr int N = T * DP / 4 / AS_THREADS, B = N < 8 ? N : 8;
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-            const int x = threadIdx.x + i * AS_THREADS, r = x / (DP / 4), d = x % (DP / 4) * 4;
-            v[i] = (r < n && d < D) ? __ldcg(reinterpret_cast<const float4 *>(p + r * pitch + d))
-                                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
+        for (int i0 = 0; i0 < N; i0 += B) {
+            float4 v[B];
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-            const int x = threadIdx.x + i * AS_THREADS, r = x / (DP / 4), d = x % (DP / 4) * 4;
-            *reinterpret_cast<float4 *>(dst + r * (DP + 4) + d) = v[i];
+            for (int i = 0; i < B; ++i) {
+                const int x = threadIdx.x + (i0 + i) * AS_THREADS, r = x / (DP / 4), d = x % (DP / 4) * 4;
+                v[i] = (r < n && d < D) ? __ldcg(reinterpret_cast<const float4 *>(p + r * pitch + d))
+                                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const int x = threadIdx.x + (i0 + i) * AS_THREADS, r = x / (DP / 4), d = x % (DP / 4) * 4;
+                *reinterpret_cast<float4 *>(dst + r * (DP + 4) + d) = v[i];
+            }
         }
         return;
     }
 #pragma unroll 8
-    for (int i = threadIdx.x; i < AS_T * DP; i += AS_THREADS) {
+    for (int i = threadIdx.x; i < T * DP; i += AS_THREADS) {
         const int r = i / DP, d = i - r * DP;
         dst[r * (DP + 4) + d] = (r < n && d < D) ? load_act(src, at + r * pitch + d, DT) : 0.0f;
     }
 }
-// acc[i][j] = A[2 ty + i] . B[tx + 16 j]
-template <int DP>
-__device__ __forceinline__ void as_dot(const float *A, const float *B, int ty, int tx, float (&acc)[2][2]) {
+// acc[i][j] = A[N ty + i] . B[tx + 16 j], N = T / 16
+template <int DP, int N>
+__device__ __forceinline__ void as_dot(const float *A, const float *B, int ty, int tx, float (&acc)[N][N]) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = 0.0f;
+        for (int j = 0; j < N; ++j) acc[i][j] = 0.0f;
 #pragma unroll 8
     for (int d = 0; d < DP; d += 4) {
-        float4 x[2], y[2];
+        float4 x[N], y[N];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            x[i] = *reinterpret_cast<const float4 *>(A + (2 * ty + i) * (DP + 4) + d);
+        for (int i = 0; i < N; ++i) {
+            x[i] = *reinterpret_cast<const float4 *>(A + (N * ty + i) * (DP + 4) + d);
             y[i] = *reinterpret_cast<const float4 *>(B + (tx + 16 * i) * (DP + 4) + d);
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < N; ++j)
                 acc[i][j] += x[i].x * y[j].x + x[i].y * y[j].y + x[i].z * y[j].z + x[i].w * y[j].w;
     }
 }
-// acc[i][c][.] += sum_n W(2 ty + i, n) B[n][4 tx + 64 c ..]; W(r, n) = w[r * rs + n * ns]
-template <int DP>
+// acc[i][c][.] += sum_n W(N ty + i, n) B[n][4 tx + 64 c ..]; W(r, n) = w[r * rs + n * ns]
+template <int DP, int N>
 __device__ __forceinline__ void as_mix(const float *w, int rs, int ns, const float *B, int ty, int tx,
-                                       float (&acc)[2][DP / 64][4]) {
+                                       float (&acc)[N][DP / 64][4]) {
 #pragma unroll 4
-    for (int n = 0; n < AS_T; ++n) {
-        const float w0 = w[(2 * ty) * rs + n * ns], w1 = w[(2 * ty + 1) * rs + n * ns];
+    for (int n = 0; n < 16 * N; ++n) {
+        float f[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = w[(N * ty + i) * rs + n * ns];
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
             const float4 b = *reinterpret_cast<const float4 *>(B + n * (DP + 4) + 4 * tx + 64 * c);
-            acc[0][c][0] += w0 * b.x, acc[0][c][1] += w0 * b.y, acc[0][c][2] += w0 * b.z, acc[0][c][3] += w0 * b.w;
-            acc[1][c][0] += w1 * b.x, acc[1][c][1] += w1 * b.y, acc[1][c][2] += w1 * b.z, acc[1][c][3] += w1 * b.w;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                acc[i][c][0] += f[i] * b.x, acc[i][c][1] += f[i] * b.y;
+                acc[i][c][2] += f[i] * b.z, acc[i][c][3] += f[i] * b.w;
+            }
         }
     }
 }
-__host__ __device__ constexpr int as_smem_bytes(int DP, int tiles) {
-    return (tiles * AS_T * (DP + 4) + 2 * AS_T * (AS_T + 1)) * 4;
+__host__ __device__ constexpr int as_smem_bytes(int DP, int T, int tiles) {
+    return (tiles * T * (DP + 4) + 2 * T * (T + 1)) * 4;
 }
 
 // grid: query tiles * B * H, splits
-template <int DT, int DP>
+template <int DT, int DP, int T>
 __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(const AttnArgs a) {
     extern __shared__ float sm[];
-    float *Q = sm, *K = Q + AS_T * (DP + 4), *V = K + AS_T * (DP + 4), *P = V + AS_T * (DP + 4);
+    constexpr int N = T / 16;
+    float *Q = sm, *K = Q + T * (DP + 4), *V = K + T * (DP + 4), *P = V + T * (DP + 4);
     griddep_wait();
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int tiles = (a.Sq + AS_T - 1) / AS_T, bh = (int)(blockIdx.x / tiles);
-    const int q0 = (int)(blockIdx.x % tiles) * AS_T, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.HK);
+    const int tiles = (a.Sq + T - 1) / T, bh = (int)(blockIdx.x / tiles);
+    const int q0 = (int)(blockIdx.x % tiles) * T, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.HK);
     const int len = attn_keys(a, b);
     const int k_begin = min(len, (int)blockIdx.y * a.split_keys), k_end = min(len, k_begin + a.split_keys);
-    as_load<DT, DP>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
-    float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.0f, 0.0f}, o[2][DP / 64][4] = {};
-    for (int k0 = k_begin; k0 < k_end; k0 += AS_T) {
-        __syncthreads();
-        as_load<DT, DP>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], k_end - k0, a.D);
-        as_load<DT, DP>(V, a.v, b * a.vs[0] + k0 * a.vs[1] + hk * a.vs[2], a.vs[1], k_end - k0, a.D);
-        __syncthreads();
-        float s[2][2];
-        as_dot<DP>(Q, K, ty, tx, s);
+    as_load<DT, DP, T>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
+    float m[N], l[N] = {}, o[N][DP / 64][4] = {};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < N; ++i) m[i] = -CUDART_INF_F;
+    for (int k0 = k_begin; k0 < k_end; k0 += T) {
+        __syncthreads();
+        as_load<DT, DP, T>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], k_end - k0, a.D);
+        as_load<DT, DP, T>(V, a.v, b * a.vs[0] + k0 * a.vs[1] + hk * a.vs[2], a.vs[1], k_end - k0, a.D);
+        __syncthreads();
+        float s[N][N];
+        as_dot<DP, N>(Q, K, ty, tx, s);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
             float mx = -CUDART_INF_F;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < N; ++j) {
                 s[i][j] = k0 + tx + 16 * j < k_end ? s[i][j] * a.scale : -CUDART_INF_F;
                 mx = fmaxf(mx, s[i][j]);
             }
@@ -155,9 +167,9 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(const AttnArg
             const float keep = expf(m[i] - ref);
             float sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < N; ++j) {
                 const float p = expf(s[i][j] - ref);
-                P[(2 * ty + i) * (AS_T + 1) + tx + 16 * j] = p;
+                P[(N * ty + i) * (T + 1) + tx + 16 * j] = p;
                 sum += p;
             }
 #pragma unroll
@@ -170,11 +182,11 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(const AttnArg
                 for (int e = 0; e < 4; ++e) o[i][c][e] *= keep;
         }
         __syncwarp();  // the rows of P that a warp reads are its own
-        as_mix<DP>(P, AS_T + 1, 1, V, ty, tx, o);
+        as_mix<DP, N>(P, T + 1, 1, V, ty, tx, o);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int q = q0 + 2 * ty + i;
+    for (int i = 0; i < N; ++i) {
+        const int q = q0 + N * ty + i;
         if (q >= a.Sq) continue;
         const float inv = l[i] > 0.0f || l[i] != l[i] ? 1.0f / l[i] : 0.0f;
         const float lse = (m[i] == -CUDART_INF_F ? 0.0f : m[i]) + logf(l[i]);
@@ -513,22 +525,23 @@ __global__ void __launch_bounds__(256) attn_stat_vec_kernel(const AttnArgs a, fl
     }
 }
 
-// P and dS of one 32 x 32 tile into shared memory, [query][key].
-template <int DP>
+// P and dS of one T x T tile into shared memory, [query][key].
+template <int DP, int T>
 __device__ __forceinline__ void as_grad_tile(const AttnArgs &a, const float *Q, const float *K, const float *V,
                                              const float *G, float *P, float *S, long long stat_at, int k0, int len,
                                              int ty, int tx) {
-    float s[2][2], dp[2][2];
-    as_dot<DP>(Q, K, ty, tx, s);
-    as_dot<DP>(G, V, ty, tx, dp);
+    constexpr int N = T / 16;
+    float s[N][N], dp[N][N];
+    as_dot<DP, N>(Q, K, ty, tx, s);
+    as_dot<DP, N>(G, V, ty, tx, dp);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float2 st = make_float2(__ldcg(a.stat_l + stat_at + 2 * ty + i), __ldcg(a.stat_d + stat_at + 2 * ty + i));
+    for (int i = 0; i < N; ++i) {
+        const float2 st = make_float2(__ldcg(a.stat_l + stat_at + N * ty + i), __ldcg(a.stat_d + stat_at + N * ty + i));
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < N; ++j) {
             const bool in = k0 + tx + 16 * j < len && st.x != -CUDART_INF_F;
             const float p = in ? exp2f(s[i][j] * a.scale * CUDART_L2E_F + st.x) : 0.0f;
-            const int at = (2 * ty + i) * (AS_T + 1) + tx + 16 * j;
+            const int at = (N * ty + i) * (T + 1) + tx + 16 * j;
             P[at] = p;
             S[at] = in ? p * (dp[i][j] + st.y) : 0.0f;
         }
@@ -536,32 +549,32 @@ __device__ __forceinline__ void as_grad_tile(const AttnArgs &a, const float *Q, 
 }
 
 // dK and dV of a tile of keys: all query tiles of all heads that share it.
-template <int DT, int DP>
+template <int DT, int DP, int T>
 __device__ __forceinline__ void as_dkdv(const AttnArgs &a, float *sm, unsigned block) {
-    constexpr int T = AS_T * (DP + 4);
-    float *K = sm, *V = K + T, *Q = V + T, *G = Q + T, *P = G + T, *S = P + AS_T * (AS_T + 1);
+    constexpr int N = T / 16, Z = T * (DP + 4);
+    float *K = sm, *V = K + Z, *Q = V + Z, *G = Q + Z, *P = G + Z, *S = P + T * (T + 1);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int tiles = (a.Sk + AS_T - 1) / AS_T, bh = (int)(block / tiles);
-    const int k0 = (int)(block % tiles) * AS_T, b = bh / a.HK, hk = bh % a.HK, group = a.H / a.HK;
+    const int tiles = (a.Sk + T - 1) / T, bh = (int)(block / tiles);
+    const int k0 = (int)(block % tiles) * T, b = bh / a.HK, hk = bh % a.HK, group = a.H / a.HK;
     const int len = attn_keys(a, b);
-    as_load<DT, DP>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], len - k0, a.D);
-    as_load<DT, DP>(V, a.v, b * a.vs[0] + k0 * a.vs[1] + hk * a.vs[2], a.vs[1], len - k0, a.D);
-    float dk[2][DP / 64][4] = {}, dv[2][DP / 64][4] = {};
+    as_load<DT, DP, T>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], len - k0, a.D);
+    as_load<DT, DP, T>(V, a.v, b * a.vs[0] + k0 * a.vs[1] + hk * a.vs[2], a.vs[1], len - k0, a.D);
+    float dk[N][DP / 64][4] = {}, dv[N][DP / 64][4] = {};
     for (int h = hk * group; h < (hk + 1) * group && k0 < len; ++h)
-        for (int q0 = 0; q0 < a.Sq; q0 += AS_T) {
+        for (int q0 = 0; q0 < a.Sq; q0 += T) {
             __syncthreads();
-            as_load<DT, DP>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
-            as_load<DT, DP>(G, a.dout, (((long long)b * a.Sq + q0) * a.H + h) * a.D, (long long)a.H * a.D, a.Sq - q0,
+            as_load<DT, DP, T>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
+            as_load<DT, DP, T>(G, a.dout, (((long long)b * a.Sq + q0) * a.H + h) * a.D, (long long)a.H * a.D, a.Sq - q0,
                             a.D);
             __syncthreads();
-            as_grad_tile<DP>(a, Q, K, V, G, P, S, ((long long)b * a.H + h) * a.Sqp + q0, k0, len, ty, tx);
+            as_grad_tile<DP, T>(a, Q, K, V, G, P, S, ((long long)b * a.H + h) * a.Sqp + q0, k0, len, ty, tx);
             __syncthreads();
-            as_mix<DP>(P, 1, AS_T + 1, G, ty, tx, dv);
-            as_mix<DP>(S, 1, AS_T + 1, Q, ty, tx, dk);
+            as_mix<DP, N>(P, 1, T + 1, G, ty, tx, dv);
+            as_mix<DP, N>(S, 1, T + 1, Q, ty, tx, dk);
         }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int t = k0 + 2 * ty + i;
+    for (int i = 0; i < N; ++i) {
+        const int t = k0 + N * ty + i;
         if (t >= a.Sk) continue;
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c)
@@ -577,29 +590,29 @@ __device__ __forceinline__ void as_dkdv(const AttnArgs &a, float *sm, unsigned b
 }
 
 // dQ of a tile of queries.
-template <int DT, int DP>
+template <int DT, int DP, int T>
 __device__ __forceinline__ void as_dq(const AttnArgs &a, float *sm, unsigned block) {
-    constexpr int T = AS_T * (DP + 4);
-    float *K = sm, *V = K + T, *Q = V + T, *G = Q + T, *P = G + T, *S = P + AS_T * (AS_T + 1);
+    constexpr int N = T / 16, Z = T * (DP + 4);
+    float *K = sm, *V = K + Z, *Q = V + Z, *G = Q + Z, *P = G + Z, *S = P + T * (T + 1);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int tiles = (a.Sq + AS_T - 1) / AS_T, bh = (int)(block / tiles);
-    const int q0 = (int)(block % tiles) * AS_T, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.HK);
+    const int tiles = (a.Sq + T - 1) / T, bh = (int)(block / tiles);
+    const int q0 = (int)(block % tiles) * T, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.HK);
     const int len = attn_keys(a, b);
-    as_load<DT, DP>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
-    as_load<DT, DP>(G, a.dout, (((long long)b * a.Sq + q0) * a.H + h) * a.D, (long long)a.H * a.D, a.Sq - q0, a.D);
-    float dq[2][DP / 64][4] = {};
-    for (int k0 = 0; k0 < len; k0 += AS_T) {
+    as_load<DT, DP, T>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
+    as_load<DT, DP, T>(G, a.dout, (((long long)b * a.Sq + q0) * a.H + h) * a.D, (long long)a.H * a.D, a.Sq - q0, a.D);
+    float dq[N][DP / 64][4] = {};
+    for (int k0 = 0; k0 < len; k0 += T) {
         __syncthreads();
-        as_load<DT, DP>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], len - k0, a.D);
-        as_load<DT, DP>(V, a.v, b * a.vs[0] + k0 * a.vs[1] + hk * a.vs[2], a.vs[1], len - k0, a.D);
+        as_load<DT, DP, T>(K, a.k, b * a.ks[0] + k0 * a.ks[1] + hk * a.ks[2], a.ks[1], len - k0, a.D);
+        as_load<DT, DP, T>(V, a.v, b * a.vs[0] + k0 * a.vs[1] + hk * a.vs[2], a.vs[1], len - k0, a.D);
         __syncthreads();
-        as_grad_tile<DP>(a, Q, K, V, G, P, S, ((long long)b * a.H + h) * a.Sqp + q0, k0, len, ty, tx);
+        as_grad_tile<DP, T>(a, Q, K, V, G, P, S, ((long long)b * a.H + h) * a.Sqp + q0, k0, len, ty, tx);
         __syncwarp();  // the rows of S that a warp reads are its own
-        as_mix<DP>(S, AS_T + 1, 1, K, ty, tx, dq);
+        as_mix<DP, N>(S, T + 1, 1, K, ty, tx, dq);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int t = q0 + 2 * ty + i;
+    for (int i = 0; i < N; ++i) {
+        const int t = q0 + N * ty + i;
         if (t >= a.Sq) continue;
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c)
@@ -613,13 +626,13 @@ __device__ __forceinline__ void as_dq(const AttnArgs &a, float *sm, unsigned blo
 }
 
 // grid: key tiles * B * HK blocks for dK and dV, then query tiles * B * H for dQ
-template <int DT, int DP>
+template <int DT, int DP, int T>
 __global__ void __launch_bounds__(AS_THREADS) attn_simt_bwd_kernel(const AttnArgs a) {
     extern __shared__ float sm[];
     griddep_wait();
-    const unsigned first = (unsigned)((a.Sk + AS_T - 1) / AS_T) * a.B * a.HK;
-    if (blockIdx.x < first) as_dkdv<DT, DP>(a, sm, blockIdx.x);
-    else as_dq<DT, DP>(a, sm, blockIdx.x - first);
+    const unsigned first = (unsigned)((a.Sk + T - 1) / T) * a.B * a.HK;
+    if (blockIdx.x < first) as_dkdv<DT, DP, T>(a, sm, blockIdx.x);
+    else as_dq<DT, DP, T>(a, sm, blockIdx.x - first);
 }
 
 }  // namespace reels

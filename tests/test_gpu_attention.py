@@ -44,6 +44,9 @@ CASES = [
     (1, 40, 50, 1, 1, 256, FL, None, False),
     (1, 5, 3000, 1, 1, 64, FL, None, False),      # key splits on the CUDA cores
     (1, 50, 50, 3, 3, 64, FL, None, True),
+    (2, 130, 200, 60, 30, 64, FL, [200, 7], False),  # the larger tile on the CUDA cores
+    (1, 70, 65, 200, 200, 100, FL, None, False),
+    (1, 190, 90, 100, 100, 36, HF, None, False),
 ]
 
 
