@@ -30,6 +30,23 @@ def _stream(device) -> int:
 
 
 # ------------------------------------------------------ norm and rotation
+_ROPE_AXES = {}  # (sizes, dims, interleaved) -> table entries, head_dim, the C arrays
+
+
+def _rope_axes(sizes, dims, interleaved):
+    sizes, dims = [int(s) for s in sizes], [int(d) for d in dims]
+    if len(sizes) != len(dims) or not 1 <= len(sizes) <= 3:
+        raise ValueError("a rotary table has one to three axes, each with a size and a number of features")
+    if min(sizes) <= 0 or min(dims) < 0 or any(d % 2 for d in dims):
+        raise ValueError("a rotary axis needs a positive size and an even number of features")
+    # fewer axes: the missing outer ones have one position and no features
+    pad = 3 - len(sizes)
+    i3 = ctypes.c_int32 * 3
+    args = (i3(*([1] * pad), *sizes), i3(*([0] * pad), *dims),
+            nat.ROPE_INTERLEAVED if interleaved else nat.ROPE_HALF)
+    return sum(s * d // 2 for s, d in zip(sizes, dims)), sum(dims), args
+
+
 class RopeTable:
     """Rotary positions of a video: ``table`` (entries, 2) holds (cos, sin) of
     the angles, axis after axis (time, height, width) as
@@ -39,27 +56,21 @@ class RopeTable:
     (i, i + head_dim / 2).  Build one with :func:`rope_table` and keep it for
     all blocks and steps of a resolution."""
 
-    __slots__ = ("table", "sizes", "dims", "interleaved", "_args")
+    __slots__ = ("table", "sizes", "dims", "interleaved", "head_dim", "_args")
 
     def __init__(self, table: torch.Tensor, sizes: Sequence[int], dims: Sequence[int], interleaved: bool = True):
-        sizes, dims = tuple(int(s) for s in sizes), tuple(int(d) for d in dims)
-        if len(sizes) != len(dims) or not 1 <= len(sizes) <= 3:
-            raise ValueError("a rotary table has one to three axes, each with a size and a number of features")
-        if min(sizes) <= 0 or min(dims) < 0 or any(d % 2 for d in dims):
-            raise ValueError("a rotary axis needs a positive size and an even number of features")
-        entries = sum(s * d // 2 for s, d in zip(sizes, dims))
-        if table.dtype != torch.float32 or tuple(table.shape) != (entries, 2) or not table.is_contiguous():
+        key = (tuple(sizes), tuple(dims), bool(interleaved))
+        known = _ROPE_AXES.get(key)
+        if known is None:
+            known = _rope_axes(*key)
+            if len(_ROPE_AXES) >= 4096:
+                _ROPE_AXES.clear()
+            _ROPE_AXES[key] = known
+        self.sizes, self.dims, self.interleaved = key
+        entries, self.head_dim, self._args = known
+        if table.dtype != torch.float32 or table.shape != (entries, 2) or not table.is_contiguous():
             raise ValueError(f"the rotary table must be contiguous fp32 of shape ({entries}, 2)")
-        # fewer axes: the missing outer ones have one position and no features
-        self.table, self.sizes, self.dims, self.interleaved = table, sizes, dims, bool(interleaved)
-        pad = 3 - len(sizes)
-        i3 = ctypes.c_int32 * 3
-        self._args = (i3(*([1] * pad), *sizes), i3(*([0] * pad), *dims),
-                      nat.ROPE_INTERLEAVED if interleaved else nat.ROPE_HALF)
-
-    @property
-    def head_dim(self) -> int:
-        return sum(self.dims)
+        self.table = table
 
 
 def rope_table(head_dim: int, sizes: Sequence[int], dims: Optional[Sequence[int]] = None, base: float = 10000.0,

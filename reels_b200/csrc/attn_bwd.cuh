@@ -42,28 +42,6 @@ __device__ __forceinline__ int attn_grad_exp(const AttnArgs &a) {
     return 13 - ilogbf(top);
 }
 
-// 32 accumulator columns of this thread's row, times f, to dst (features c0 ..): 16-bit or fp32.
-template <int DT>
-__device__ __forceinline__ void ab_store32(const uint32_t (&o)[32], float f, typename Elem<DT>::T *dst, float *part,
-                                           int c0, int D) {
-#pragma unroll
-    for (int e = 0; e < 32; e += 8) {
-        if (c0 + e >= D) continue;
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[e + k]) * f;
-        if (part) {
-            float4 *p = reinterpret_cast<float4 *>(part + c0 + e);
-            p[0] = make_float4(v[0], v[1], v[2], v[3]);
-            p[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            *reinterpret_cast<uint4 *>(dst + c0 + e) =
-                make_uint4(Elem<DT>::pack2(v[0], v[1]), Elem<DT>::pack2(v[2], v[3]), Elem<DT>::pack2(v[4], v[5]),
-                           Elem<DT>::pack2(v[6], v[7]));
-        }
-    }
-}
-
 // ------------------------------------------------------------ dK and dV
 // Unit: a tile of 128 keys of one key head and a range of the walk over the
 // query tiles of the heads that share it.  Everything is computed transposed
@@ -337,6 +315,7 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap &tmQ, const CUtensor
                               ? (half ? a.part_k : a.part_v) + (long long)w.split * a.B * a.Sk * a.HK * a.D + at
                               : nullptr;
             auto *dst = reinterpret_cast<typename Elem<DT>::T *>(half ? a.dk : a.dv) + at;
+            const bool sectors = at_sectors(half ? a.dk : a.dv, a.D);
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) {
                 uint32_t o[32];
@@ -353,7 +332,7 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap &tmQ, const CUtensor
 #pragma unroll
                     for (int k = 0; k < 32; ++k) o[k] = 0u;
                 }
-                if (t < a.Sk) ab_store32<DT>(o, f, dst, part, 32 * i, a.D);
+                if (t < a.Sk) at_store32<DT>(o, f, dst, part, 32 * i, a.D, sectors);
                 __syncwarp();
             }
         }
@@ -656,25 +635,26 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap &tmQ, const CUtensorMa
             // the two groups of warps write half of the features each
             auto *dst = reinterpret_cast<typename Elem<DT>::T *>(a.dq) +
                         (((long long)w.b * a.Sq + row) * a.H + w.h) * a.D;
+            const bool sectors = at_sectors(a.dq, a.D);
+            const int c0 = half * (DP / 2);
+            uint32_t o[DP / 2];
+            if (w.nk > 0) {
 #pragma unroll
-            for (int i = 0; i < DP / 64; ++i) {
-                const int c0 = half * (DP / 2) + 32 * i;
-                uint32_t o[32];
-                if (w.nk > 0) {
-                    at_tmem_ld32(O + c0, o);
-                    tmem_wait_ld();
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = 0u;
-                }
-                if (i == DP / 64 - 1 && w.nk > 0) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(acc_empty);
-                }
-                if (row < a.Sq) ab_store32<DT>(o, f, dst, nullptr, c0, a.D);
+                for (int i = 0; i < DP / 64; ++i) at_tmem_ld32(O + c0 + 32 * i, o + 32 * i);
+                tmem_wait_ld();
+                tc_fence_before();
                 __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty);
+            } else {
+#pragma unroll
+                for (int k = 0; k < DP / 2; ++k) o[k] = 0u;
             }
+            if (row < a.Sq) {
+#pragma unroll
+                for (int i = 0; i < DP / 64; ++i)
+                    at_store32<DT>(o + 32 * i, f, dst, nullptr, c0 + 32 * i, a.D, sectors);
+            }
+            __syncwarp();
         }
     }
 

@@ -131,6 +131,42 @@ struct AtRegisters {
     static __device__ __forceinline__ void fewer() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEWER)); }
 };
 
+// 32 fp32 values of this thread's row times f, as 16-bit values at dst + c0 up
+// to feature D, in whole 32-byte sectors where alignment allows (a warp writes
+// 32 rows at once: half the requests), or as they are at part + c0.
+template <int DT>
+__device__ __forceinline__ void at_store32(const uint32_t *o, float f, typename Elem<DT>::T *dst, float *part, int c0,
+                                           int D, bool sectors) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 16) {
+        if (c0 + e >= D) continue;
+        F2 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = mul2(at_pair(o, e / 2 + k), F2(f, f));
+        if (part) {
+#pragma unroll
+            for (int k = 0; k < 8; k += 2)
+                if (c0 + e + 2 * k < D) {
+                    const float2 x = v[k].get(), y = v[k + 1].get();
+                    *reinterpret_cast<float4 *>(part + c0 + e + 2 * k) = make_float4(x.x, x.y, y.x, y.y);
+                }
+            continue;
+        }
+        const uint4 lo = make_uint4(at_pack<DT>(v[0]), at_pack<DT>(v[1]), at_pack<DT>(v[2]), at_pack<DT>(v[3]));
+        const uint4 hi = make_uint4(at_pack<DT>(v[4]), at_pack<DT>(v[5]), at_pack<DT>(v[6]), at_pack<DT>(v[7]));
+        if (sectors) {
+            st_global_v8(dst + c0 + e, lo, hi);
+        } else {
+            *reinterpret_cast<uint4 *>(dst + c0 + e) = lo;
+            if (c0 + e + 8 < D) *reinterpret_cast<uint4 *>(dst + c0 + e + 8) = hi;
+        }
+    }
+}
+// Whether rows of D 16-bit features from `p` on are whole 32-byte sectors.
+__device__ __forceinline__ bool at_sectors(const void *p, int D) {
+    return ((reinterpret_cast<uintptr_t>(p) & 31) | (D & 15)) == 0;
+}
+
 // A wait of a whole warp on one barrier.
 __device__ __forceinline__ bool at_wait(uint64_t *bar, uint32_t parity, volatile int *abort, unsigned *err,
                                         unsigned code) {

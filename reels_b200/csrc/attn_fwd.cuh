@@ -261,6 +261,7 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
         const uint32_t S = tmem + t * 128 + lanes, O = tmem + 256 + t * 128 + lanes;
         const float c = a.scale * CUDART_L2E_F;
         const F2 c2 = F2(c, c);
+        const bool sectors = at_sectors(a.out, a.D);
         uint32_t ns = 0, nu = 0;
         bool good = true;
         for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
@@ -348,40 +349,25 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
             }
             typename Elem<DT>::T *out = reinterpret_cast<typename Elem<DT>::T *>(a.out) +
                                         (((long long)w.b * a.Sq + row) * a.H + w.h) * a.D;
-            float *part = a.part_o + (at * a.Sq + row) * a.D;
+            float *part = a.splits > 1 ? a.part_o + (at * a.Sq + row) * a.D : nullptr;
+            uint32_t o[DP];
+            if (w.nk > 0) {
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                uint32_t o[32];
-                if (w.nk > 0) {
-                    at_tmem_ld32(O + 32 * i, o);
-                    tmem_wait_ld();
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0u;
-                }
-                if (i == DP / 32 - 1 && w.nk > 0) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&o_empty[t]);
-                }
-#pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    if (!in || 32 * i + e >= a.D) continue;
-                    float v[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(o[e + k]) * inv;
-                    if (a.splits > 1) {
-                        float4 *dst = reinterpret_cast<float4 *>(part + 32 * i + e);
-                        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-                        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-                    } else {
-                        *reinterpret_cast<uint4 *>(out + 32 * i + e) =
-                            make_uint4(Elem<DT>::pack2(v[0], v[1]), Elem<DT>::pack2(v[2], v[3]),
-                                       Elem<DT>::pack2(v[4], v[5]), Elem<DT>::pack2(v[6], v[7]));
-                    }
-                }
+                for (int i = 0; i < DP / 32; ++i) at_tmem_ld32(O + 32 * i, o + 32 * i);
+                tmem_wait_ld();
+                tc_fence_before();
                 __syncwarp();
+                if (lane == 0) mbar_arrive(&o_empty[t]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < DP; ++e) o[e] = 0u;
             }
+            if (in) {
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i)
+                    at_store32<DT>(o + 32 * i, inv, out, part, 32 * i, a.D, sectors);
+            }
+            __syncwarp();
         }
     }
 
