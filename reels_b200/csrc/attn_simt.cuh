@@ -442,23 +442,27 @@ __device__ __forceinline__ void as_rows(const void *x, const void *y, long long 
                 }
             }
         }
+        float mine = 0.0f;  // lane i of the group keeps row i's product
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            float dot = 0.0f, n2 = 0.0f;
+            F2 g[4], h[4], d2 = F2(0.0f, 0.0f), n2 = F2(0.0f, 0.0f);
+            read8<DT>(reinterpret_cast<const T *>(&u[i]), g);
+            if (y) read8<DT>(reinterpret_cast<const T *>(&v[i]), h);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float g = load_act(&u[i], j, DT);
-                if (y) dot += g * load_act(&v[i], j, DT);
-                if (DT == DT_F16) n2 += g * g;
+            for (int j = 0; j < 4; ++j) {
+                if (y) d2 = fma2(g[j], h[j], d2);
+                if (DT == DT_F16) n2 = fma2(g[j], g[j], n2);
             }
+            float dot = d2.get().x + d2.get().y, norm = n2.get().x + n2.get().y;
 #pragma unroll
             for (int w = G / 2; w > 0; w >>= 1) {
                 if (y) dot += __shfl_xor_sync(0xffffffffu, dot, w);
-                if (DT == DT_F16) n2 += __shfl_xor_sync(0xffffffffu, n2, w);
+                if (DT == DT_F16) norm += __shfl_xor_sync(0xffffffffu, norm, w);
             }
-            top = fmaxf(top, n2);
-            if (sub == 0 && r0 + i < rows) use(r0 + i, dot);
+            top = fmaxf(top, norm);
+            if (sub == i) mine = dot;
         }
+        if (y && sub < R && r0 + sub < rows) use(r0 + sub, mine);
     }
 }
 

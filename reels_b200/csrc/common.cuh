@@ -101,6 +101,27 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
     return r;
 }
 
+// Eight consecutive elements, from memory to four packed pairs.
+template <int DT>
+__device__ __forceinline__ void read8(const typename Elem<DT>::T *p, F2 (&v)[4]) {
+    if constexpr (DT == DT_F32) {
+        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+        v[0] = F2(a.x, a.y), v[1] = F2(a.z, a.w), v[2] = F2(b.x, b.y), v[3] = F2(b.z, b.w);
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == DT_BF16)
+                v[j] = F2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+            else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+                v[j] = F2(f.x, f.y);
+            }
+        }
+    }
+}
+
 // ------------------------------------------------------------------ PTX
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));

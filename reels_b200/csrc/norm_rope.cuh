@@ -103,33 +103,13 @@ __device__ __forceinline__ int nr_axis(const NormRopeArgs &a, int i, int &base) 
     return 2;
 }
 
-// Eight consecutive elements, from memory to four packed pairs and back.
-template <int DT>
-__device__ __forceinline__ void nr_read(const typename Elem<DT>::T *p, F2 (&v)[4]) {
-    if constexpr (DT == DT_F32) {
-        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-        v[0] = F2(a.x, a.y), v[1] = F2(a.z, a.w), v[2] = F2(b.x, b.y), v[3] = F2(b.z, b.w);
-    } else {
-        const uint4 a = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (DT == DT_BF16)
-                v[j] = F2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
-            else {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
-                v[j] = F2(f.x, f.y);
-            }
-        }
-    }
-}
 template <int DT>
 __device__ __forceinline__ void nr_read_global(const typename Elem<DT>::T *p, F2 (&v)[4]) {
     __align__(16) typename Elem<DT>::T t[8];
 #pragma unroll
     for (int j = 0; j < (int)sizeof(t) / 16; ++j)
         reinterpret_cast<uint4 *>(t)[j] = __ldcg(reinterpret_cast<const uint4 *>(p) + j);
-    nr_read<DT>(t, v);
+    read8<DT>(t, v);
 }
 template <int DT>
 __device__ __forceinline__ void nr_write(typename Elem<DT>::T *p, const F2 (&v)[4]) {
@@ -248,8 +228,8 @@ __global__ void __launch_bounds__(UPT == 1 ? 512 : 256, UPT == 1 ? 2 : UPT == 2 
     for (int k = 0; k < UPT; ++k) feat[k] = ((int)threadIdx.x + k * (int)blockDim.x) / uph * a.D + i0;
     auto owned = [&](int k) { return (int)threadIdx.x + k * (int)blockDim.x < upr; };
     auto read = [&](const T *from, int k, F2 (&lo)[4], F2 (&hi)[4]) {
-        nr_read<DT>(from + feat[k], lo);
-        nr_read<DT>(from + feat[k] + a.D / 2, hi);
+        read8<DT>(from + feat[k], lo);
+        read8<DT>(from + feat[k] + a.D / 2, hi);
     };
     auto weigh = [&](int k, F2 (&lo)[4], F2 (&hi)[4]) {
         F2 wl[4], wh[4];
