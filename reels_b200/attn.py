@@ -15,6 +15,7 @@ import ctypes
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 from .lowvram import _check_numel, _dt, _ptr, _require_cuda
@@ -188,6 +189,7 @@ class RMSNormRopeFunction(torch.autograd.Function):
         return rms_norm_rope(x, heads, weight, rope, epsilon, tokens_per_sample, positions)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         x, weight, positions = ctx.saved_tensors
         heads, rope, epsilon, tps = ctx.args
@@ -330,6 +332,7 @@ class AttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, kv_lengths = ctx.saved_tensors
         return (*attention_backward(dout, q, k, v, out, lse, ctx.scale, kv_lengths), None, None)

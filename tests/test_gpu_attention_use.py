@@ -321,3 +321,15 @@ def test_current_device_is_kept_and_the_c_calls_take_any_stream(torch, reels):
         out.data_ptr(), l2.data_ptr(), None, 0, s.cuda_stream))
     s.synchronize()
     assert torch.cuda.current_device() == 0 and torch.equal(out, want) and torch.equal(l2, lse)
+
+
+def test_a_second_derivative_is_refused(torch, reels):
+    """The gradients carry no graph of their own: differentiating them raises."""
+    q, k, v = (torch.randn((1, 8, 2, 64), device="cuda", requires_grad=True) for _ in range(3))
+    dq, = torch.autograd.grad(reels.AttentionFunction.apply(q, k, v).square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dq.sum().backward()
+    x = torch.randn((4, 128), device="cuda", requires_grad=True)
+    dx, = torch.autograd.grad(reels.RMSNormRopeFunction.apply(x, 2).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
