@@ -3,6 +3,7 @@
 // softmax attention and its gradient (attn_fwd.cuh, attn_bwd.cuh,
 // attn_simt.cuh), behind the C ABI of include/reels_lowvram.h.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <mutex>
 #include <type_traits>
@@ -69,7 +70,7 @@ int check_norm_rope(const void *x, int64_t M, int64_t heads, int64_t D, const re
 constexpr int kNormRopeSmem = 220 * 1024;  // of an SM's 228 KB, 1 KB a block is the system's
 
 template <int DT, bool BWD, bool ROPE, bool HALF, int UPT>
-cudaError_t launch_norm_rope(const NormRopeArgs &a, int threads, int sms, cudaStream_t st) {
+cudaError_t launch_norm_rope(const NormRopeArgs &a, int threads, const HostCall &call, cudaStream_t st) {
     // Blocks that fit beside each other with a ring of at least two rows, then
     // as many rows as the shared memory holds.
     const int budget = kNormRopeSmem, fixed = nr_smem_bytes(a.C, bytes_of(DT), BWD, 0, a.D) + 1024;
@@ -78,11 +79,14 @@ cudaError_t launch_norm_rope(const NormRopeArgs &a, int threads, int sms, cudaSt
     const int stages = std::max(2, std::min(NR_STAGES, (budget / blocks - fixed) / step));  // (two rows were checked to fit)
     const int smem = nr_smem_bytes(a.C, bytes_of(DT), BWD, stages, a.D);
     auto kern = norm_rope_kernel<DT, BWD, ROPE, HALF, UPT>;
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // the most any call asks for, once per device: calls of several threads agree on it
+    static std::atomic<uint64_t> ready{0};
+    if (!(ready.load() >> call.device & 1)) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormRopeSmem);
         if (e != cudaSuccess) return e;
+        ready.fetch_or(uint64_t(1) << call.device);
     }
-    const dim3 grid((unsigned)std::min<int64_t>(a.M, (int64_t)sms * blocks));
+    const dim3 grid((unsigned)std::min<int64_t>(a.M, (int64_t)call.sms * blocks));
     return host_launch_pdl(kern, grid, dim3((unsigned)threads), smem, st, a, stages);
 }
 
@@ -130,16 +134,16 @@ int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t head
     // angles, waits and sums are shared); backward one, whose registers leave
     // room for twice the warps: 8190 x 5120 forward 31 us with two and 37 with
     // one, backward 54 and 49.
-    const int upt = units > 2 * 256 ? (bwd && units <= NR_THREADS ? 1 : 4) : bwd || units <= 32 ? 1 : 2;
+    const int upt = units > 512 ? 4 : bwd || units <= 32 ? 1 : 2;
     const int threads = (int)ceil_div(std::max<int64_t>(ceil_div(units, upt), rope ? D / 2 : 1), 32) * 32;
     cudaError_t e = cudaSuccess;
     with_dtype(dt, [&](auto t) {
         constexpr int DT = decltype(t)::value;
         auto form = [&](auto b, auto r, auto h) {
             constexpr bool B = decltype(b)::value, R = decltype(r)::value, H = decltype(h)::value;
-            e = upt == 1   ? launch_norm_rope<DT, B, R, H, 1>(a, threads, call.sms, st)
-                : upt == 2 ? launch_norm_rope<DT, B, R, H, 2>(a, threads, call.sms, st)
-                           : launch_norm_rope<DT, B, R, H, 4>(a, threads, call.sms, st);
+            e = upt == 1   ? launch_norm_rope<DT, B, R, H, 1>(a, threads, call, st)
+                : upt == 2 ? launch_norm_rope<DT, B, R, H, 2>(a, threads, call, st)
+                           : launch_norm_rope<DT, B, R, H, 4>(a, threads, call, st);
         };
         auto dir = [&](auto b) {
             if (!rope) form(b, std::false_type{}, std::false_type{});

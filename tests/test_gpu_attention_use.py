@@ -333,3 +333,33 @@ def test_a_second_derivative_is_refused(torch, reels):
     dx, = torch.autograd.grad(reels.RMSNormRopeFunction.apply(x, 2).square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dx.sum().backward()
+
+
+def test_calls_of_several_threads(torch, reels):
+    """Two widths of one kernel's form, whose launches need different amounts
+    of shared memory, from two threads at once: the results of the calls made alone."""
+    import threading
+    xs = [torch.randn((64, c), device="cuda").bfloat16() for c in (1536, 5120)]
+    douts = [torch.randn_like(x) for x in xs]
+    run = lambda i: (reels.rms_norm_rope(xs[i], 12 if i == 0 else 40),
+                     reels.rms_norm_rope_backward(xs[i], douts[i], 12 if i == 0 else 40))
+    want, bad = [run(0), run(1)], []
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(300):
+                    got = run(i)
+                torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                bad.append((i, "differs"))
+        except Exception as e:  # reported below, by the test's own thread
+            bad.append((i, e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
