@@ -133,7 +133,9 @@ int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t head
     // Units a thread, and a thread for each pair of a head.  Forward, two (the
     // angles, waits and sums are shared); backward one, whose registers leave
     // room for twice the warps: 8190 x 5120 forward 31 us with two and 37 with
-    // one, backward 54 and 49.
+    // one, backward 54 and 49.  Forward rows of up to 512 features fill no more
+    // than a warp with one.  Past 512 units (8192 features) neither fits a
+    // block: four.
     const int upt = units > 512 ? 4 : bwd || units <= 32 ? 1 : 2;
     const int threads = (int)ceil_div(std::max<int64_t>(ceil_div(units, upt), rope ? D / 2 : 1), 32) * 32;
     cudaError_t e = cudaSuccess;
@@ -217,8 +219,8 @@ AttnPlan plan_attention(const reels_attn_shape &s, int dt, const void *q, const 
     const int64_t per = ceil_div(tiles, want);
     p.splits = (int)ceil_div(tiles, per);
     p.split_keys = (int)std::min<int64_t>(per * tile, INT32_MAX - 256);
-    // Backward: one launch of the dK, dV walks and then the dQ walks, 1.9 and
-    // 1.35 us a step.  The first are split where a whole one would outlast the
+    // Backward: one launch of the dK, dV walks and then the dQ walks, about 1.9
+    // and 1.35 us a step of 128 features (only their ratio to the ends counts).  The first are split where a whole one would outlast the
     // average SM: the launch ends about half a unit behind the average, and the
     // partial sums pass through memory twice (about 5 TB/s) and a launch.
     if (p.tc && s.q_tokens > 0 && s.k_tokens > 0) {
@@ -571,10 +573,11 @@ int reels_attention_backward(const reels_attn_shape *shape, const void *q, const
     n.kv = k_tiles * s.batch * s.kv_heads * plan.red_splits;
     n.q = q_tiles * s.batch * s.heads;
     // A block's start and end take some 3 us.  With many units of each kind a
-    // block stays on its SM and the walks are launched one after the other (2 x
-    // 6144 tokens, 32 heads: 3160 us; together, in blocks of two units, 3274);
-    // with few, blocks of about 32 steps of both let the SMs even out (8190
-    // queries over 512 keys, 40 heads: 352 us together, 381 one by one).
+    // block stays on its SM and the walks are launched one after the other (both
+    // ways measured at 2 x 6144 tokens, 32 heads: 3160 us, against 3274 together
+    // in blocks of two units); with few, blocks of about 32 steps of both let
+    // the SMs even out (8190 queries over 512 keys, 40 heads: 352 us together,
+    // 381 one by one).
     const bool apart = std::min(n.kv, n.q) >= 8ll * call.sms;
     const int64_t fill = ceil_div(n.kv + n.q, call.sms);
     auto blocks_of = [&](int64_t units, int64_t steps) {

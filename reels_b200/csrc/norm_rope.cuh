@@ -11,7 +11,11 @@
 // whose two sums (x^2 and h x) come from the same pass over x and dout.
 // All arithmetic is fp32, each output is rounded once.
 //
-// Bound: HBM, 2 passes of the row forward (x, y), 3 backward (x, dout, dx).
+// Bound: HBM, 2 passes of the row forward (x, y), 3 backward (x, dout, dx),
+// with issue slots next to it on short rows.  Measured, bf16: 32760 x 1536
+// forward 44 us (4.6 TB/s), 8190 x 5120 forward 32.5 us (5.2 TB/s) and backward
+// 48.6 (5.2); fp16, 12288 x 4096: 38.8 us (5.2) and 61.9 (4.9).  A copy runs at
+// 6.5 TB/s.
 #pragma once
 #include "common.cuh"
 
@@ -372,7 +376,8 @@ __global__ void __launch_bounds__(UPT == 1 ? 512 : 256, UPT == 1 ? 2 : UPT == 2 
 }
 
 // Any width, alignment and head size: one block of 256 threads a row, scalar
-// accesses, the row read a second time (from L1/L2) for the result.
+// accesses, the row read a second time (from L1/L2) for the result.  For what
+// the vector form cannot take; not tuned.
 template <int DT, bool BWD>
 __global__ void __launch_bounds__(256) norm_rope_any_kernel(const NormRopeArgs a) {
     __shared__ float2 buf[2][8];
