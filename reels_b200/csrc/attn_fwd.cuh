@@ -55,16 +55,20 @@ struct AttnUnit {
 };
 
 // Unit u: query tile pairs fastest, so that neighbouring CTAs read the same keys.
-__device__ __forceinline__ AttnUnit attn_unit(const AttnArgs &a, long long u) {
-    const int pairs = (a.Sq + 2 * AT_TILE - 1) / (2 * AT_TILE);
+// Each role decodes a unit while it ends the one before, so that no unit begins
+// with the divisions and the load of its length (32760 queries over 384 keys, 12
+// heads: 111 to 106 us).
+__device__ __forceinline__ AttnUnit attn_unit(const AttnArgs &a, long long unit) {
+    const unsigned pairs = (unsigned)(a.Sq + 2 * AT_TILE - 1) / (2 * AT_TILE);
+    unsigned u = (unsigned)unit;  // the host keeps units below 2^31
     AttnUnit w;
     w.q0 = (int)(u % pairs) * 2 * AT_TILE;
     u /= pairs;
-    w.h = (int)(u % a.H);
-    u /= a.H;
-    w.b = (int)(u % a.B);
-    w.split = (int)(u / a.B);
-    w.hk = w.h / (a.H / a.HK);
+    w.h = (int)(u % (unsigned)a.H);
+    u /= (unsigned)a.H;
+    w.b = (int)(u % (unsigned)a.B);
+    w.split = (int)(u / (unsigned)a.B);
+    w.hk = (int)((unsigned)w.h / (unsigned)(a.H / a.HK));
     w.tiles = a.Sq - w.q0 > AT_TILE ? 2 : 1;
     const int len = attn_keys(a, w.b);
     w.k0 = min(len, w.split * a.split_keys);
@@ -130,8 +134,10 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
         AfRegisters::fewer();
         uint32_t g = 0, qn[2] = {0, 0}, nraw = 0;
         bool good = true;
+        AttnUnit next = attn_unit(a, blockIdx.x);
         for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
-            const AttnUnit w = attn_unit(a, u);
+            const AttnUnit w = next;
+            next = attn_unit(a, min(u + gridDim.x, units - 1));
             if (w.nk == 0) continue;
             auto load_q = [&](int t) {
                 good = good && at_wait(&q_empty[t], (qn[t] & 1) ^ 1, abort, a.err, DEVERR_TIMEOUT_AB_EMPTY);
@@ -211,8 +217,10 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
             if (leader) mbar_arrive(&turn[t ^ 1]);
             ++nt;
         };
+        AttnUnit next = attn_unit(a, blockIdx.x);
         for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
-            const AttnUnit w = attn_unit(a, u);
+            const AttnUnit w = next;
+            next = attn_unit(a, min(u + gridDim.x, units - 1));
             if (w.nk == 0) continue;
             const bool two = w.tiles == 2;
             if (t >= w.tiles) {  // no second tile: only pass the ring on
@@ -273,9 +281,13 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
         const bool sectors = at_sectors(a.out, a.D);
         uint32_t ns = 0, nu = 0;
         bool good = true;
+        AttnUnit next = attn_unit(a, blockIdx.x);
         for (long long u = blockIdx.x; u < units && good; u += gridDim.x) {
-            const AttnUnit w = attn_unit(a, u);
-            if (t >= w.tiles) continue;
+            const AttnUnit w = next;
+            if (t >= w.tiles) {
+                next = attn_unit(a, min(u + gridDim.x, units - 1));
+                continue;
+            }
             const int row = w.q0 + t * AT_TILE + (warp & 3) * 32 + lane;
             float m = 0.0f, l = 0.0f;  // m: the maximum in use, in log2 units, less the fp16 shift
             for (int j = 0; j < w.nk; ++j) {
@@ -346,6 +358,7 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
                 l += total.x + total.y;
             }
             if (!good) break;
+            next = attn_unit(a, min(u + gridDim.x, units - 1));
             const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
             const float lse = w.nk > 0 ? (m + log2f(l)) * CUDART_LN2_F : -CUDART_INF_F;
             const long long at = ((long long)w.split * a.B + w.b) * a.H + w.h;
