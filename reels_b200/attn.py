@@ -180,10 +180,12 @@ def rms_norm_rope_backward(x: torch.Tensor, dout: torch.Tensor, heads: int, weig
 
 class RMSNormRopeFunction(torch.autograd.Function):
     """Autograd rule of :func:`rms_norm_rope`: a gradient for x (the norm's
-    weight is frozen)."""
+    weight is frozen; one that asks for a gradient is refused)."""
 
     @staticmethod
     def forward(ctx, x, heads, weight=None, rope=None, epsilon=1e-6, tokens_per_sample=None, positions=None):
+        if ctx.needs_input_grad[2]:
+            raise ValueError("the norm's weight is frozen and receives no gradient")
         ctx.save_for_backward(x, weight, positions)
         ctx.args = (heads, rope, epsilon, tokens_per_sample)
         return rms_norm_rope(x, heads, weight, rope, epsilon, tokens_per_sample, positions)

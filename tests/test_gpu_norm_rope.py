@@ -166,3 +166,14 @@ def test_in_place_and_unaligned(torch):
                                                     torch.cuda.current_stream().cuda_stream))
     # the two forms sum a row in different orders: one rounding apart at most
     assert float((x.float() - want.float()).abs().max()) <= 2.0 ** -8 * float(want.float().abs().max())
+
+
+def test_a_weight_that_asks_for_a_gradient_is_refused(torch):
+    from reels_b200 import RMSNormRopeFunction
+    x = torch.randn((4, 128), device="cuda", requires_grad=True)
+    w = torch.ones(128, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="frozen"):
+        RMSNormRopeFunction.apply(x, 2, w)
+    with torch.no_grad():
+        RMSNormRopeFunction.apply(x, 2, w)
+    RMSNormRopeFunction.apply(x, 2, w.detach()).sum().backward()
