@@ -129,7 +129,9 @@ def _norm_rope_args(x, heads, weight, rope, tokens_per_sample, positions):
                 raise ValueError("positions must be integers on the input's device")
             if positions.shape[-1] != axes or positions.numel() != M * axes:
                 raise ValueError(f"positions must have one row of {axes} for each of the {M} tokens")
-            pos = positions.reshape(M, axes).to(torch.int32)
+            pos = positions.reshape(M, axes)
+            if pos.dtype == torch.int64:  # what 32 bits do not hold stays outside every table
+                pos = pos.clamp(-1, 2 ** 31 - 1).to(torch.int32)
             if axes < 3:  # the missing outer axes stand at their only position
                 pos = torch.nn.functional.pad(pos, (3 - axes, 0))
             pos = pos.contiguous()

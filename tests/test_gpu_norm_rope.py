@@ -177,3 +177,18 @@ def test_a_weight_that_asks_for_a_gradient_is_refused(torch):
     with torch.no_grad():
         RMSNormRopeFunction.apply(x, 2, w)
     RMSNormRopeFunction.apply(x, 2, w.detach()).sum().backward()
+
+
+def test_positions_past_32_bits_do_not_wrap(torch):
+    from reels_b200 import check_device_status, rms_norm_rope, rope_table
+    from reels_b200._native import NativeError
+    rope = rope_table(64, (2, 2, 2))
+    x = torch.randn((1, 2, 128), device="cuda").bfloat16()
+    plain = rms_norm_rope(x, 2)
+    pos = torch.tensor([[[1, 1, -2 ** 32 + 1], [-2 ** 40, 0, 0]]], device="cuda")
+    assert torch.equal(rms_norm_rope(x, 2, None, rope, positions=pos), plain)
+    check_device_status()
+    pos = torch.tensor([[[1, 1, 2 ** 32 + 1], [2 ** 32, 1, 1]]], device="cuda")
+    assert torch.equal(rms_norm_rope(x, 2, None, rope, positions=pos), plain)
+    with pytest.raises(NativeError, match="position"):
+        check_device_status()
