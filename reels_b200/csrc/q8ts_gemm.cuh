@@ -1074,9 +1074,14 @@ __global__ void __launch_bounds__(TsGeom<BT, KB2, PAIR>::THREADS, 1)
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0 && rows_ok) {
-                    tma_store_2d(&tmO, st_tile, c.n0 + 32 * q, m_base);
-                    if (store_pre) tma_store_2d(&tmP, pre_tile, c.n0 + 32 * q, m_base);
+                if (lane == 0) {
+                    if (rows_ok) {
+                        tma_store_2d(&tmO, st_tile, c.n0 + 32 * q, m_base);
+                        if (store_pre) tma_store_2d(&tmP, pre_tile, c.n0 + 32 * q, m_base);
+                    }
+                    // One group a chunk, an empty one past the last token too: the
+                    // wait above counts groups as chunks.  Without it the second
+                    // chunk past the end wrote over a tile still being stored.
                     bulk_commit_group();
                 }
             }
