@@ -182,12 +182,10 @@ def rms_norm_rope_backward(x: torch.Tensor, dout: torch.Tensor, heads: int, weig
 
 class RMSNormRopeFunction(torch.autograd.Function):
     """Autograd rule of :func:`rms_norm_rope`: a gradient for x (the norm's
-    weight is frozen; one that asks for a gradient is refused)."""
+    weight is frozen: a backward pass that asks for its gradient raises)."""
 
     @staticmethod
     def forward(ctx, x, heads, weight=None, rope=None, epsilon=1e-6, tokens_per_sample=None, positions=None):
-        if ctx.needs_input_grad[2]:
-            raise ValueError("the norm's weight is frozen and receives no gradient")
         ctx.save_for_backward(x, weight, positions)
         ctx.args = (heads, rope, epsilon, tokens_per_sample)
         return rms_norm_rope(x, heads, weight, rope, epsilon, tokens_per_sample, positions)
@@ -195,6 +193,8 @@ class RMSNormRopeFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        if any(ctx.needs_input_grad[1:]):  # as long as the arguments that were given
+            raise ValueError("the norm's weight is frozen and receives no gradient")
         x, weight, positions = ctx.saved_tensors
         heads, rope, epsilon, tps = ctx.args
         dx = rms_norm_rope_backward(x, dout.contiguous(), heads, weight, rope, epsilon, tps, positions)

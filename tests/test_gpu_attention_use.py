@@ -363,3 +363,22 @@ def test_calls_of_several_threads(torch, reels):
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.parametrize("Sq,H,D,dtype,length", [(1, 1, 128, "bfloat16", None), (1, 1, 64, "float16", 9001),
+                                                 (2, 1, 128, "bfloat16", 70), (20, 1, 64, "float32", 12000)])
+def test_many_key_splits(torch, reels, Sq, H, D, dtype, length):
+    """More splits than a warp has lanes, some of them behind the sample's length."""
+    import ctypes
+    from reels_b200 import _native as nat
+    Sk = 20011
+    c = ac.Case(1, Sq, Sk, H, H, D, getattr(torch, dtype), None if length is None else [length], seed=17)
+    i3 = ctypes.c_int64 * 3
+    shape = nat.AttnShape(1, H, H, Sq, Sk, D, i3(*c.q.stride()[:3]), i3(*c.k.stride()[:3]), i3(*c.v.stride()[:3]))
+    info, types = (ctypes.c_int64 * 4)(), {"bfloat16": nat.BF16, "float16": nat.F16, "float32": nat.F32}
+    nat.check("plan", nat.lib().reels_attention_plan(ctypes.byref(shape), types[dtype], info))
+    assert info[1] > 32
+    out, lse = reels.attention(c.q, c.k, c.v, kv_lengths=c.lengths, return_lse=True)
+    want = ac.reference(c, backward=False)
+    ac.check("out", out, want["out"])
+    ac.check("lse", lse, want["lse"])

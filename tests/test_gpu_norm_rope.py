@@ -173,7 +173,7 @@ def test_a_weight_that_asks_for_a_gradient_is_refused(torch):
     x = torch.randn((4, 128), device="cuda", requires_grad=True)
     w = torch.ones(128, device="cuda", requires_grad=True)
     with pytest.raises(ValueError, match="frozen"):
-        RMSNormRopeFunction.apply(x, 2, w)
+        RMSNormRopeFunction.apply(x, 2, w).sum().backward()
     with torch.no_grad():
         RMSNormRopeFunction.apply(x, 2, w)
     RMSNormRopeFunction.apply(x, 2, w.detach()).sum().backward()
@@ -192,3 +192,18 @@ def test_positions_past_32_bits_do_not_wrap(torch):
     assert torch.equal(rms_norm_rope(x, 2, None, rope, positions=pos), plain)
     with pytest.raises(NativeError, match="position"):
         check_device_status()
+
+
+def test_offsets_past_32_bits(torch):
+    """1.4 million rows of 1536 features: the last lie 2.15e9 elements in."""
+    from reels_b200 import rms_norm_rope, rms_norm_rope_backward, rope_table
+    rope = rope_table(128, (10, 10, 10))
+    part = torch.randn((1, 1000, 1536), device="cuda").bfloat16()
+    x = part.expand(1400, -1, -1).contiguous()
+    want = rms_norm_rope(part, 12, None, rope)
+    y = rms_norm_rope(x, 12, None, rope)
+    assert torch.equal(y[-1:], want) and torch.equal(y[:1], want)
+    want = rms_norm_rope_backward(part, part.flip(1), 12, None, rope)
+    y.copy_(part.flip(1).expand(1400, -1, -1))
+    dx = rms_norm_rope_backward(x, y, 12, None, rope)
+    assert torch.equal(dx[-1:], want) and torch.equal(dx[:1], want)
