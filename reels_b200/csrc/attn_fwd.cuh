@@ -317,8 +317,11 @@ __global__ void __launch_bounds__(AF_THREADS, 1)
                 for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[120 + e]));
                 mx[0] = at_max3(mx[0], mx[1], mx[2]);
                 mx[3] = at_max3(mx[3], mx[4], mx[5]);
-                float top = fmaxf(at_max3(mx[0], mx[3], mx[6]), mx[7]) * c;
-                top = (top == -CUDART_INF_F ? 0.0f : top) - AtRange<DT>::FWD_SHIFT;
+                // Scores of -infinity alone have no maximum: the lowest number stands for it,
+                // below every live tile's (0 would cost a row of low scores its sum), and
+                // still leaves exp2(-inf - m) = 0.
+                const float top = fmaxf(fmaxf(at_max3(mx[0], mx[3], mx[6]), mx[7]) * c, -CUDART_MAX_NORMAL_F) -
+                                  AtRange<DT>::FWD_SHIFT;
                 if (j == 0) m = top;
                 else if (__any_sync(0xffffffffu, top - m > 8.0f)) {
                     const float to = top - m > 8.0f ? top : m, keep = at_exp2(m - to);

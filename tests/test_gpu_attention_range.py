@@ -1,0 +1,43 @@
+"""GPU tests of attention's range: scores of -infinity."""
+import math
+
+import pytest
+
+import attention_case as ac
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as _t
+    from reels_b200 import build
+    build.build()
+    return _t
+
+
+@pytest.fixture(scope="module")
+def reels(torch):
+    import reels_b200
+    return reels_b200
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("Sq,Sk,D", [(300, 700, 128), (300, 700, 64), (2, 700, 128), (130, 5000, 64)])
+@pytest.mark.parametrize("first", [True, False])
+def test_tiles_of_scores_of_minus_infinity(torch, reels, Sq, Sk, D, dtype, first):
+    """200 keys whose scores are -infinity, ahead of or behind keys with scores
+    of about -1000: they have no weight, and do not stand for a maximum of 0."""
+    n = 200
+    c = ac.Case(1, Sq, Sk, 2, 2, D, getattr(torch, dtype), seed=22, spread=0.5)
+    c.q[..., 0], c.q[..., 1] = 1.0, 32.0
+    c.k[..., 0], c.k[..., 1] = 0.0, -32.0 * D ** 0.5
+    gone = slice(0, n) if first else slice(Sk - n, Sk)
+    live = slice(n, Sk) if first else slice(0, Sk - n)
+    c.k[:, gone, :, 0] = -math.inf
+    out, lse = reels.attention(c.q, c.k, c.v, return_lse=True)
+    reels.check_device_status()
+    c.k, c.v = c.k[:, live], c.v[:, live]
+    want = ac.reference(c, backward=False)
+    ac.check("lse", lse, want["lse"])
+    ac.check("out", out, want["out"])
