@@ -347,11 +347,12 @@ __global__ void __launch_bounds__(UPT == 1 ? 512 : 256, UPT == 1 ? 2 : UPT == 2 
                 F2 lo[4], hi[4];
                 if (BWD) {
                     read(xs, k, xl[0], xh[0]);
-                    const float c2 = -r * r * r * (sum.y * a.inv_c);
+                    // r^3 would leave fp32 from r = 7e12 on: rows of small values without epsilon
+                    const float c2 = -r * (r * (sum.y * a.inv_c));
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        lo[j] = fma2(xl[0][j], F2(c2, c2), mul2(hl[k][j], F2(r, r)));
-                        hi[j] = fma2(xh[0][j], F2(c2, c2), mul2(hh[k][j], F2(r, r)));
+                        lo[j] = mul2(fma2(xl[0][j], F2(c2, c2), hl[k][j]), F2(r, r));
+                        hi[j] = mul2(fma2(xh[0][j], F2(c2, c2), hh[k][j]), F2(r, r));
                     }
                 } else {
 #pragma unroll
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const NormRopeArgs a
         }
         sum = nr_block_sum<BWD>(sum, buf[flip]);
         const float r = 1.0f / sqrtf(sum.x / (float)a.C + a.eps);
-        const float c2 = BWD ? r * r * (sum.y / (float)a.C) : 0.0f;
+        const float c2 = BWD ? r * (r * (sum.y / (float)a.C)) : 0.0f;
         for (int i = threadIdx.x; i < a.C / step; i += blockDim.x) {
             int f0, f1;
             float2 cs;

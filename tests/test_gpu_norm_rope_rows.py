@@ -1,0 +1,81 @@
+"""GPU parity of the q/k norm with rotary positions and of its pullback for
+rows of very small values, against plain 64-bit arithmetic.
+
+Bound per element: u |y| for the output's rounding (u half a step of the
+type) and g = (C + 32) fp32 steps of the magnitudes that enter it: |n| of both
+features of the pair forward, r (|h| of the pair + |x| r^2 mean |h x|) backward."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, FL = "bfloat16", "float16", "float32"
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch as _t
+    from reels_b200 import build
+    build.build()
+    return _t
+
+
+def _check(torch, x, dout, w, y, dx, eps, cs, heads, half):
+    """y and dx (M, C) against the definition; cs (M, D/2, 2) 64-bit (cos, sin), or None."""
+    M, C = x.shape
+    u, g = torch.finfo(x.dtype).eps / 2, (C + 32) * 2.0 ** -23
+    tiny = torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps
+
+    def spin(t, back=False, magnitude=False):
+        if cs is None:
+            return t.abs() if magnitude else t
+        t = t.view(M, heads, C // heads)
+        a, b = t.chunk(2, -1) if half else (t[..., 0::2], t[..., 1::2])
+        if magnitude:
+            p = q = a.abs() + b.abs()
+        else:
+            c, s = cs[:, None, :, 0], cs[:, None, :, 1] * (-1 if back else 1)
+            p, q = a * c - b * s, a * s + b * c
+        return (torch.cat((p, q), -1) if half else torch.stack((p, q), -1).flatten(-2)).reshape(M, C)
+
+    xd, gd, wd = x.double(), dout.double(), 1.0 if w is None else w.double()
+    r = 1 / (xd.square().mean(-1, keepdim=True) + eps).sqrt()
+    n = xd * r * wd
+    want = spin(n)
+    bound = u * want.abs() + g * spin(n, magnitude=True) + tiny
+    assert float(((y.double() - want).abs() / bound).max()) <= 1.0
+    h, hm = spin(gd, back=True) * wd, spin(gd, magnitude=True) * (1.0 if w is None else wd.abs())
+    want = r * (h - xd * r * r * (h * xd).mean(-1, keepdim=True))
+    bound = u * want.abs() + g * r * (hm + xd.abs() * r * r * (hm * xd.abs()).mean(-1, keepdim=True)) + tiny
+    fits = want.abs() < torch.finfo(x.dtype).max
+    assert float(((dx.double() - want).abs() / bound)[fits].max()) <= 1.0
+
+
+def _angles(torch, rope, coords, on):
+    """(cos, sin) of the table at a token's coordinates, in 64 bits; tokens that are not `on` are not turned."""
+    parts, at = [], 0
+    for size, dim, pos in zip(rope.sizes, rope.dims, coords):
+        t = rope.table[at:at + size * dim // 2].view(size, dim // 2, 2).double()
+        parts.append(t[pos.clamp(0, size - 1)])
+        at += size * dim // 2
+    still = torch.tensor([1.0, 0.0], dtype=torch.float64, device="cuda")
+    return torch.where(on[:, None, None], torch.cat(parts, 1), still)
+
+
+@pytest.mark.parametrize("dtype", [BF, FL])
+@pytest.mark.parametrize("C,heads", [(256, 2), (100, 5)])  # the vector and the scalar form
+@pytest.mark.parametrize("rotated", [False, True])
+def test_rows_of_very_small_values(torch, dtype, C, heads, rotated):
+    """r = 1e13 and more without epsilon: r^3 is beyond fp32, dx = r (h - x r^2 mean(h x)) is not."""
+    from reels_b200 import rms_norm_rope, rms_norm_rope_backward, rope_table
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    dt = getattr(torch, dtype)
+    sizes = torch.tensor([1e-13, 1e-14, 3e-16, 1e-17], device="cuda")[:, None]
+    x = (sizes * torch.randn((4, C), generator=gen, device="cuda")).to(dt)
+    dout = torch.randn((4, C), generator=gen, device="cuda").to(dt)
+    w = (1 + 0.2 * torch.randn(C, generator=gen, device="cuda")).to(dt)
+    rope = rope_table(C // heads, (4,), (C // heads,)) if rotated else None
+    cs = _angles(torch, rope, (torch.arange(4, device="cuda"),), torch.ones(4, dtype=torch.bool, device="cuda")) if rotated else None
+    y = rms_norm_rope(x, heads, w, rope, 0.0)
+    dx = rms_norm_rope_backward(x, dout, heads, w, rope, 0.0)
+    assert bool(torch.isfinite(dx.float()).all())
+    _check(torch, x, dout, w, y, dx, 0.0, cs, heads, False)
