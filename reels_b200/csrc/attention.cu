@@ -540,7 +540,9 @@ int reels_attention_backward(const reels_attn_shape *shape, const void *q, const
     else
         with_tc_type(act_dtype, s.head_dim, [&](auto t, auto d) {
             constexpr int DT = decltype(t)::value, G = decltype(d)::value / 8;
-            const int64_t blocks = ceil_div(s.batch * s.q_tokens * s.heads, 256 / G * 4);
+            // for fp16 the rows of v are read too, and there may be many more of them
+            const int64_t read = std::max(s.batch * s.q_tokens * s.heads, DT == DT_F16 ? keys : 0);
+            const int64_t blocks = ceil_div(read, 256 / G * 4);
             float2 *range = reinterpret_cast<float2 *>(ws + w.range);
             a.range = range;
             a.ranges = (int)std::min<int64_t>(blocks, kStatBlocks);

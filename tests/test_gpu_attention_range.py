@@ -1,4 +1,5 @@
-"""GPU tests of attention's range: scores of -infinity."""
+"""GPU tests of attention's range: scores of -infinity,
+fp16 gradients of few queries over many keys."""
 import math
 
 import pytest
@@ -41,3 +42,32 @@ def test_tiles_of_scores_of_minus_infinity(torch, reels, Sq, Sk, D, dtype, first
     want = ac.reference(c, backward=False)
     ac.check("lse", lse, want["lse"])
     ac.check("out", out, want["out"])
+
+
+def test_fp16_gradient_of_few_queries_over_many_keys(torch, reels):
+    """What fp16 needs beside bf16, the sizes of the rows of v, is read by as
+    many blocks as there are rows: 16 queries over 9000 keys take about the
+    time that bf16 takes."""
+    times = {}
+    runs = {}
+    for dtype in (torch.bfloat16, torch.float16):
+        c = ac.Case(1, 16, 9000, 12, 12, 128, dtype, seed=23)
+        out, lse = reels.attention(c.q, c.k, c.v, return_lse=True)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            reels.attention_backward(c.dout, c.q, c.k, c.v, out, lse)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                kept = [reels.attention_backward(c.dout, c.q, c.k, c.v, out, lse) for _ in range(10)]
+        runs[dtype] = (g, c, out, lse, kept)
+    torch.cuda.synchronize()
+    for _ in range(10):  # in turn, and the best of each: another load on the GPU slows both
+        for dtype, (g, *_) in runs.items():
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            g.replay()
+            end.record()
+            end.synchronize()
+            times[dtype] = min(times.get(dtype, math.inf), start.elapsed_time(end))
+    assert times[torch.float16] <= 1.5 * times[torch.bfloat16], times
