@@ -240,9 +240,10 @@ AttnPlan plan_attention(const reels_attn_shape &s, int dt, const void *q, const 
 }
 
 struct AttnWs {
-    size_t part_o = 0, part_lse = 0, stat_l = 0, stat_d = 0, range = 0, part_k = 0, part_v = 0, total = 0;
+    size_t part_o = 0, part_lse = 0, stat_l = 0, stat_d = 0, stat_n = 0, v_n = 0, range = 0, part_k = 0, part_v = 0,
+           total = 0;
 };
-AttnWs attn_ws(const reels_attn_shape &s, const AttnPlan &p, bool bwd) {
+AttnWs attn_ws(const reels_attn_shape &s, const AttnPlan &p, int dt, bool bwd) {
     AttnWs w;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -260,7 +261,11 @@ AttnWs attn_ws(const reels_attn_shape &s, const AttnPlan &p, bool bwd) {
         const size_t rows = (size_t)s.batch * s.heads * p.Sqp;
         w.stat_l = take(rows * 4);
         w.stat_d = take(rows * 4);
-        w.range = take(kStatBlocks * 8);
+        if (p.tc && dt == REELS_F16) {
+            w.stat_n = take(rows * 4);
+            w.v_n = take((size_t)s.batch * s.kv_heads * s.k_tokens * 4);
+            w.range = take((size_t)s.batch * s.kv_heads * 8);
+        }
         if (p.red_splits > 1) {
             const size_t n = (size_t)p.red_splits * s.batch * s.k_tokens * s.kv_heads * s.head_dim * 4;
             w.part_k = take(n);
@@ -393,9 +398,9 @@ size_t reels_attention_workspace_bytes(const reels_attn_shape *shape, int act_dt
     if (check_shape(shape, act_dtype) != REELS_OK) return 0;
     // The larger of the two paths: which one runs also depends on the pointers.
     AttnPlan p = plan_attention(*shape, act_dtype, nullptr, nullptr, nullptr);
-    size_t n = attn_ws(*shape, p, pass == REELS_PASS_BACKWARD).total;
+    size_t n = attn_ws(*shape, p, act_dtype, pass == REELS_PASS_BACKWARD).total;
     p = plan_attention(*shape, act_dtype, reinterpret_cast<const void *>(1), nullptr, nullptr);
-    return std::max(n, attn_ws(*shape, p, pass == REELS_PASS_BACKWARD).total);
+    return std::max(n, attn_ws(*shape, p, act_dtype, pass == REELS_PASS_BACKWARD).total);
 }
 
 int reels_attention_plan(const reels_attn_shape *shape, int act_dtype, int64_t *info) {
@@ -424,7 +429,7 @@ int reels_attention_forward(const reels_attn_shape *shape, const void *q, const 
     const bool tc = p.tc && aligned16(out) && s.k_tokens > 0;
     AttnPlan plan = p;
     if (!tc && p.tc) plan = plan_attention(s, act_dtype, reinterpret_cast<const void *>(1), k, v);
-    const AttnWs w = attn_ws(s, plan, false);
+    const AttnWs w = attn_ws(s, plan, act_dtype, false);
     rc = check_workspace(workspace, ws_bytes, w.total);
     if (rc) return rc;
     HostCall call;
@@ -515,7 +520,7 @@ int reels_attention_backward(const reels_attn_shape *shape, const void *q, const
     AttnPlan plan = plan_attention(s, act_dtype, q, k, v);
     if (plan.tc && !(aligned16(out) && aligned16(dout) && aligned16(dq) && aligned16(dk) && aligned16(dv)))
         plan = plan_attention(s, act_dtype, reinterpret_cast<const void *>(1), k, v);
-    const AttnWs w = attn_ws(s, plan, true);
+    const AttnWs w = attn_ws(s, plan, act_dtype, true);
     rc = check_workspace(workspace, ws_bytes, w.total);
     if (rc) return rc;
     rc = call.bind(q);
@@ -543,11 +548,16 @@ int reels_attention_backward(const reels_attn_shape *shape, const void *q, const
             // for fp16 the rows of v are read too, and there may be many more of them
             const int64_t read = std::max(s.batch * s.q_tokens * s.heads, DT == DT_F16 ? keys : 0);
             const int64_t blocks = ceil_div(read, 256 / G * 4);
+            float *stat_n = reinterpret_cast<float *>(ws + w.stat_n), *v_n = reinterpret_cast<float *>(ws + w.v_n);
             float2 *range = reinterpret_cast<float2 *>(ws + w.range);
-            a.range = range;
-            a.ranges = (int)std::min<int64_t>(blocks, kStatBlocks);
-            e = host_launch_pdl(attn_stat_vec_kernel<DT, G>, dim3((unsigned)a.ranges), dim3(256), 0, st, a, stat_l,
-                                stat_d, range, AtRange<DT>::BWD_SHIFT);
+            a.stat_n = stat_n, a.range = range;
+            e = host_launch_pdl(attn_stat_vec_kernel<DT, G>, dim3((unsigned)std::min<int64_t>(blocks, kStatBlocks)),
+                                dim3(256), 0, st, a, stat_l, stat_d, stat_n, v_n, AtRange<DT>::BWD_SHIFT);
+            if (DT == DT_F16 && e == cudaSuccess) {
+                host_count_launch();
+                e = host_launch_pdl(attn_range_kernel, dim3((unsigned)(s.batch * s.kv_heads)), dim3(1024), 0, st, a,
+                                    static_cast<const float *>(v_n), range);
+            }
         });
     RA_LAUNCH(e);
     if (!plan.tc) {

@@ -31,24 +31,13 @@ namespace reels {
 constexpr int AB_THREADS = 32 * 12;  // 8 elementwise warps, loads, MMA issue, two idle
 using AbRegisters = AtRegisters<216>;
 
-// fp16: exponent e with |dS| 2^e <= 2^15, from |dP|, |delta| <= |dO row| |v row|
-// whose largest values the blocks of the statistics kernel left.  Called by
-// whole warps.
+// fp16: exponent e with |dS| 2^e <= 2^15, from |dP|, |delta| <= |dO row| |v row|:
+// `top` is the largest |dO row| times the largest |v row| of what shares e.
+// That is a sample's key head for dK, whose sums run over the rows, and a row
+// for dQ.  (What lies 2^-40 and more below the bound rounds to 0.)
 template <int DT>
-__device__ __forceinline__ int attn_grad_exp(const AttnArgs &a) {
-    if (DT != DT_F16) return 0;
-    float g = 0.0f, v = 0.0f;
-    for (int i = threadIdx.x & 31; i < a.ranges; i += 32) {
-        const float2 r = __ldcg(a.range + i);
-        g = fmaxf(g, r.x), v = fmaxf(v, r.y);
-    }
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) {
-        g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, w));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, w));
-    }
-    const float top = g * v;
-    if (!(top > 1e-30f) || !(top < 1e30f)) return 0;
+__device__ __forceinline__ int attn_grad_exp(float top) {
+    if (DT != DT_F16 || !(top > 1e-30f) || !(top < 1e30f)) return 0;
     return 13 - ilogbf(top);
 }
 
@@ -248,14 +237,18 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap &tmQ, const CUtensor
         const uint32_t S = tmem + lanes + 64 * half, DS = S + 128, O = tmem + lanes + 256 + 128 * half;
         const float c = a.scale * CUDART_L2E_F;
         const F2 c2 = F2(c, c);
-        const int e = attn_grad_exp<DT>(a);
-        const float g1 = exp2f((float)e - AtRange<DT>::BWD_SHIFT);
-        const F2 grow = F2(g1, g1);
-        const float f = half ? a.scale * exp2f(-(float)e) : exp2f(-AtRange<DT>::BWD_SHIFT);
         uint32_t g = 0, ns = 0, nu = 0;
         bool good = true;
         for (long long u = u0; u < units && good; u += step) {
             const AttnKvUnit w = attn_kv_unit(a, u);
+            int e = 0;
+            if (DT == DT_F16) {
+                const float2 r = __ldcg(a.range + (long long)w.b * a.HK + w.hk);
+                e = attn_grad_exp<DT>(r.x * r.y);
+            }
+            const float g1 = exp2f((float)e - AtRange<DT>::BWD_SHIFT);
+            const F2 grow = F2(g1, g1);
+            const float f = half ? a.scale * exp2f(-(float)e) : exp2f(-AtRange<DT>::BWD_SHIFT);
             const int row = (warp & 3) * 32 + lane;
             const bool live = row < w.rows;
             for (int i = 0; i < w.n; ++i, ++g, ++ns) {
@@ -579,10 +572,7 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap &tmQ, const CUtensorMa
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t DS = tmem + lanes + 256 + 64 * half, O = tmem + lanes + 384;
         const float c = a.scale * CUDART_L2E_F;
-        const int e = attn_grad_exp<DT>(a);
         const F2 c2 = F2(c, c);
-        const float g1 = exp2f((float)e - AtRange<DT>::BWD_SHIFT), f = a.scale * exp2f(-(float)e);
-        const F2 grow = F2(g1, g1);
         uint32_t g = 0, nu = 0;
         bool good = true;
         for (long long u = u0; u < units && good; u += step) {
@@ -591,6 +581,11 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap &tmQ, const CUtensorMa
             const long long st = ((long long)w.b * a.H + w.h) * a.Sqp + row;
             const float sl = __ldcg(a.stat_l + st), sd = __ldcg(a.stat_d + st);
             const F2 L = F2(sl, sl), delta = F2(sd, sd);
+            int e = 0;
+            if (DT == DT_F16)
+                e = attn_grad_exp<DT>(__ldcg(a.stat_n + st) * __ldcg(a.range + (long long)w.b * a.HK + w.hk).y);
+            const float g1 = exp2f((float)e - AtRange<DT>::BWD_SHIFT), f = a.scale * exp2f(-(float)e);
+            const F2 grow = F2(g1, g1);
             for (int j = 0; j < w.nk; ++j, ++g) {
                 const int t = g & 1;
                 good = at_wait(&s_full[t], (g >> 1) & 1, abort, a.err, DEVERR_TIMEOUT_ACC);

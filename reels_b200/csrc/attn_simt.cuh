@@ -42,8 +42,8 @@ struct AttnArgs {
     const float *stat_l, *stat_d;            // [B][H][Sqp]: -L in log2 units (-inf: no part), -delta
     int Sqp;                                 // Sq rounded up to whole tiles
     void *dq, *dk, *dv;                      // contiguous, in the layout of q, k and v
-    const float2 *range;                     // fp16: [ranges] largest |dO row| and |v row| of a block
-    int ranges;
+    const float *stat_n;                     // fp16: [B][H][Sqp] |dO row|
+    const float2 *range;                     // fp16: [B][HK] largest |dO row| of the heads that share it, and |v row|
     int red_splits;                          // dK, dV: ranges of the (head, query tile) walk
     float *part_k, *part_v;                  // [red_splits][B][Sk][HK][D]
     unsigned *err;
@@ -423,11 +423,10 @@ __global__ void __launch_bounds__(256) attn_stat_kernel(const AttnArgs a, float 
     }
 }
 
-// The largest |row|^2 and, with `y`, x . y of rows of D = 8 n <= 8 G features:
-// G lanes a row with 16 bytes each, four rows in flight.
+// x . y (with `y`) and, for fp16, |x| of rows of D = 8 n <= 8 G features: G
+// lanes a row with 16 bytes each, four rows in flight.
 template <int DT, int G, typename At, typename Use>
-__device__ __forceinline__ void as_rows(const void *x, const void *y, long long rows, int D, At at, Use use,
-                                        float &top) {
+__device__ __forceinline__ void as_rows(const void *x, const void *y, long long rows, int D, At at, Use use) {
     using T = typename Elem<DT>::T;
     constexpr int R = 4;
     const int sub = threadIdx.x % G;
@@ -447,7 +446,7 @@ __device__ __forceinline__ void as_rows(const void *x, const void *y, long long 
                 }
             }
         }
-        float mine = 0.0f;  // lane i of the group keeps row i's product
+        float mine = 0.0f, size = 0.0f;  // lane i of the group keeps row i's
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             F2 g[4], h[4], d2 = F2(0.0f, 0.0f), n2 = F2(0.0f, 0.0f);
@@ -464,74 +463,92 @@ __device__ __forceinline__ void as_rows(const void *x, const void *y, long long 
                 if (y) dot += __shfl_xor_sync(0xffffffffu, dot, w);
                 if (DT == DT_F16) norm += __shfl_xor_sync(0xffffffffu, norm, w);
             }
-            top = fmaxf(top, norm);
-            if (sub == i) mine = dot;
+            if (sub == i) mine = dot, size = norm;
         }
-        if (y && sub < R && r0 + sub < rows) use(r0 + sub, mine);
+        if (sub < R && r0 + sub < rows) use(r0 + sub, mine, sqrtf(size));
     }
 }
 
 // The same for the tensor-core kernels: rows in memory order (the heads of a
 // token side by side), `shift` added to -L (fp16, see AtRange), and for fp16
-// each block's largest |dO row| and |v row|.  Bound: HBM, out and dO once (2 x
-// 6144 tokens, 32 heads of 128: 201 MB in 37 us, 5.4 TB/s).
+// the rows' |dO| and, for v_n [B][HK][Sk], |v| (0 behind a sample's length).
+// Bound: HBM, out and dO once (2 x 6144 tokens, 32 heads of 128: 201 MB in
+// 37 us, 5.4 TB/s).
 template <int DT, int G>
 __global__ void __launch_bounds__(256) attn_stat_vec_kernel(const AttnArgs a, float *stat_l, float *stat_d,
-                                                            float2 *range, float shift) {
+                                                            float *stat_n, float *v_n, float shift) {
     griddep_wait();
+    // a row's head, token and sample (64-bit divisions would cost more than the rows)
+    auto where = [](long long r, long long rows, int heads, int tokens, int &b, int &t, int &h) {
+        if (rows <= 0x7fffffff) {
+            const uint32_t tok = (uint32_t)r / (uint32_t)heads;
+            h = (int)((uint32_t)r - tok * heads), b = (int)(tok / (uint32_t)tokens);
+            t = (int)(tok - b * (uint32_t)tokens);
+        } else {
+            const long long tok = r / heads;
+            h = (int)(r - tok * heads), b = (int)(tok / tokens), t = (int)(tok - (long long)b * tokens);
+        }
+    };
     const long long rows = (long long)a.B * a.Sq * a.H;
-    float top = 0.0f, top_v = 0.0f;
     as_rows<DT, G>(
         a.dout, a.out, rows, a.D, [&](long long r) { return r * a.D; },
-        [&](long long r, float delta) {
+        [&](long long r, float delta, float size) {
             int b, q, h;
-            if (rows <= 0x7fffffff) {  // (64-bit divisions would cost more than the rows)
-                const uint32_t tok = (uint32_t)r / (uint32_t)a.H;
-                h = (int)((uint32_t)r - tok * a.H), b = (int)(tok / (uint32_t)a.Sq), q = (int)(tok - b * (uint32_t)a.Sq);
-            } else {
-                const long long tok = r / a.H;
-                h = (int)(r - tok * a.H), b = (int)(tok / a.Sq), q = (int)(tok - (long long)b * a.Sq);
-            }
-            const long long bh = (long long)b * a.H + h;
+            where(r, rows, a.H, a.Sq, b, q, h);
+            const long long bh = (long long)b * a.H + h, at = bh * a.Sqp + q;
             const float lse = __ldcg(a.lse + bh * a.Sq + q);
             const bool dead = lse == -CUDART_INF_F;
-            stat_l[bh * a.Sqp + q] = dead ? -CUDART_INF_F : shift - lse * CUDART_L2E_F;
-            stat_d[bh * a.Sqp + q] = dead ? 0.0f : -delta;
-        },
-        top);
+            stat_l[at] = dead ? -CUDART_INF_F : shift - lse * CUDART_L2E_F;
+            stat_d[at] = dead ? 0.0f : -delta;
+            if (DT == DT_F16) stat_n[at] = size;
+        });
     const int pad = a.Sqp - a.Sq;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < (long long)a.B * a.H * pad; i += gridDim.x * 256ll) {
         const long long at = i / pad * a.Sqp + a.Sq + i % pad;
         stat_l[at] = -CUDART_INF_F;
         stat_d[at] = 0.0f;
+        if (DT == DT_F16) stat_n[at] = 0.0f;
     }
     if (DT == DT_F16) {
-        __shared__ float2 warps[8];
+        const long long keys = (long long)a.B * a.Sk * a.HK;
+        int b, t, h;
         as_rows<DT, G>(
-            a.v, nullptr, (long long)a.B * a.Sk * a.HK, a.D,
+            a.v, nullptr, keys, a.D,
             [&](long long r) {
-                int h, t, b;
-                if ((long long)a.B * a.Sk * a.HK <= 0x7fffffff) {
-                    const uint32_t tok = (uint32_t)r / (uint32_t)a.HK;
-                    h = (int)((uint32_t)r - tok * a.HK), b = (int)(tok / (uint32_t)a.Sk);
-                    t = (int)(tok - b * (uint32_t)a.Sk);
-                } else {
-                    h = (int)(r % a.HK), t = (int)(r / a.HK % a.Sk), b = (int)(r / a.HK / a.Sk);
-                }
+                where(r, keys, a.HK, a.Sk, b, t, h);
                 return t < attn_keys(a, b) ? b * a.vs[0] + t * a.vs[1] + h * a.vs[2] : -1ll;
             },
-            [](long long, float) {}, top_v);
+            [&](long long r, float, float size) {
+                where(r, keys, a.HK, a.Sk, b, t, h);
+                v_n[((long long)b * a.HK + h) * a.Sk + t] = size;
+            });
+    }
+}
+
+// The largest |dO row| and |v row| of each sample and key head, a block each: a
+// gradient's range goes by what its own sums hold, so that nothing of one
+// sample or head is lost beside the gradients of another.  (A launch of 3 us
+// where a maximum by atomics would need its memory cleared by another.)
+__global__ void __launch_bounds__(1024) attn_range_kernel(const AttnArgs a, const float *v_n, float2 *range) {
+    __shared__ float2 warps[32];
+    griddep_wait();
+    const long long rows = (long long)(a.H / a.HK) * a.Sqp;  // the heads of a group lie side by side
+    const float *n = a.stat_n + blockIdx.x * rows, *v = v_n + blockIdx.x * (long long)a.Sk;
+    float2 top = make_float2(0.0f, 0.0f);
+#pragma unroll 8
+    for (long long i = threadIdx.x; i < rows; i += 1024) top.x = fmaxf(top.x, __ldcg(n + i));
+#pragma unroll 8
+    for (int i = threadIdx.x; i < a.Sk; i += 1024) top.y = fmaxf(top.y, __ldcg(v + i));
 #pragma unroll
-        for (int w = 16; w > 0; w >>= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-            top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, w));
-        }
-        if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = make_float2(top, top_v);
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < 8; ++w) top = fmaxf(top, warps[w].x), top_v = fmaxf(top_v, warps[w].y);
-            range[blockIdx.x] = make_float2(sqrtf(top), sqrtf(top_v));
-        }
+    for (int w = 16; w > 0; w >>= 1) {
+        top.x = fmaxf(top.x, __shfl_xor_sync(0xffffffffu, top.x, w));
+        top.y = fmaxf(top.y, __shfl_xor_sync(0xffffffffu, top.y, w));
+    }
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 32; ++w) top.x = fmaxf(top.x, warps[w].x), top.y = fmaxf(top.y, warps[w].y);
+        range[blockIdx.x] = top;
     }
 }
 

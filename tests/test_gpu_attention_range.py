@@ -1,6 +1,7 @@
-"""GPU tests of attention's range: scores of -infinity,
-fp16 gradients of few queries over many keys."""
+"""GPU tests of attention's range: fp16 gradients of parts whose sizes lie far
+apart, scores of -infinity, fp16 gradients of few queries over many keys."""
 import math
+import types
 
 import pytest
 
@@ -21,6 +22,43 @@ def torch():
 def reels(torch):
     import reels_b200
     return reels_b200
+
+
+def _part(c, b=slice(None), h=slice(None), hk=slice(None), rows=slice(None)):
+    """A part of a case whose outputs do not depend on the rest, so that no
+    term of its bounds is taken over more than the part."""
+    return types.SimpleNamespace(q=c.q[b, rows, h], k=c.k[b, :, hk], v=c.v[b, :, hk], dout=c.dout[b, rows, h],
+                                 dtype=c.dtype, scale=c.scale, lengths=None if c.lengths is None else c.lengths[b])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("over", ["samples", "heads", "rows"])
+def test_fp16_gradients_of_sizes_far_apart(torch, reels, over, D):
+    """Gradients of the output, or values, that differ by 2^20 from sample to
+    sample, from key head to key head and (for dq) from row to row: the small
+    ones keep their bits."""
+    B, S, H, HK = 2, 1500, 4, 2
+    c = ac.Case(B, S, S, H, HK, D, torch.float16, [S, S - 7], seed=21, spread=0.5)
+    size = torch.ones((B, S, H, 1), device="cuda")
+    if over == "samples":
+        size[1] = 2.0 ** -20
+    elif over == "heads":
+        size[:, :, :2] = 2.0 ** -20
+        c.v[:, :, 1] *= 2.0 ** 6
+    else:
+        size[:, ::3] = 2.0 ** -20
+    c.dout = (c.dout.float() * 2.0 ** 8 * size).half()
+    out, lse = reels.attention(c.q, c.k, c.v, kv_lengths=c.lengths, return_lse=True)
+    dq, dk, dv = reels.attention_backward(c.dout, c.q, c.k, c.v, out, lse, kv_lengths=c.lengths)
+    reels.check_device_status()
+    for b in range(B):
+        for g in range(HK):
+            s, h, hk = slice(b, b + 1), slice(2 * g, 2 * g + 2), slice(g, g + 1)
+            for rows in ((slice(0, None, 3), slice(1, None, 3), slice(2, None, 3)) if over == "rows" else (slice(None),)):
+                ac.check("dq", dq[s, rows, h], ac.reference(_part(c, s, h, hk, rows))["dq"])
+            want = ac.reference(_part(c, s, h, hk))
+            ac.check("dk", dk[s, :, hk], want["dk"])
+            ac.check("dv", dv[s, :, hk], want["dv"])
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
