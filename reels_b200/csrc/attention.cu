@@ -71,6 +71,7 @@ constexpr int kNormRopeSmem = 220 * 1024;  // of an SM's 228 KB, 1 KB a block is
 
 template <int DT, bool BWD, bool ROPE, bool HALF, int UPT>
 cudaError_t launch_norm_rope(const NormRopeArgs &a, int threads, const HostCall &call, cudaStream_t st) {
+    static_assert(!(BWD && UPT == 2), "a form that no call takes");
     // Blocks that fit beside each other with a ring of at least two rows, then
     // as many rows as the shared memory holds.
     const int budget = kNormRopeSmem, fixed = nr_smem_bytes(a.C, bytes_of(DT), BWD, 0, a.D) + 1024;
@@ -143,9 +144,9 @@ int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t head
         constexpr int DT = decltype(t)::value;
         auto form = [&](auto b, auto r, auto h) {
             constexpr bool B = decltype(b)::value, R = decltype(r)::value, H = decltype(h)::value;
-            e = upt == 1   ? launch_norm_rope<DT, B, R, H, 1>(a, threads, call, st)
-                : upt == 2 ? launch_norm_rope<DT, B, R, H, 2>(a, threads, call, st)
-                           : launch_norm_rope<DT, B, R, H, 4>(a, threads, call, st);
+            if (upt == 1) e = launch_norm_rope<DT, B, R, H, 1>(a, threads, call, st);
+            else if (upt == 4) e = launch_norm_rope<DT, B, R, H, 4>(a, threads, call, st);
+            else if constexpr (!B) e = launch_norm_rope<DT, B, R, H, 2>(a, threads, call, st);
         };
         auto dir = [&](auto b) {
             if (!rope) form(b, std::false_type{}, std::false_type{});
