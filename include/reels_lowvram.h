@@ -356,6 +356,10 @@ typedef struct reels_rope {
     int32_t pairing;
 } reels_rope;
 
+/* Or-ed into act_dtype of the two calls below: weight is fp32 beside
+ * activations of another type. */
+#define REELS_NORM_WEIGHT_F32 0x100
+
 /* out = R(x / sqrt(mean(x^2) + epsilon) * weight), one pass per row of
  * x [M][heads * head_dim]: the norm spans all heads of a token, weight
  * [heads * head_dim] is nullable, rope is nullable (the norm alone, as for

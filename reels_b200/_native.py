@@ -20,6 +20,7 @@ PASS_FORWARD, PASS_BACKWARD, PASS_DROPOUT = 0, 1, 2
 PATH_NONE, PATH_TENSORCORE, PATH_CUDACORE = 0, 1, 2
 ACT_NONE, ACT_GELU_TANH = 0, 1
 ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+NORM_WEIGHT_F32 = 0x100  # or-ed into the q/k norm's dtype
 OK, EINVAL, EDEVICE = 0, -1, -2
 
 class OptTensor(ctypes.Structure):

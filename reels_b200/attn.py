@@ -106,11 +106,12 @@ def _norm_rope_args(x, heads, weight, rope, tokens_per_sample, positions):
         raise ValueError("the features must be heads * head_dim")
     xf = x if x.is_contiguous() else x.contiguous()
     M = x.numel() // C
-    w = weight
+    w, dt = weight, _dt(x.dtype)
     if w is not None:
         _check_numel(w, C, "norm weight", x.device)
-        if w.dtype != x.dtype or not w.is_contiguous():
-            w = w.contiguous().to(x.dtype)
+        if w.dtype != x.dtype:  # fp32 holds what the other types hold
+            w, dt = w.float(), dt | nat.NORM_WEIGHT_F32
+        w = w.contiguous()
     if tokens_per_sample is None:
         tps = x.shape[-2] if x.dim() >= 2 else 1
     else:
@@ -139,7 +140,7 @@ def _norm_rope_args(x, heads, weight, rope, tokens_per_sample, positions):
         r = ctypes.byref(nat.Rope(rope.table.data_ptr(), _ptr(pos), sizes, dims, pairing))
     elif positions is not None:
         raise ValueError("positions need a rotary table")
-    return xf, M, heads, C // heads, w, r, max(tps, 1), pos
+    return xf, M, heads, C // heads, w, r, max(tps, 1), pos, dt
 
 
 def rms_norm_rope(x: torch.Tensor, heads: int, weight: Optional[torch.Tensor] = None,
@@ -148,6 +149,7 @@ def rms_norm_rope(x: torch.Tensor, heads: int, weight: Optional[torch.Tensor] = 
     """``rotate(x / sqrt(mean(x ** 2) + epsilon) * weight)`` in one pass per
     token, the norm over all heads of ``x`` (..., tokens, heads * head_dim).
 
+    ``weight`` may be of another type than x: it enters in fp32.
     ``rope=None`` is the norm alone (the cross-attention's q and k).  Tokens
     are at (t, h, w) of the table's sizes in raster order, starting again
     every ``tokens_per_sample`` tokens (default: x's tokens dimension), and
@@ -155,9 +157,9 @@ def rms_norm_rope(x: torch.Tensor, heads: int, weight: Optional[torch.Tensor] = 
     ``positions`` (..., tokens, axes), integers, each token is where its row
     says; a negative position marks padding.  A position behind its table
     leaves the token unturned and is reported by :func:`check_device_status`."""
-    xf, M, heads, D, w, r, tps, pos = _norm_rope_args(x, heads, weight, rope, tokens_per_sample, positions)
+    xf, M, heads, D, w, r, tps, pos, dt = _norm_rope_args(x, heads, weight, rope, tokens_per_sample, positions)
     out = torch.empty_like(xf)
-    code = nat.lib().reels_rms_norm_rope(xf.data_ptr(), M, heads, D, _ptr(w), r, tps, float(epsilon), _dt(x.dtype),
+    code = nat.lib().reels_rms_norm_rope(xf.data_ptr(), M, heads, D, _ptr(w), r, tps, float(epsilon), dt,
                                          out.data_ptr(), _stream(x.device))
     nat.check("rms_norm_rope", code)
     return out
@@ -171,11 +173,11 @@ def rms_norm_rope_backward(x: torch.Tensor, dout: torch.Tensor, heads: int, weig
     _require_cuda(dout)
     if dout.shape != x.shape or dout.dtype != x.dtype or dout.device != x.device:
         raise ValueError("dout must have the shape, dtype and device of x")
-    xf, M, heads, D, w, r, tps, pos = _norm_rope_args(x, heads, weight, rope, tokens_per_sample, positions)
+    xf, M, heads, D, w, r, tps, pos, dt = _norm_rope_args(x, heads, weight, rope, tokens_per_sample, positions)
     df = dout if dout.is_contiguous() else dout.contiguous()
     dx = torch.empty_like(xf)
     code = nat.lib().reels_rms_norm_rope_backward(xf.data_ptr(), df.data_ptr(), M, heads, D, _ptr(w), r, tps,
-                                                  float(epsilon), _dt(x.dtype), dx.data_ptr(), _stream(x.device))
+                                                  float(epsilon), dt, dx.data_ptr(), _stream(x.device))
     nat.check("rms_norm_rope_backward", code)
     return dx
 

@@ -69,17 +69,17 @@ int check_norm_rope(const void *x, int64_t M, int64_t heads, int64_t D, const re
 
 constexpr int kNormRopeSmem = 220 * 1024;  // of an SM's 228 KB, 1 KB a block is the system's
 
-template <int DT, bool BWD, bool ROPE, bool HALF, int UPT>
+template <int DT, bool BWD, bool ROPE, bool HALF, int UPT, bool W32>
 cudaError_t launch_norm_rope(const NormRopeArgs &a, int threads, const HostCall &call, cudaStream_t st) {
-    static_assert(!(BWD && UPT == 2), "a form that no call takes");
+    static_assert(!(BWD && UPT == 2) && !(W32 && (!BWD || DT == DT_F32)), "a form that no call takes");
     // Blocks that fit beside each other with a ring of at least two rows, then
     // as many rows as the shared memory holds.
-    const int budget = kNormRopeSmem, fixed = nr_smem_bytes(a.C, bytes_of(DT), BWD, 0, a.D) + 1024;
+    const int budget = kNormRopeSmem, fixed = nr_smem_bytes(a.C, bytes_of(DT), BWD, W32, 0, a.D) + 1024;
     const int step = a.C * bytes_of(DT) * (BWD ? 2 : 1);
     const int blocks = std::max(1, std::min({(UPT == 1 ? 1024 : UPT == 2 ? 768 : 256) / threads, 24, budget / (fixed + 2 * step)}));
     const int stages = std::max(2, std::min(NR_STAGES, (budget / blocks - fixed) / step));  // (two rows were checked to fit)
-    const int smem = nr_smem_bytes(a.C, bytes_of(DT), BWD, stages, a.D);
-    auto kern = norm_rope_kernel<DT, BWD, ROPE, HALF, UPT>;
+    const int smem = nr_smem_bytes(a.C, bytes_of(DT), BWD, W32, stages, a.D);
+    auto kern = norm_rope_kernel<DT, BWD, ROPE, HALF, UPT, W32>;
     // the most any call asks for, once per device: calls of several threads agree on it
     static std::atomic<uint64_t> ready{0};
     if (!(ready.load() >> call.device & 1)) {
@@ -93,6 +93,8 @@ cudaError_t launch_norm_rope(const NormRopeArgs &a, int threads, const HostCall 
 
 int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t heads, int64_t D, const void *weight,
               const reels_rope *rope, int64_t tps, float eps, int dt, void *out, void *stream) {
+    const bool w32 = (dt & REELS_NORM_WEIGHT_F32) != 0;
+    dt &= ~REELS_NORM_WEIGHT_F32;
     int rc = check_norm_rope(x, M, heads, D, rope, tps, eps, dt);
     if (rc) return rc;
     if (M == 0) return host_ok(REELS_PATH_NONE);
@@ -103,7 +105,7 @@ int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t head
     if (rc) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     NormRopeArgs a = {};
-    a.x = x, a.dout = dout, a.weight = weight, a.out = out;
+    a.x = x, a.dout = dout, a.weight = weight, a.w32 = w32, a.out = out;
     a.M = M, a.C = (int)(heads * D), a.D = (int)D, a.tps = (int)tps, a.eps = eps, a.inv_c = 1.0f / (float)a.C;
     a.err = call.status;
     if (rope) {
@@ -119,7 +121,7 @@ int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t head
     const bool vec = a.C % 16 == 0 && heads_fit && aligned16(x) && aligned16(out) && aligned16(weight) &&
                      (!bwd || aligned16(dout)) &&
                      // two rows have to fit the shared memory beside the weight
-                     nr_smem_bytes(a.C, bytes_of(dt), bwd, 2, a.D) <= kNormRopeSmem;
+                     nr_smem_bytes(a.C, bytes_of(dt), bwd, w32, 2, a.D) <= kNormRopeSmem;
     if (!vec) {
         const dim3 grid((unsigned)std::min<int64_t>(M, 8ll * call.sms));
         with_dtype(dt, [&](auto t) {
@@ -144,9 +146,15 @@ int norm_rope(const void *x, const void *dout, bool bwd, int64_t M, int64_t head
         constexpr int DT = decltype(t)::value;
         auto form = [&](auto b, auto r, auto h) {
             constexpr bool B = decltype(b)::value, R = decltype(r)::value, H = decltype(h)::value;
-            if (upt == 1) e = launch_norm_rope<DT, B, R, H, 1>(a, threads, call, st);
-            else if (upt == 4) e = launch_norm_rope<DT, B, R, H, 4>(a, threads, call, st);
-            else if constexpr (!B) e = launch_norm_rope<DT, B, R, H, 2>(a, threads, call, st);
+            if constexpr (B && DT != DT_F32)
+                if (w32 && weight) {
+                    e = upt == 1 ? launch_norm_rope<DT, B, R, H, 1, true>(a, threads, call, st)
+                                 : launch_norm_rope<DT, B, R, H, 4, true>(a, threads, call, st);
+                    return;
+                }
+            if (upt == 1) e = launch_norm_rope<DT, B, R, H, 1, false>(a, threads, call, st);
+            else if (upt == 4) e = launch_norm_rope<DT, B, R, H, 4, false>(a, threads, call, st);
+            else if constexpr (!B) e = launch_norm_rope<DT, B, R, H, 2, false>(a, threads, call, st);
         };
         auto dir = [&](auto b) {
             if (!rope) form(b, std::false_type{}, std::false_type{});

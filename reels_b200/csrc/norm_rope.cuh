@@ -43,7 +43,8 @@ struct NrDivide {
 struct NormRopeArgs {
     const void *x;
     const void *dout;     // backward only
-    const void *weight;   // [C], nullable
+    const void *weight;   // [C], nullable, of x's type or (w32) fp32
+    int w32;
     void *out;            // y, or dx
     const float2 *table;  // (cos, sin): axis after axis, [size][pairs]
     const int *pos;       // [M][3], nullable: raster order of the grid
@@ -175,15 +176,17 @@ __device__ __forceinline__ float2 nr_block_sum(float2 v, float2 *buf) {
 constexpr int NR_THREADS = 512;  // at most
 constexpr int NR_STAGES = 4;     // at most
 // Shared memory: stages of rows, the weight (forward as fp32, which spares
-// conversions; backward as it is, which leaves room for another block), angles
-// of three rows.
-__host__ __device__ constexpr int nr_smem_bytes(int C, int elem, bool bwd, int stages, int D) {
-    return stages * C * elem * (bwd ? 2 : 1) + C * (bwd ? elem : 4) + 3 * (D / 2) * 8;
+// conversions; backward as it is, which for 16-bit types leaves room for another
+// block), angles of three rows.
+__host__ __device__ constexpr int nr_smem_bytes(int C, int elem, bool bwd, bool w32, int stages, int D) {
+    return stages * C * elem * (bwd ? 2 : 1) + C * (bwd && !w32 ? elem : 4) + 3 * (D / 2) * 8;
 }
 
-template <int DT, bool BWD, bool ROPE, bool HALF, int UPT>
+// W32: backward with an fp32 weight beside 16-bit rows.
+template <int DT, bool BWD, bool ROPE, bool HALF, int UPT, bool W32>
 __global__ void __launch_bounds__(UPT == 1 ? 512 : 256, UPT == 1 ? 2 : UPT == 2 ? 3 : 1) norm_rope_kernel(const NormRopeArgs a, const int stages) {
     using T = typename Elem<DT>::T;
+    constexpr bool PLANES = !BWD || W32;  // the weight's form in shared memory
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ float2 buf[2][NR_THREADS / 32];
     __shared__ uint64_t full[NR_STAGES];
@@ -192,7 +195,7 @@ __global__ void __launch_bounds__(UPT == 1 ? 512 : 256, UPT == 1 ? 2 : UPT == 2 
     // fp32 as two planes, the first and second four of every eight features,
     // so that a warp's 16-byte reads meet no bank twice
     uint8_t *const weight = ring + stages * slot_bytes;
-    float2 *const turn = reinterpret_cast<float2 *>(weight + a.C * (BWD ? (int)sizeof(T) : 4));
+    float2 *const turn = reinterpret_cast<float2 *>(weight + a.C * (PLANES ? 4 : (int)sizeof(T)));
     volatile int *const abort = &abort_flag;
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) mbar_init(&full[s], 1);
@@ -215,8 +218,9 @@ __global__ void __launch_bounds__(UPT == 1 ? 512 : 256, UPT == 1 ? 2 : UPT == 2 
         F2 w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = F2(1.0f, 1.0f);
-        if (a.weight) nr_read_global<DT>(reinterpret_cast<const T *>(a.weight) + 8 * i, w);
-        if (BWD) {
+        if (a.weight && a.w32) nr_read_global<DT_F32>(reinterpret_cast<const float *>(a.weight) + 8 * i, w);
+        else if (a.weight) nr_read_global<DT>(reinterpret_cast<const T *>(a.weight) + 8 * i, w);
+        if (!PLANES) {
             nr_write<DT>(reinterpret_cast<T *>(weight) + 8 * i, w);
         } else {
             const float2 p = w[0].get(), q = w[1].get(), u = w[2].get(), v = w[3].get();
@@ -237,7 +241,7 @@ __global__ void __launch_bounds__(UPT == 1 ? 512 : 256, UPT == 1 ? 2 : UPT == 2 
     };
     auto weigh = [&](int k, F2 (&lo)[4], F2 (&hi)[4]) {
         F2 wl[4], wh[4];
-        if (BWD) {
+        if (!PLANES) {
             read(reinterpret_cast<const T *>(weight), k, wl, wh);
         } else {
             const float4 *const w = reinterpret_cast<const float4 *>(weight) + feat[k] / 8;
@@ -407,7 +411,7 @@ __global__ void __launch_bounds__(256) norm_rope_any_kernel(const NormRopeArgs a
                 cs = __ldcg(a.table + base + t.p[ax] * a.pairs[ax]);
             }
         };
-        auto w_of = [&](int f) { return a.weight ? load_act(a.weight, f, DT) : 1.0f; };
+        auto w_of = [&](int f) { return a.weight ? load_act(a.weight, f, a.w32 ? DT_F32 : DT) : 1.0f; };
         float2 sum = make_float2(0.0f, 0.0f);
         for (int i = threadIdx.x; i < a.C / step; i += blockDim.x) {
             int f0, f1;

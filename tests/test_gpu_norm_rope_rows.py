@@ -1,5 +1,6 @@
 """GPU parity of the q/k norm with rotary positions and of its pullback for
-rows of very small values, against plain 64-bit arithmetic.
+rows of very small values and weights of another type than the rows, against
+plain 64-bit arithmetic.
 
 Bound per element: u |y| for the output's rounding (u half a step of the
 type) and g = (C + 32) fp32 steps of the magnitudes that enter it: |n| of both
@@ -79,3 +80,29 @@ def test_rows_of_very_small_values(torch, dtype, C, heads, rotated):
     dx = rms_norm_rope_backward(x, dout, heads, w, rope, 0.0)
     assert bool(torch.isfinite(dx.float()).all())
     _check(torch, x, dout, w, y, dx, 0.0, cs, heads, False)
+
+
+@pytest.mark.parametrize("x_type,w_type", [(BF, FL), (HF, FL), (BF, HF), (FL, BF), (HF, "float64")])
+@pytest.mark.parametrize("C,heads,T", [(512, 4, 700), (10240, 80, 300), (100, 5, 9)])
+@pytest.mark.parametrize("rotated", [0, 1, 2])
+def test_a_weight_of_another_type_keeps_its_bits(torch, x_type, w_type, C, heads, T, rotated):
+    """The weight enters in fp32, whatever x is: nothing of it is rounded to x's type."""
+    from reels_b200 import RMSNormRopeFunction, check_device_status, rms_norm_rope, rope_table
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn((T, C), generator=gen, device="cuda").to(getattr(torch, x_type)).requires_grad_(True)
+    dout = torch.randn((T, C), generator=gen, device="cuda").to(x.dtype)
+    # quarters of x's step next to 1, where w's type holds them: rounding would lose them
+    step = torch.finfo(x.dtype).eps / 4
+    w = (1 + step * (1 + torch.randint(0, 3, (C,), generator=gen, device="cuda"))).to(getattr(torch, w_type))
+    rope = rope_table(C // heads, (T,), (C // heads,), interleaved=rotated == 1) if rotated else None
+    at = torch.arange(T, device="cuda")
+    cs = _angles(torch, rope, (at,), at >= 0) if rotated else None
+    y = RMSNormRopeFunction.apply(x, heads, w, rope)
+    y.backward(dout)
+    check_device_status()
+    x, dx = x.detach(), x.grad
+    assert torch.equal(y.detach(), rms_norm_rope(x, heads, w, rope))
+    assert y.dtype == x.dtype and dx.dtype == x.dtype
+    # against the same weight in 64 bits: rounded to x's type it would be off by up to half a step,
+    # which the bound allows for the output's rounding alone
+    _check(torch, x, dout, w, y.detach(), dx, 1e-6, cs, heads, rotated == 2)
