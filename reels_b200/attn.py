@@ -2,10 +2,10 @@
 output projection: the norm of q and k with the video's rotary positions, and
 softmax attention, forward and backward.
 
-Activations are tokens-first like everywhere in this package.  The functions
-take what the projections return, ``(batch, tokens, heads * head_dim)``, or
-views of it by head, ``(batch, tokens, heads, head_dim)``; parts of a fused
-q/k/v projection are read in place.  All arithmetic runs in
+Activations are tokens-first like everywhere in this package.  The norm takes
+what the projections return, ``(batch, tokens, heads * head_dim)``; attention
+takes views of it by head, ``(batch, tokens, heads, head_dim)``, and reads
+parts of a fused q/k/v projection in place.  All arithmetic runs in
 libreels_lowvram.so on the GPU; sums, softmax statistics and norms are fp32
 and every output is rounded once.
 """
@@ -104,6 +104,10 @@ def _norm_rope_args(x, heads, weight, rope, tokens_per_sample, positions):
     heads = int(heads)
     if heads <= 0 or C == 0 or C % heads:
         raise ValueError("the features must be heads * head_dim")
+    # (a weight has an entry for each feature, a table's axes sum to head_dim: they tell the two apart)
+    if x.dim() == 4 and x.shape[-2] == heads > 1 and weight is None and rope is None and tokens_per_sample is None:
+        raise ValueError("x looks like a view by head, but the norm spans all heads: pass (..., tokens, heads * "
+                         "head_dim), or tokens_per_sample if these are tokens")
     xf = x if x.is_contiguous() else x.contiguous()
     M = x.numel() // C
     w, dt = weight, _dt(x.dtype)
@@ -147,7 +151,8 @@ def rms_norm_rope(x: torch.Tensor, heads: int, weight: Optional[torch.Tensor] = 
                   rope: Optional[RopeTable] = None, epsilon: float = 1e-6, tokens_per_sample: Optional[int] = None,
                   positions: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``rotate(x / sqrt(mean(x ** 2) + epsilon) * weight)`` in one pass per
-    token, the norm over all heads of ``x`` (..., tokens, heads * head_dim).
+    token, the norm over all heads of ``x`` (..., tokens, heads * head_dim);
+    a view by head is flattened first (``x.flatten(-2)``).
 
     ``weight`` may be of another type than x: it enters in fp32.
     ``rope=None`` is the norm alone (the cross-attention's q and k).  Tokens

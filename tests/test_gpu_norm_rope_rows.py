@@ -106,3 +106,17 @@ def test_a_weight_of_another_type_keeps_its_bits(torch, x_type, w_type, C, heads
     # against the same weight in 64 bits: rounded to x's type it would be off by up to half a step,
     # which the bound allows for the output's rounding alone
     _check(torch, x, dout, w, y.detach(), dx, 1e-6, cs, heads, rotated == 2)
+
+
+def test_a_view_by_head_is_not_normed_per_head(torch):
+    """The norm spans all heads: a view by head, which shows only one head as
+    its last dimension, is refused where nothing else tells it from tokens."""
+    from reels_b200 import rms_norm_rope, rms_norm_rope_backward
+    x = torch.randn((2, 6, 8, 64), device="cuda").bfloat16()
+    for call in (lambda: rms_norm_rope(x, 8), lambda: rms_norm_rope_backward(x, x, 8)):
+        with pytest.raises(ValueError, match="view by head"):
+            call()
+    want = rms_norm_rope(x.flatten(-2), 8)
+    assert want.shape == (2, 6, 512)
+    # 8 tokens of 64 features in 8 heads, said so
+    assert torch.equal(rms_norm_rope(x, 8, tokens_per_sample=8), rms_norm_rope(x.view(12, 8, 64), 8).view(x.shape))
