@@ -71,8 +71,9 @@ __device__ __forceinline__ AttnUnit attn_unit(const AttnArgs &a, long long unit)
     w.hk = (int)((unsigned)w.h / (unsigned)(a.H / a.HK));
     w.tiles = a.Sq - w.q0 > AT_TILE ? 2 : 1;
     const int len = attn_keys(a, w.b);
-    w.k0 = min(len, w.split * a.split_keys);
-    w.kn = min(len, w.k0 + a.split_keys) - w.k0;
+    int end;
+    w.k0 = attn_split(a, len, w.split, end);
+    w.kn = end - w.k0;
     w.nk = (w.kn + AT_TILE - 1) / AT_TILE;
     return w;
 }

@@ -56,6 +56,14 @@ __device__ __forceinline__ int attn_keys(const AttnArgs &a, int b) {
     return n < 0 ? 0 : (n < a.Sk ? n : a.Sk);
 }
 
+// The first key of a split and the end of its keys, of `len` (splits times
+// split_keys may lie past 32 bits).
+__device__ __forceinline__ int attn_split(const AttnArgs &a, int len, int split, int &end) {
+    const int begin = (int)min((long long)len, (long long)split * a.split_keys);
+    end = begin + min(len - begin, a.split_keys);
+    return begin;
+}
+
 // T rows of D elements into dst[T][DP + 4], rows from `n` on and features
 // from D on as zeros.  fp32 rows that allow it in 16-byte pieces.
 template <int DT, int DP, int T>
@@ -143,7 +151,8 @@ __global__ void __launch_bounds__(AS_THREADS) attn_simt_fwd_kernel(const AttnArg
     const int tiles = (a.Sq + T - 1) / T, bh = (int)(blockIdx.x / tiles);
     const int q0 = (int)(blockIdx.x % tiles) * T, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.HK);
     const int len = attn_keys(a, b);
-    const int k_begin = min(len, (int)blockIdx.y * a.split_keys), k_end = min(len, k_begin + a.split_keys);
+    int k_end;
+    const int k_begin = attn_split(a, len, (int)blockIdx.y, k_end);
     as_load<DT, DP, T>(Q, a.q, b * a.qs[0] + q0 * a.qs[1] + h * a.qs[2], a.qs[1], a.Sq - q0, a.D);
     float m[N], l[N] = {}, o[N][DP / 64][4] = {};
 #pragma unroll
@@ -233,7 +242,8 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a) {
     const int lane = threadIdx.x & 31, sub = lane % G, grp = threadIdx.x / G;
     const int b = blockIdx.x / a.HK, hk = blockIdx.x % a.HK, group = a.H / a.HK, rows = a.Sq * group;
     const int len = attn_keys(a, b);
-    const int k_begin = min(len, (int)blockIdx.y * a.split_keys), k_end = min(len, k_begin + a.split_keys);
+    int k_end;
+    const int k_begin = attn_split(a, len, (int)blockIdx.y, k_end);
     const bool live = 8 * sub < a.D;
     float q[R][8], acc[R][8] = {}, m[R], l[R] = {};
 #pragma unroll
@@ -538,7 +548,7 @@ __global__ void __launch_bounds__(1024) attn_range_kernel(const AttnArgs a, cons
 #pragma unroll 8
     for (long long i = threadIdx.x; i < rows; i += 1024) top.x = fmaxf(top.x, __ldcg(n + i));
 #pragma unroll 8
-    for (int i = threadIdx.x; i < a.Sk; i += 1024) top.y = fmaxf(top.y, __ldcg(v + i));
+    for (long long i = threadIdx.x; i < a.Sk; i += 1024) top.y = fmaxf(top.y, __ldcg(v + i));
 #pragma unroll
     for (int w = 16; w > 0; w >>= 1) {
         top.x = fmaxf(top.x, __shfl_xor_sync(0xffffffffu, top.x, w));

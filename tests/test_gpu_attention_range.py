@@ -109,3 +109,14 @@ def test_fp16_gradient_of_few_queries_over_many_keys(torch, reels):
             end.synchronize()
             times[dtype] = min(times.get(dtype, math.inf), start.elapsed_time(end))
     assert times[torch.float16] <= 1.5 * times[torch.bfloat16], times
+
+
+def test_the_last_of_two_billion_keys(torch, reels):
+    """Key splits whose lengths add up to more than 32 bits: the last one counts too."""
+    Sk = 2 ** 31 - 257
+    q = torch.full((1, 1, 1, 1), 0.5, device="cuda")
+    k = torch.full((1, 1, 1, 1), 2.0, device="cuda").expand(1, Sk, 1, 1)
+    out, lse = reels.attention(q, k, k, scale=1.0, return_lse=True)
+    # equal scores of 1: sums of whole numbers below 2^24 in a split, then 592 of them to fp32's rounding
+    assert float(out) == pytest.approx(2.0, rel=1e-5)
+    assert float(lse) == pytest.approx(1.0 + math.log(Sk), rel=1e-6)
