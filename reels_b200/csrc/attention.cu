@@ -217,13 +217,15 @@ AttnPlan plan_attention(const reels_attn_shape &s, int dt, const void *q, const 
     // Forward: few rows leave SMs idle, so the keys are split over them and
     // joined; a split keeps at least four tiles of keys (two on the CUDA cores).
     // Blocks beside each other on an SM: 1 of the tensor-core kernel, 2 of the
-    // few-row kernel, 4 others.
+    // few-row kernel with one or two rows, 1 with more (their registers; planned
+    // for two, the splits ran one behind the other: 8 rows over 32760 keys of 12
+    // heads 104 us against 96, 4 rows 86.5 against 82.3), 4 others.
     if (s.head_dim <= 128 && ceil_div(s.q_tokens, 64) * s.batch * s.heads >= 2 * kPlanSms) p.tile = 64;
     const int tile = p.few ? 64 : p.tc ? AT_TILE : p.tile;
     const int64_t rows = p.few ? (int64_t)s.batch * s.kv_heads
                                : ceil_div(s.q_tokens, p.tc ? 2 * AT_TILE : p.tile) * s.batch * s.heads;
     const int64_t tiles = std::max<int64_t>(1, ceil_div(s.k_tokens, tile));
-    int64_t want = rows > 0 ? std::min<int64_t>((p.few ? 2 : p.tc ? 1 : 4) * kPlanSms / rows, tiles / (p.tc ? 4 : 2)) : 1;
+    int64_t want = rows > 0 ? std::min<int64_t>((p.few == 1 || p.few == 2 ? 2 : p.tc ? 1 : 4) * kPlanSms / rows, tiles / (p.tc ? 4 : 2)) : 1;
     want = std::max<int64_t>(1, std::min<int64_t>(want, 1024));
     const int64_t per = ceil_div(tiles, want);
     p.splits = (int)ceil_div(tiles, per);
