@@ -1,6 +1,7 @@
-"""GPU parity of the q/k norm with rotary positions and of its pullback for
-rows of very small values and weights of another type than the rows, against
-plain 64-bit arithmetic.
+"""GPU parity of the q/k norm with rotary positions and of its pullback where
+a block of the vector form works through many rows, for rows of very small
+values and for weights of another type than the rows, against plain 64-bit
+arithmetic.
 
 Bound per element: u |y| for the output's rounding (u half a step of the
 type) and g = (C + 32) fp32 steps of the magnitudes that enter it: |n| of both
@@ -60,6 +61,46 @@ def _angles(torch, rope, coords, on):
         at += size * dim // 2
     still = torch.tensor([1.0, 0.0], dtype=torch.float64, device="cuda")
     return torch.where(on[:, None, None], torch.cat(parts, 1), still)
+
+
+@pytest.mark.parametrize("B,T,heads,D,sizes,half,dtype,given", [
+    (1, 7001, 12, 128, (7, 20, 50), False, BF, False),   # one token of padding
+    (3, 4003, 8, 64, (10, 20, 20), True, HF, False),     # samples begin inside a block's walk
+    (7, 1003, 5, 64, (4, 10, 25), False, FL, False),     # padding in every sample
+    (2, 2500, 3, 16, (25, 10, 10), True, FL, True),      # narrow rows, given positions
+    (1, 3001, 128, 128, (3, 20, 50), True, BF, False),   # the widest rows
+    (1, 2203, 72, 128, (2, 20, 50), False, FL, True),    # wide, fp32 (the pullback's scalar form)
+    (11, 509, 40, 128, (5, 10, 10), False, HF, True),
+    (1, 6007, 24, 64, None, False, BF, False),           # the norm alone
+    (2, 3001, 100, 128, None, False, HF, False),
+])
+def test_many_rows_a_block(torch, B, T, heads, D, sizes, half, dtype, given):
+    from reels_b200 import check_device_status, rms_norm_rope, rms_norm_rope_backward, rope_table
+    gen = torch.Generator(device="cuda").manual_seed(T)
+    dt, C, eps = getattr(torch, dtype), heads * D, 1e-6
+    x = (1.7 * torch.randn((B, T, C), generator=gen, device="cuda")).to(dt)
+    dout = torch.randn((B, T, C), generator=gen, device="cuda").to(dt)
+    w = (1 + 0.2 * torch.randn(C, generator=gen, device="cuda")).to(dt)
+    rope = pos = cs = None
+    if sizes is not None:
+        rope = rope_table(D, sizes, interleaved=not half)
+        i = torch.arange(T, device="cuda").repeat(B)
+        if given:
+            pos = torch.stack([torch.randint(-1 if n == 0 else 0, s, (B, T), generator=gen, device="cuda")
+                               for n, s in enumerate(sizes)], -1)
+            coords = pos.view(-1, 3).unbind(1)
+            on = coords[0] >= 0
+        else:
+            coords = (i // (sizes[1] * sizes[2]), i // sizes[2] % sizes[1], i % sizes[2])
+            on = coords[0] < sizes[0]
+        cs = _angles(torch, rope, coords, on)
+    y = rms_norm_rope(x, heads, w, rope, eps, positions=pos)
+    dx = rms_norm_rope_backward(x, dout, heads, w, rope, eps, positions=pos)
+    check_device_status()
+    flat = lambda t: t.view(-1, C)
+    for part in torch.arange(B * T, device="cuda").split(4096):  # the 64-bit values of all rows would take many GB
+        _check(torch, flat(x)[part], flat(dout)[part], w, flat(y)[part], flat(dx)[part], eps,
+               None if cs is None else cs[part], heads, half)
 
 
 @pytest.mark.parametrize("dtype", [BF, FL])
