@@ -18,7 +18,12 @@
 // P and dS enter their products in the tensors' 16-bit type; that rounding (half
 // a step, independent from term to term) and the result's own make an error of
 // sqrt(2) times the latter.  delta is taken from the forward's rounded out, as
-// the caller has it, in fp32.
+// the caller has it, in fp32, which makes it 1.5 for dQ.  (dS in two parts, what
+// its rounding leaves as a second operand: 1.1, and 12% more time for forward and
+// backward of 2 x 6144 tokens, 32 heads of 128.)
+//
+// Registers: 216 a thread for the elementwise warps; beyond them the compiler
+// keeps 20 to 40 bytes a thread of dK, dV and of dQ at heads of 128 in local memory.
 //
 // In both, the second product's operand (P', dS', dS) is written by the CUDA
 // cores into tensor memory over the scores it came from, which the issuing

@@ -13,9 +13,9 @@
 //
 // Bound: HBM, 2 passes of the row forward (x, y), 3 backward (x, dout, dx),
 // with issue slots next to it on short rows.  Measured, bf16: 32760 x 1536
-// forward 44 us (4.6 TB/s), 8190 x 5120 forward 32.5 us (5.2 TB/s) and backward
-// 48.6 (5.2); fp16, 12288 x 4096: 38.8 us (5.2) and 61.9 (4.9).  A copy runs at
-// 6.5 TB/s.
+// forward 43 us (4.6 TB/s) and backward 56 (5.4), 8190 x 5120 forward 33 us (5.1
+// TB/s) and backward 46 (5.4); fp16, 12288 x 4096: 40 us (5.1) and 59 (5.1); fp32,
+// 32760 x 1536: 75 us (5.4) and 101 (6.0).  A copy runs at 6.5 TB/s.
 #pragma once
 #include "common.cuh"
 
